@@ -1,4 +1,4 @@
-"""ctypes binding of libaimet_amd.so (the C ABI declared in include/aimet_amd.h).
+"""ctypes binding of libaimet_amd.so (the C ABI declared in include/aimet_amd.h and include/aimet_amd_serving.h).
 
 The library is the only compute path of this package: if it is missing, or a tensor does not live on a HIP device,
 the callers raise -- there is no CPU or eager-PyTorch fallback.
@@ -121,6 +121,34 @@ class SlotsFinalizeItem(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """ahq_kv_cache"""
+
+    _fields_ = [("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("capacity", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("block", ctypes.c_int32), ("k_codes", ctypes.c_void_p),
+                ("v_codes", ctypes.c_void_p), ("k_amax", ctypes.c_void_p), ("v_amax", ctypes.c_void_p)]
+
+
+class KvTokens(ctypes.Structure):
+    """ahq_kv_tokens"""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("tokens", ctypes.c_int32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("stride_batch", ctypes.c_int64 * 2), ("stride_head", ctypes.c_int64 * 2),
+                ("stride_token", ctypes.c_int64 * 2), ("start", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("start_all", ctypes.c_int32), ("count_all", ctypes.c_int32)]
+
+
+class KvQueries(ctypes.Structure):
+    """ahq_kv_queries"""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("query_heads", ctypes.c_int32), ("queries", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("q_stride_batch", ctypes.c_int64), ("q_stride_head", ctypes.c_int64), ("q_stride_query", ctypes.c_int64),
+                ("out_stride_batch", ctypes.c_int64), ("out_stride_head", ctypes.c_int64),
+                ("out_stride_query", ctypes.c_int64), ("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("length_all", ctypes.c_int32), ("count_all", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 DLQ_PDF_SIZE = 1536
 
 
@@ -215,6 +243,19 @@ _SIGNATURES = {
                                              ctypes.c_int32, _P, _P, _P, ctypes.c_size_t, _P]),
 }
 
+# every symbol include/aimet_amd_serving.h declares
+_SERVING_SIGNATURES = {
+    "ahq_int4_packed_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    "ahq_int4_pack": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P]),
+    "ahq_int4_linear": (ctypes.c_int, [ctypes.c_int32, _P, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
+                                       ctypes.c_int64, ctypes.c_int64, _P, _P, ctypes.c_float, _P, _P, ctypes.c_int64,
+                                       _P]),
+    "ahq_kv_append": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.POINTER(KvTokens), _P]),
+    "ahq_kv_dequantize": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.c_int32, ctypes.c_int32, _P, _P, _P]),
+    "ahq_kv_attend_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(KvCache), ctypes.POINTER(KvQueries)]),
+    "ahq_kv_attend": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.POINTER(KvQueries), _P, ctypes.c_size_t, _P]),
+}
+
 
 def exported_symbols() -> Sequence[str]:
     return tuple(_SIGNATURES)
@@ -234,7 +275,7 @@ def load() -> ctypes.CDLL:
         lib = ctypes.CDLL(LIB_PATH)
     except OSError as e:
         raise HipLibraryError(f"cannot load {LIB_PATH}: {e}") from e
-    for name, (res, args) in _SIGNATURES.items():
+    for name, (res, args) in (*_SIGNATURES.items(), *_SERVING_SIGNATURES.items()):
         try:
             fn = getattr(lib, name)
         except AttributeError as e:

@@ -1,0 +1,321 @@
+// Linear layers on packed 4-bit weights.
+//
+//   y[m, n] = sum_g s[n, g] * ( sum_{k in g} x[m, k] * (u[n, k] + z[n, g]) ) + b[n]
+//
+// u are the codes counted from the lower end of their grid (0..15), z = offset + qmin + zero-point shift, s the float32
+// scale of the group.  The inner sums run on the matrix cores with both factors exact: u is a whole number that
+// bfloat16 and float16 hold, x is used as it is (float32 as a sum of three bfloat16 parts), the accumulators are
+// float32.  z is taken out of the inner sum as z * sum(x), where sum(x) is one more matrix instruction against ones; it
+// enters as the starting value of the group's accumulator.  The scale multiplies the finished group sum in float32, so
+// the only rounding to fewer bits is the one of y.  An infinite x makes its row NaN (0 * inf and inf - inf both occur).
+//
+// Weight layout: tiles of 16 rows x 128 columns, 1 KB each, along a row of tiles first.  Lane 16 c + i of the wave that
+// owns a tile finds its 16 bytes at 16 * lane: word j holds row i, columns 32 j + 8 c + e, e = 0..3 in the low and 4..7
+// in the high halves of bytes 0..3.  A code in the low half of a zero byte is the float8 (e4m3) number u * 2^-9, normal
+// or not, so v_cvt_scalef32_pk_*_fp8 with the scale 512 turns two codes into two exact 16-bit floats: 7 vector
+// instructions for 8 codes.
+
+#include "../../include/aimet_amd_serving.h"
+#include "ahq_host.h"
+#include "mma.h"
+
+namespace ahq {
+
+constexpr int kTileRows = 16;
+constexpr int kTileCols = 128;
+constexpr int kTileBytes = 1024;
+
+// -------------------------------------------------------------------------------------------------------- fragments --
+template <typename T> struct Int4Traits;
+template <> struct Int4Traits<bf16_t> { typedef bf16x8 Frag; static constexpr int kParts = 1; };
+template <> struct Int4Traits<f16_t> { typedef f16x8 Frag; static constexpr int kParts = 1; };
+template <> struct Int4Traits<float> { typedef bf16x8 Frag; static constexpr int kParts = 3; };
+
+template <typename Frag> __device__ __forceinline__ Frag decode_codes(uint32_t w);
+template <> __device__ __forceinline__ bf16x8 decode_codes<bf16x8>(uint32_t w) {
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    union { bf16x2 h[4]; bf16x8 v; } r;
+    r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false);
+    r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
+    r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false);
+    r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+    return r.v;
+}
+template <> __device__ __forceinline__ f16x8 decode_codes<f16x8>(uint32_t w) {
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    union { f16x2 h[4]; f16x8 v; } r;
+    r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false);
+    r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
+    r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false);
+    r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
+    return r.v;
+}
+
+template <typename Frag> __device__ __forceinline__ Frag ones_fragment();
+template <> __device__ __forceinline__ bf16x8 ones_fragment<bf16x8>() {
+    const uint32_t w = 0x3f803f80u;
+    return __builtin_bit_cast(bf16x8, u32x4_t{w, w, w, w});
+}
+template <> __device__ __forceinline__ f16x8 ones_fragment<f16x8>() {
+    const uint32_t w = 0x3c003c00u;
+    return __builtin_bit_cast(f16x8, u32x4_t{w, w, w, w});
+}
+
+// Eight activations from column k on, as matrix operands; columns from `cols` on count as zero.  `vec`: rows start on
+// 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ void load_activations(const T* __restrict__ row, int64_t k, int64_t cols, bool vec,
+                                                 typename Int4Traits<T>::Frag* out) {
+    if constexpr (sizeof(T) == 2) {
+        u32x4_t w = {0u, 0u, 0u, 0u};
+        if (vec && k + 8 <= cols) {
+            w = *reinterpret_cast<const u32x4_t*>(row + k);
+        } else if (k < cols) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < cols) w[e / 2] |= (uint32_t)row[k + e].bits << (16 * (e & 1));
+        }
+        out[0] = __builtin_bit_cast(typename Int4Traits<T>::Frag, w);
+    } else {
+        float v[8];
+        if (vec && k + 8 <= cols) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + k), b = *reinterpret_cast<const f32x4*>(row + k + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < cols ? row[k + e] : 0.0f;
+        }
+        split_bf16<3>(v, out);
+    }
+}
+
+struct Int4Args {
+    const void* x;
+    const uint8_t* w;
+    const float* scale;   // [groups][rows padded to 16]
+    const int8_t* zero;   // same layout, or null: z = zero_const everywhere
+    const void* bias;
+    void* y;
+    int64_t m, n, k, ldx, ldy;
+    int64_t tiles;          // 128-column tiles of a row
+    int64_t npad;           // rows padded to 16
+    int64_t groups;
+    uint64_t fold_inverse;  // ceil(2^32 / folds per group)
+    float zero_const;
+    int32_t vec_x, vec_y;
+};
+
+// ------------------------------------------------------------------------------------------------- few activations --
+// A workgroup owns 16 * NT rows of the weight and 16 * MT activations; its waves take the 128-column tiles in turn and
+// their sums are added through LDS in wave order.  FOLD: matrix instructions (of 32 columns) whose sum shares a scale.
+template <typename T, int FOLD, int MT, int NT>
+__global__ __launch_bounds__(8 * kWave) void int4_linear_kernel(Int4Args a) {
+    typedef typename Int4Traits<T>::Frag Frag;
+    constexpr int P = Int4Traits<T>::kParts;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const int i = lane & 15, c = lane >> 4;
+    const int64_t tile0 = (int64_t)blockIdx.x * NT;
+    const int64_t ntiles = a.npad / kTileRows;
+    const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+    const Frag ones = ones_fragment<Frag>();
+    const T* x = static_cast<const T*>(a.x);
+
+    const u32x4_t* wp[NT];
+    int64_t row4[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int64_t t = tile0 + nt < ntiles ? tile0 + nt : ntiles - 1;
+        wp[nt] = reinterpret_cast<const u32x4_t*>(a.w + t * a.tiles * kTileBytes) + lane;
+        row4[nt] = t * kTileRows + 4 * c;
+    }
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    for (int64_t kt = wave; kt < a.tiles; kt += waves) {
+        u32x4_t w[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) w[nt] = wp[nt][kt * (kTileBytes / 16)];
+#pragma unroll
+        for (int f = 0; f < 4 / FOLD; ++f) {
+            Frag xf[FOLD][MT][P];
+            f32x4 sum[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int64_t m = m0 + 16 * mt + i;
+                const bool live = m < a.m;
+                const T* row = x + (live ? m : 0) * a.ldx;
+                sum[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < FOLD; ++j) {
+                    const int64_t k = kt * kTileCols + 32 * (f * FOLD + j) + 8 * c;
+                    load_activations<T>(row, k, live ? a.k : 0, a.vec_x, xf[j][mt]);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) sum[mt] = mma(ones, xf[j][mt][p], sum[mt]);
+                }
+            }
+            const uint64_t fold = (uint64_t)(kt * (4 / FOLD) + f);
+            int64_t g = (int64_t)((fold * a.fold_inverse) >> 32);
+            g = g < a.groups ? g : a.groups - 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const f32x4 s = *reinterpret_cast<const f32x4*>(a.scale + g * a.npad + row4[nt]);
+                f32x4 z = {a.zero_const, a.zero_const, a.zero_const, a.zero_const};
+                if (a.zero) {
+                    const uint32_t b = *reinterpret_cast<const uint32_t*>(a.zero + g * a.npad + row4[nt]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[r] += (float)(int8_t)(b >> (8 * r));
+                }
+                Frag wf[FOLD];
+#pragma unroll
+                for (int j = 0; j < FOLD; ++j) wf[j] = decode_codes<Frag>(w[nt][f * FOLD + j]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    f32x4 part;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) part[r] = z[r] * sum[mt][r];
+#pragma unroll
+                    for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) part = mma(wf[j], xf[j][mt][p], part);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[nt][mt][r] = __builtin_fmaf(s[r], part[r], acc[nt][mt][r]);
+                }
+            }
+        }
+    }
+
+    extern __shared__ f32x4 red[];  // [waves][NT * MT][64]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) red[(wave * NT * MT + nt * MT + mt) * kWave + lane] = acc[nt][mt];
+    __syncthreads();
+    for (int o = threadIdx.x; o < NT * MT * kWave; o += blockDim.x) {
+        f32x4 v = red[o];
+        for (int w = 1; w < waves; ++w) {
+            const f32x4 u = red[w * NT * MT * kWave + o];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += u[r];
+        }
+        const int l = o & (kWave - 1), q = o / kWave;
+        const int64_t n = (tile0 + q / MT) * kTileRows + 4 * (l >> 4), m = m0 + 16 * (q % MT) + (l & 15);
+        if (m >= a.m || n >= a.n) continue;
+        T* y = static_cast<T*>(a.y) + m * a.ldy + n;
+        const T* bias = static_cast<const T*>(a.bias);
+        Pack<T, 4> out;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float b = bias && n + r < a.n ? load_f32(bias[n + r]) : 0.0f;
+            out.v[r] = store_cast<T>(v[r] + b);
+        }
+        if (a.vec_y && n + 4 <= a.n) {
+            store_pack<T, 4>(y, out);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n + r < a.n) y[r] = out.v[r];
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------- packing --
+__global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restrict__ codes, int64_t n, int64_t k,
+                                                           int32_t qmin, int64_t tiles, int64_t words,
+                                                           uint32_t* __restrict__ out) {
+    const int64_t id = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (id >= words) return;
+    const int j = (int)(id & 3), lane = (int)((id >> 2) & 63);
+    const int64_t tile = id >> 8;
+    const int64_t row = tile / tiles * kTileRows + (lane & 15);
+    const int64_t col = tile % tiles * kTileCols + 32 * j + 8 * (lane >> 4);
+    uint32_t w = 0;
+    if (row < n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (col + e >= k) break;
+            const uint32_t u = (uint32_t)(codes[row * k + col + e] - qmin) & 15u;
+            w |= u << (e < 4 ? 8 * e : 8 * (e - 4) + 4);
+        }
+    }
+    out[id] = w;
+}
+
+// ------------------------------------------------------------------------------------------------------------- host --
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <typename T, int FOLD>
+int launch_few(const Int4Args& a, hipStream_t stream) {
+    const int64_t ntiles = a.npad / kTileRows;
+    const int waves = a.tiles >= 16 ? 8 : a.tiles >= 4 ? 4 : 1;
+    if (a.m <= 16) {
+        int4_linear_kernel<T, FOLD, 1, 1><<<dim3((unsigned)ntiles, (unsigned)ceil_div(a.m, 16)), waves * kWave, waves * 1024, stream>>>(a);
+    } else {
+        int4_linear_kernel<T, FOLD, 2, 2><<<dim3((unsigned)ceil_div(ntiles, 2), (unsigned)ceil_div(a.m, 32)), waves * kWave, waves * 4096, stream>>>(a);
+    }
+    return check_launch("ahq_int4_linear");
+}
+
+template <typename T>
+int launch_linear(const Int4Args& a, int fold, hipStream_t stream) {
+    if (fold == 1) return launch_few<T, 1>(a, stream);
+    if (fold == 2) return launch_few<T, 2>(a, stream);
+    return launch_few<T, 4>(a, stream);
+}
+
+}  // namespace ahq
+
+extern "C" size_t ahq_int4_packed_bytes(int64_t n, int64_t k) {
+    if (n <= 0 || k <= 0 || n > (1ll << 31) || k > (1ll << 20)) return 0;
+    return (size_t)(ahq::ceil_div(n, ahq::kTileRows) * ahq::ceil_div(k, ahq::kTileCols) * ahq::kTileBytes);
+}
+
+extern "C" int ahq_int4_pack(const int8_t* codes, int64_t n, int64_t k, int32_t qmin, void* packed, void* stream) {
+    using namespace ahq;
+    if (!codes || !packed) return set_error("null argument"), AHQ_ERR_INVALID;
+    if (ahq_int4_packed_bytes(n, k) == 0) return set_error("bad weight shape"), AHQ_ERR_INVALID;
+    if (qmin < -128 || qmin > 112) return set_error("qmin outside [-128, 112]"), AHQ_ERR_INVALID;
+    if ((uintptr_t)packed % 16) return set_error("packed weights must be 16-byte aligned"), AHQ_ERR_INVALID;
+    const int64_t tiles = ceil_div(k, kTileCols), words = (int64_t)ahq_int4_packed_bytes(n, k) / 4;
+    if (ceil_div(words, kBlock) > 0x7fffffffll) return set_error("weight too large"), AHQ_ERR_UNSUPPORTED;
+    int4_pack_kernel<<<(unsigned)ceil_div(words, kBlock), kBlock, 0, static_cast<hipStream_t>(stream)>>>(
+        codes, n, k, qmin, tiles, words, static_cast<uint32_t*>(packed));
+    return check_launch("ahq_int4_pack");
+}
+
+extern "C" int ahq_int4_linear(int32_t dtype, const void* x, int64_t m, int64_t ldx, const void* packed, int64_t n,
+                               int64_t k, int64_t group, const float* scale, const int8_t* zero, float zero_const,
+                               const void* bias, void* y, int64_t ldy, void* stream) {
+    using namespace ahq;
+    if (dtype < AHQ_F32 || dtype > AHQ_BF16) return set_error("bad dtype"), AHQ_ERR_INVALID;
+    if (m < 0 || ahq_int4_packed_bytes(n, k) == 0) return set_error("bad shape"), AHQ_ERR_INVALID;
+    if (m == 0) return AHQ_OK;
+    if (!x || !packed || !scale || !y) return set_error("null argument"), AHQ_ERR_INVALID;
+    if (ldx < k || ldy < n) return set_error("row strides smaller than the rows"), AHQ_ERR_INVALID;
+    if (group <= 0 || group > k || k % group) return set_error("the group must divide the row"), AHQ_ERR_INVALID;
+    if (group != k && group % 32) return set_error("groups are multiples of 32 columns or the whole row"), AHQ_ERR_UNSUPPORTED;
+    if (((uintptr_t)packed | (uintptr_t)scale | (uintptr_t)zero) % 16)
+        return set_error("packed weights, scales and zero points must be 16-byte aligned"), AHQ_ERR_INVALID;
+    const size_t e = dtype == AHQ_F32 ? 4 : 2;
+    if (((uintptr_t)x | (uintptr_t)y | (uintptr_t)bias) % e) return set_error("misaligned tensor"), AHQ_ERR_INVALID;
+    if (m > (1ll << 30)) return set_error("too many activations"), AHQ_ERR_UNSUPPORTED;
+    Int4Args a;
+    a.x = x, a.w = static_cast<const uint8_t*>(packed), a.scale = scale, a.zero = zero, a.bias = bias, a.y = y;
+    a.m = m, a.n = n, a.k = k, a.ldx = ldx, a.ldy = ldy;
+    a.tiles = ceil_div(k, kTileCols), a.npad = ceil_div(n, kTileRows) * kTileRows, a.groups = k / group;
+    a.zero_const = zero_const;
+    // The scale is applied every 32, 64 or 128 columns: as rarely as one scale lasts (128 keeps the group sums short
+    // where a scale covers a whole row).
+    const int fold = group == k || group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;
+    const uint64_t folds = group == k ? (uint64_t)a.tiles * 4 : (uint64_t)(group / (32 * fold));
+    a.fold_inverse = ((1ull << 32) + folds - 1) / folds;
+    a.vec_x = (uintptr_t)x % 16 == 0 && (ldx * (int64_t)e) % 16 == 0;
+    a.vec_y = (uintptr_t)y % (4 * e) == 0 && ldy % 4 == 0;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == AHQ_F32) return launch_linear<float>(a, fold, s);
+    if (dtype == AHQ_F16) return launch_linear<f16_t>(a, fold, s);
+    return launch_linear<bf16_t>(a, fold, s);
+}

@@ -27,10 +27,13 @@ from torch.nn import functional as F
 
 from aimet_amd.quantization._decompose import _DecompositionError, _decompose_prequantized_tensor
 from aimet_amd.quantization._utils import concretize_block_size, patch_attr
+from aimet_amd.quantization.affine.packed import PackedWeight, packed_linear
+from aimet_amd.quantization.affine.encoding import AffineEncoding
 from aimet_amd.quantization.affine.quantizer import AffineQuantizerBase, GroupedBlockQuantizeDequantize
 from aimet_amd.quantization.base.quantizer import QuantizerBase
 
-__all__ = ["QuantizedLinear", "compute_encodings", "quantized_linears", "fold_param_quantizers", "inference_mode",
+__all__ = ["QuantizedLinear", "PackedLinear", "compute_encodings", "quantized_linears", "fold_param_quantizers",
+           "inference_mode", "pack_linears",
            "remove_input_quantizers", "remove_output_quantizers", "remove_param_quantizers",
            "remove_activation_quantizers", "remove_all_quantizers"]
 
@@ -333,6 +336,29 @@ class QuantizedLinear(nn.Linear):
             setattr(self, name, nn.Parameter(qdq, requires_grad=param.requires_grad))
             self.param_quantizers[name] = None
 
+    def pack(self) -> "PackedLinear":
+        """The inference form of this layer: its weight as 4-bit codes under the weight quantizer's encoding (or the one
+        a folded weight carries), its activation quantizers shared, its bias quantize-dequantized once.  Raises
+        where the weight has no affine encoding of at most 16 levels."""
+        from aimet_amd.quantization.tensor import QuantizedTensorBase
+
+        self._compute_param_encodings(overwrite=False)
+        wq, bq = self.param_quantizers["weight"], self.param_quantizers["bias"]
+        with torch.no_grad():
+            # the codes are those of the values the layer computes with: the quantizer's own arithmetic decides between
+            # two codes, and values that lie on the grid are read back exactly
+            weight = self.weight
+            if isinstance(wq, AffineQuantizerBase) and wq.is_initialized():
+                weight = wq(weight)
+            if not isinstance(weight, QuantizedTensorBase) or not isinstance(weight.encoding, AffineEncoding):
+                raise RuntimeError("packing needs a weight with an affine encoding")
+            weight = PackedWeight.from_encoding(weight.dequantize(), weight.encoding)
+            bias = self.bias
+            if bias is not None:
+                bias = bias if bq is None else bq(bias)
+                bias = bias.detach().as_subclass(torch.Tensor).clone()
+        return PackedLinear(weight, bias, self.input_quantizers[0], self.output_quantizers[0])
+
     @contextlib.contextmanager
     def compute_encodings(self, _verdicts=None):
         """nn/base.py:392-427: weights are calibrated on entry; activation quantizers observe their inputs and pass
@@ -355,6 +381,62 @@ class QuantizedLinear(nn.Linear):
                     continue
                 stack.enter_context(qtzr._compute_encodings(passthrough=True))  # pylint: disable=protected-access
             yield
+
+
+class PackedLinear(nn.Module):
+    """A linear layer that runs on 4-bit codes (``QuantizedLinear.pack``): quantize-dequantizes its input and output as
+    the layer it was made from, but reads a packed weight instead of quantize-dequantizing a floating-point one.
+    Inference only: nothing in it learns and ``forward`` refuses tensors that require gradients."""
+
+    def __init__(self, weight: PackedWeight, bias: Optional[torch.Tensor] = None, input_quantizer=None,
+                 output_quantizer=None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        self._packed = weight
+        self.register_buffer("weight_codes", weight.codes)
+        self.register_buffer("weight_scale", weight.scale)
+        self.register_buffer("weight_zero", weight.zero)
+        self.register_buffer("bias", bias)
+        self.input_quantizers = nn.ModuleList([input_quantizer])
+        self.output_quantizers = nn.ModuleList([output_quantizer])
+
+    @property
+    def weight(self) -> PackedWeight:
+        w = self._packed
+        if w.codes is not self.weight_codes or w.scale is not self.weight_scale or w.zero is not self.weight_zero:
+            w = self._packed = PackedWeight(self.weight_codes, self.weight_scale, self.weight_zero, w.zero_const, w.shape,
+                                            w.group)
+        return w
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:  # pylint: disable=redefined-builtin
+        iq, oq = self.input_quantizers[0], self.output_quantizers[0]
+        if iq is not None:
+            input = iq(input)
+        out = packed_linear(input, self.weight, self.bias)
+        return out if oq is None else oq(out)
+
+    def _apply(self, fn, recurse=True):
+        """Conversions to another floating-point type leave the scales in float32."""
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
+    def get_extra_state(self):
+        w = self._packed
+        return {"shape": w.shape, "group": w.group, "zero_const": w.zero_const}
+
+    def set_extra_state(self, state):
+        w = self._packed
+        if (tuple(state["shape"]), state["group"]) != (w.shape, w.group):
+            raise RuntimeError(f"a packed weight of shape {tuple(state['shape'])} and groups of {state['group']} columns "
+                               f"does not fit one of shape {w.shape} and groups of {w.group}")
+        self._packed = PackedWeight(w.codes, w.scale, w.zero, state["zero_const"], w.shape, w.group)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, group={self._packed.group}, "
+                f"bias={self.bias is not None}")
 
 
 def quantized_linears(model: nn.Module) -> Iterable[QuantizedLinear]:
@@ -570,6 +652,22 @@ def fold_param_quantizers(model: nn.Module):
     """QuantizationSimModel.fold_param_quantizers (quantsim/quantsim.py:930-960)."""
     for m in quantized_linears(model):
         m.fold_param_quantizers()
+
+
+def pack_linears(model: nn.Module) -> int:
+    """Replaces every QuantizedLinear of ``model`` whose weight has an affine encoding of at most 16 levels by its
+    packed form (QuantizedLinear.pack); returns how many.  Other layers are left as they are."""
+    count = 0
+    for parent in list(model.modules()):
+        for name, child in list(parent.named_children()):
+            if not isinstance(child, QuantizedLinear):
+                continue
+            wq = child.param_quantizers["weight"]
+            encoded = wq if wq is not None else getattr(child.weight, "encoding", None)
+            if isinstance(encoded, (AffineQuantizerBase, AffineEncoding)) and encoded.qmax - encoded.qmin <= 15:
+                setattr(parent, name, child.pack())
+                count += 1
+    return count
 
 
 def _remove_from_all(model, method: str) -> _Removed:

@@ -16,6 +16,7 @@ from torch.nn import functional as F
 
 from aimet_amd import nn as qnn
 from aimet_amd.quantization.affine import QuantizeDequantize
+from aimet_amd.quantization.kv_cache import QuantizedKVCache
 
 
 @dataclass
@@ -65,14 +66,18 @@ class Attention(nn.Module):
         self.v_proj = nn.Linear(h, h, bias=False)
         self.o_proj = nn.Linear(h, h, bias=False)
 
-    def forward(self, x, rope):
+    def forward(self, x, rope, cache=None, start=0):
         B, T, C = x.shape
         H = self.cfg.heads
         q = self.q_proj(x).view(B, T, H, C // H).transpose(1, 2)
         k = self.k_proj(x).view(B, T, H, C // H).transpose(1, 2)
         v = self.v_proj(x).view(B, T, H, C // H).transpose(1, 2)
         q, k = rotary(q, *rope), rotary(k, *rope)
-        y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        if cache is None:
+            y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        else:
+            cache.append(k, v, start)
+            y = cache.attend(q, start + T)
         return self.o_proj(y.transpose(1, 2).reshape(B, T, C))
 
 
@@ -95,8 +100,8 @@ class Block(nn.Module):
         self.post_norm = RMSNorm(cfg.hidden, cfg.eps)
         self.mlp = MLP(cfg)
 
-    def forward(self, x, rope):
-        x = x + self.attn(self.input_norm(x), rope)
+    def forward(self, x, rope, cache=None, start=0):
+        x = x + self.attn(self.input_norm(x), rope, cache, start)
         return x + self.mlp(self.post_norm(x))
 
 
@@ -117,11 +122,18 @@ class Llama(nn.Module):
                                             like.device, like.dtype)
         return self._rope[key]
 
-    def forward(self, ids):
+    def forward(self, ids, caches=None, start=0):
+        """Logits of the tokens ``ids`` [batch, tokens]; with ``caches`` (make_caches) those tokens stand at position
+        ``start`` of their sequences, behind what the caches hold, and are stored there."""
         x = self.embed(ids)
-        rope = self.rope(ids.shape[1], x)
-        for b in self.blocks:
-            x = b(x, rope)
+        if caches is None:
+            rope = self.rope(ids.shape[1], x)
+            for b in self.blocks:
+                x = b(x, rope)
+        else:
+            rope = tuple(t[:, :, start:start + ids.shape[1]] for t in self.rope(caches[0].capacity, x))
+            for b, cache in zip(self.blocks, caches):
+                x = b(x, rope, cache, start)
         return self.lm_head(self.norm(x))
 
 
@@ -150,6 +162,28 @@ def quantize(model: Llama, weight_bitwidth: int = 4, block: int = 64, act_bitwid
         return iq.to(dev), wq.to(dev), oq.to(dev)
 
     return qnn.wrap_linears(model, make)
+
+
+def make_caches(model: Llama, batch: int, capacity: int, block_tokens: int = 64):
+    """An 8-bit key/value cache for every layer."""
+    cfg = model.cfg
+    device = model.embed.weight.device
+    return [QuantizedKVCache(batch, cfg.heads, capacity, cfg.hidden // cfg.heads, block_tokens, device)
+            for _ in range(cfg.layers)]
+
+
+@torch.no_grad()
+def generate(model: Llama, ids: torch.Tensor, tokens: int, caches=None):
+    """Greedy continuation of the prompts ``ids`` [batch, prompt] by ``tokens`` tokens (the prompt in one pass, then one
+    token at a time over the 8-bit caches).  Returns [batch, prompt + tokens]."""
+    caches = make_caches(model, ids.shape[0], ids.shape[1] + tokens) if caches is None else caches
+    new, start = ids, 0
+    for _ in range(tokens):
+        logits = model(new, caches, start)
+        start += new.shape[1]
+        new = logits[:, -1:].argmax(-1)
+        ids = torch.cat([ids, new], dim=1)
+    return ids
 
 
 def calibration_batches(cfg: LlamaConfig, device, batches: int = 8, seq: int = 2048, batch: int = 1, seed: int = 1):
