@@ -121,6 +121,13 @@ class SlotsFinalizeItem(ctypes.Structure):
     ]
 
 
+class Int4Weight(ctypes.Structure):
+    """ahq_int4_weight"""
+
+    _fields_ = [("n", ctypes.c_int64), ("k", ctypes.c_int64), ("group", ctypes.c_int64), ("packed", ctypes.c_void_p),
+                ("scale", ctypes.c_void_p), ("zero", ctypes.c_void_p), ("zero_const", ctypes.c_float)]
+
+
 class KvCache(ctypes.Structure):
     """ahq_kv_cache"""
 
@@ -247,9 +254,8 @@ _SIGNATURES = {
 _SERVING_SIGNATURES = {
     "ahq_int4_packed_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     "ahq_int4_pack": (ctypes.c_int, [_P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, _P, _P]),
-    "ahq_int4_linear": (ctypes.c_int, [ctypes.c_int32, _P, ctypes.c_int64, ctypes.c_int64, _P, ctypes.c_int64,
-                                       ctypes.c_int64, ctypes.c_int64, _P, _P, ctypes.c_float, _P, _P, ctypes.c_int64,
-                                       _P]),
+    "ahq_int4_linear": (ctypes.c_int, [ctypes.POINTER(Int4Weight), ctypes.c_int32, _P, ctypes.c_int64, ctypes.c_int64, _P,
+                                       _P, ctypes.c_int64, _P]),
     "ahq_kv_append": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.POINTER(KvTokens), _P]),
     "ahq_kv_dequantize": (ctypes.c_int, [ctypes.POINTER(KvCache), ctypes.c_int32, ctypes.c_int32, _P, _P, _P]),
     "ahq_kv_attend_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(KvCache), ctypes.POINTER(KvQueries)]),

@@ -27,9 +27,10 @@ constexpr int kTileBytes = 1024;
 
 // -------------------------------------------------------------------------------------------------------- fragments --
 template <typename T> struct Int4Traits;
-template <> struct Int4Traits<bf16_t> { typedef bf16x8 Frag; static constexpr int kParts = 1; };
-template <> struct Int4Traits<f16_t> { typedef f16x8 Frag; static constexpr int kParts = 1; };
-template <> struct Int4Traits<float> { typedef bf16x8 Frag; static constexpr int kParts = 3; };
+typedef float f32x8 __attribute__((ext_vector_type(8), aligned(16)));
+template <> struct Int4Traits<bf16_t> { typedef bf16x8 Frag; typedef u32x4_t Raw; static constexpr int kParts = 1; };
+template <> struct Int4Traits<f16_t> { typedef f16x8 Frag; typedef u32x4_t Raw; static constexpr int kParts = 1; };
+template <> struct Int4Traits<float> { typedef bf16x8 Frag; typedef f32x8 Raw; static constexpr int kParts = 3; };
 
 template <typename Frag> __device__ __forceinline__ Frag decode_codes(uint32_t w);
 template <> __device__ __forceinline__ bf16x8 decode_codes<bf16x8>(uint32_t w) {
@@ -61,13 +62,11 @@ template <> __device__ __forceinline__ f16x8 ones_fragment<f16x8>() {
     return __builtin_bit_cast(f16x8, u32x4_t{w, w, w, w});
 }
 
-// Eight activations from column k on, as matrix operands; columns from `cols` on count as zero.  `vec`: rows start on
-// 16-byte boundaries.
+// Eight activations from column k on; columns from `cols` on count as zero.  `vec`: rows start on 16-byte boundaries.
 template <typename T>
-__device__ __forceinline__ void load_activations(const T* __restrict__ row, int64_t k, int64_t cols, bool vec,
-                                                 typename Int4Traits<T>::Frag* out) {
+__device__ __forceinline__ typename Int4Traits<T>::Raw load_raw(const T* __restrict__ row, int64_t k, int64_t cols, bool vec) {
+    typename Int4Traits<T>::Raw w = {};
     if constexpr (sizeof(T) == 2) {
-        u32x4_t w = {0u, 0u, 0u, 0u};
         if (vec && k + 8 <= cols) {
             w = *reinterpret_cast<const u32x4_t*>(row + k);
         } else if (k < cols) {
@@ -75,17 +74,25 @@ __device__ __forceinline__ void load_activations(const T* __restrict__ row, int6
             for (int e = 0; e < 8; ++e)
                 if (k + e < cols) w[e / 2] |= (uint32_t)row[k + e].bits << (16 * (e & 1));
         }
+    } else {
+        if (vec && k + 8 <= cols) {
+            w = *reinterpret_cast<const f32x8*>(row + k);
+        } else if (k < cols) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < cols) w[e] = row[k + e];
+        }
+    }
+    return w;
+}
+template <typename T>
+__device__ __forceinline__ void raw_to_fragments(const typename Int4Traits<T>::Raw& w, typename Int4Traits<T>::Frag* out) {
+    if constexpr (sizeof(T) == 2) {
         out[0] = __builtin_bit_cast(typename Int4Traits<T>::Frag, w);
     } else {
         float v[8];
-        if (vec && k + 8 <= cols) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(row + k), b = *reinterpret_cast<const f32x4*>(row + k + 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = k + e < cols ? row[k + e] : 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) v[e] = w[e];
         split_bf16<3>(v, out);
     }
 }
@@ -93,13 +100,13 @@ __device__ __forceinline__ void load_activations(const T* __restrict__ row, int6
 struct Int4Args {
     const void* x;
     const uint8_t* w;
-    const float* scale;   // [groups][rows padded to 16]
+    const float* scale;   // [row tile][groups][16]
     const int8_t* zero;   // same layout, or null: z = zero_const everywhere
     const void* bias;
     void* y;
     int64_t m, n, k, ldx, ldy;
     int64_t tiles;          // 128-column tiles of a row
-    int64_t npad;           // rows padded to 16
+    int64_t ntiles;         // tiles of 16 rows
     int64_t groups;
     uint64_t fold_inverse;  // ceil(2^32 / folds per group)
     float zero_const;
@@ -107,27 +114,47 @@ struct Int4Args {
 };
 
 // ------------------------------------------------------------------------------------------------- few activations --
+// What a wave reads for one 128-column tile of NT row tiles: codes, scales and zero points of its folds and, where one
+// tile of activations is all there is, those too.
+template <typename T, int FOLD, int MT, int NT, bool WITH_X>
+struct Int4Stage {
+    u32x4_t w[NT];
+    f32x4 scale[4 / FOLD][NT];
+    uint32_t zero[4 / FOLD][NT];
+    typename Int4Traits<T>::Raw x[WITH_X ? 4 : 1];
+};
+
 // A workgroup owns 16 * NT rows of the weight and 16 * MT activations; its waves take the 128-column tiles in turn and
 // their sums are added through LDS in wave order.  FOLD: matrix instructions (of 32 columns) whose sum shares a scale.
-template <typename T, int FOLD, int MT, int NT>
-__global__ __launch_bounds__(8 * kWave) void int4_linear_kernel(Int4Args a) {
+// Bound by the stream of codes: a wave asks for its next tile before it works on the present one.
+template <typename T, int FOLD, int MT, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void int4_linear_kernel(Int4Args a) {
     typedef typename Int4Traits<T>::Frag Frag;
     constexpr int P = Int4Traits<T>::kParts;
+    constexpr bool kWithX = MT == 1;
+    typedef Int4Stage<T, FOLD, MT, NT, kWithX> Stage;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
     const int i = lane & 15, c = lane >> 4;
     const int64_t tile0 = (int64_t)blockIdx.x * NT;
-    const int64_t ntiles = a.npad / kTileRows;
     const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
     const Frag ones = ones_fragment<Frag>();
-    const T* x = static_cast<const T*>(a.x);
-
+    const T* rows[MT];
+    int64_t cols[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int64_t m = m0 + 16 * mt + i;
+        rows[mt] = static_cast<const T*>(a.x) + (m < a.m ? m : 0) * a.ldx;
+        cols[mt] = m < a.m ? a.k : 0;  // rows behind the last one count as zero
+    }
     const u32x4_t* wp[NT];
-    int64_t row4[NT];
+    const float* sp[NT];
+    const int8_t* zp[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int64_t t = tile0 + nt < ntiles ? tile0 + nt : ntiles - 1;
+        const int64_t t = tile0 + nt < a.ntiles ? tile0 + nt : a.ntiles - 1;
         wp[nt] = reinterpret_cast<const u32x4_t*>(a.w + t * a.tiles * kTileBytes) + lane;
-        row4[nt] = t * kTileRows + 4 * c;
+        sp[nt] = a.scale + t * a.groups * kTileRows + 4 * c;
+        zp[nt] = a.zero + t * a.groups * kTileRows + 4 * c;
     }
     f32x4 acc[NT][MT];
 #pragma unroll
@@ -135,43 +162,55 @@ __global__ __launch_bounds__(8 * kWave) void int4_linear_kernel(Int4Args a) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int64_t kt = wave; kt < a.tiles; kt += waves) {
-        u32x4_t w[NT];
+    const auto load = [&](Stage& st, int64_t kt) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) w[nt] = wp[nt][kt * (kTileBytes / 16)];
+        for (int nt = 0; nt < NT; ++nt) st.w[nt] = wp[nt][kt * (kTileBytes / 16)];
+        if constexpr (kWithX) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st.x[j] = load_raw<T>(rows[0], kt * kTileCols + 32 * j + 8 * c, cols[0], a.vec_x);
+        }
+#pragma unroll
+        for (int f = 0; f < 4 / FOLD; ++f) {
+            const uint64_t fold = (uint64_t)(kt * (4 / FOLD) + f);
+            int64_t g = (int64_t)((fold * a.fold_inverse) >> 32);
+            g = g < a.groups ? g : a.groups - 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                st.scale[f][nt] = *reinterpret_cast<const f32x4*>(sp[nt] + g * kTileRows);
+                if (a.zero) st.zero[f][nt] = *reinterpret_cast<const uint32_t*>(zp[nt] + g * kTileRows);
+            }
+        }
+    };
+    const auto compute = [&](const Stage& st, int64_t kt) {
 #pragma unroll
         for (int f = 0; f < 4 / FOLD; ++f) {
             Frag xf[FOLD][MT][P];
             f32x4 sum[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const int64_t m = m0 + 16 * mt + i;
-                const bool live = m < a.m;
-                const T* row = x + (live ? m : 0) * a.ldx;
                 sum[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < FOLD; ++j) {
-                    const int64_t k = kt * kTileCols + 32 * (f * FOLD + j) + 8 * c;
-                    load_activations<T>(row, k, live ? a.k : 0, a.vec_x, xf[j][mt]);
+                    if constexpr (kWithX)
+                        raw_to_fragments<T>(st.x[f * FOLD + j], xf[j][mt]);
+                    else
+                        raw_to_fragments<T>(load_raw<T>(rows[mt], kt * kTileCols + 32 * (f * FOLD + j) + 8 * c, cols[mt], a.vec_x), xf[j][mt]);
+                }
+#pragma unroll
+                for (int j = 0; j < FOLD; ++j)
 #pragma unroll
                     for (int p = 0; p < P; ++p) sum[mt] = mma(ones, xf[j][mt][p], sum[mt]);
-                }
             }
-            const uint64_t fold = (uint64_t)(kt * (4 / FOLD) + f);
-            int64_t g = (int64_t)((fold * a.fold_inverse) >> 32);
-            g = g < a.groups ? g : a.groups - 1;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const f32x4 s = *reinterpret_cast<const f32x4*>(a.scale + g * a.npad + row4[nt]);
                 f32x4 z = {a.zero_const, a.zero_const, a.zero_const, a.zero_const};
                 if (a.zero) {
-                    const uint32_t b = *reinterpret_cast<const uint32_t*>(a.zero + g * a.npad + row4[nt]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) z[r] += (float)(int8_t)(b >> (8 * r));
+                    for (int r = 0; r < 4; ++r) z[r] += (float)(int8_t)(st.zero[f][nt] >> (8 * r));
                 }
                 Frag wf[FOLD];
 #pragma unroll
-                for (int j = 0; j < FOLD; ++j) wf[j] = decode_codes<Frag>(w[nt][f * FOLD + j]);
+                for (int j = 0; j < FOLD; ++j) wf[j] = decode_codes<Frag>(st.w[nt][f * FOLD + j]);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     f32x4 part;
@@ -182,9 +221,23 @@ __global__ __launch_bounds__(8 * kWave) void int4_linear_kernel(Int4Args a) {
 #pragma unroll
                         for (int p = 0; p < P; ++p) part = mma(wf[j], xf[j][mt][p], part);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[nt][mt][r] = __builtin_fmaf(s[r], part[r], acc[nt][mt][r]);
+                    for (int r = 0; r < 4; ++r) acc[nt][mt][r] = __builtin_fmaf(st.scale[f][nt][r], part[r], acc[nt][mt][r]);
                 }
             }
+        }
+    };
+    if (wave < a.tiles) {
+        Stage even, odd;
+        load(even, wave);
+        for (int64_t kt = wave;;) {
+            if (kt + waves < a.tiles) load(odd, kt + waves);
+            compute(even, kt);
+            kt += waves;
+            if (kt >= a.tiles) break;
+            if (kt + waves < a.tiles) load(even, kt + waves);
+            compute(odd, kt);
+            kt += waves;
+            if (kt >= a.tiles) break;
         }
     }
 
@@ -222,6 +275,167 @@ __global__ __launch_bounds__(8 * kWave) void int4_linear_kernel(Int4Args a) {
     }
 }
 
+// ---------------------------------------------------------------------------------- few activations, all of them in LDS --
+// For activations that fit LDS (decoding: one to a few tokens).  One workgroup of 16 waves to a compute unit; `splits`
+// waves share a row tile and take its 128-column tiles in turn, so a workgroup owns 16 / splits row tiles.  Activations
+// are the A operand here, the weight's rows the columns of the result: a lane's results belong to one channel, whose scale
+// and zero point are one register.  Bound by the stream of codes, so a wave asks for DEPTH tiles at once, right behind
+// its share of the activations; those are read back from LDS, whose waits do not hold up the stream.
+constexpr int kLdsWaves = 16;
+constexpr int kLdsThreads = kLdsWaves * kWave;
+
+template <typename T, int FOLD, int MT, int DEPTH, bool ASYM>
+__global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a, int splits, int row_bytes) {
+    typedef typename Int4Traits<T>::Frag Frag;
+    constexpr int P = Int4Traits<T>::kParts;
+    constexpr int kFolds = 4 / FOLD;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int i = lane & 15, c = lane >> 4;
+    const int m = (int)a.m, tiles = (int)a.tiles, groups = (int)a.groups;
+    const int per_group = kLdsWaves / splits;
+    const int split = wave % splits;
+    const int64_t tile = (int64_t)blockIdx.x * per_group + wave / splits;
+    extern __shared__ u32x4_t lds[];
+    char* xs = reinterpret_cast<char*>(lds);
+
+    // activations: [part][row][columns], rows padded by 16 bytes so that 16 of them lie on different banks
+    const int chunks = tiles * 16, total = m * chunks;
+    const auto fetch = [&](int id) {
+        const int row = id / chunks;
+        return load_raw<T>(static_cast<const T*>(a.x) + row * a.ldx, (id - row * chunks) * 8, a.k, a.vec_x);
+    };
+    const auto put = [&](int id, const typename Int4Traits<T>::Raw& raw) {
+        const int row = id / chunks;
+        Frag f[P];
+        raw_to_fragments<T>(raw, f);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            *reinterpret_cast<Frag*>(xs + (p * m + row) * row_bytes + (id - row * chunks) * 16) = f[p];
+    };
+    // all but the last kBatch rounds are stored at once; those wait until the first codes have been asked for
+    constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;
+    int id = threadIdx.x;
+    typename Int4Traits<T>::Raw raw[kBatch];
+    for (; id + kBatch * kLdsThreads < total; id += kBatch * kLdsThreads) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) raw[u] = fetch(id + u * kLdsThreads);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) put(id + u * kLdsThreads, raw[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+        if (id + u * kLdsThreads < total) raw[u] = fetch(id + u * kLdsThreads);
+
+    const bool live = tile < a.ntiles;
+    const int64_t tile_at = live ? tile : a.ntiles - 1;
+    const u32x4_t* wp = reinterpret_cast<const u32x4_t*>(a.w + tile_at * a.tiles * kTileBytes) + lane;
+    const float* sp = a.scale + tile_at * a.groups * kTileRows + i;
+    const int8_t* zp = ASYM ? a.zero + tile_at * a.groups * kTileRows + i : nullptr;
+    u32x4_t w[DEPTH];
+    float scale[DEPTH][kFolds];
+    int zero[DEPTH][kFolds];
+    const auto load = [&](int d, int kt) {
+        w[d] = __builtin_nontemporal_load(wp + kt * (kTileBytes / 16));
+#pragma unroll
+        for (int f = 0; f < kFolds; ++f) {
+            int g = (int)(((uint64_t)(unsigned)(kt * kFolds + f) * a.fold_inverse) >> 32);
+            g = g < groups ? g : groups - 1;
+            scale[d][f] = sp[g * kTileRows];
+            if constexpr (ASYM) zero[d][f] = zp[g * kTileRows];
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (split + d * splits < tiles) load(d, split + d * splits);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+        if (id + u * kLdsThreads < total) put(id + u * kLdsThreads, raw[u]);
+    __syncthreads();
+
+    f32x4 acc[MT];
+    const char* xrow[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int row = 16 * mt + i;  // rows behind the last one repeat it and are not stored
+        xrow[mt] = xs + (row < m ? row : m - 1) * row_bytes + 16 * c;
+    }
+    // sums of the activations over each fold, times z where it is the same everywhere: [fold][MT][16]
+    f32x4* sums = reinterpret_cast<f32x4*>(xs + P * m * row_bytes);
+    const Frag ones = ones_fragment<Frag>();
+    for (int fold = wave; fold < tiles * kFolds; fold += kLdsWaves)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + (fold * FOLD + j) * 64), ones, part);
+            if constexpr (!ASYM) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) part[r] *= a.zero_const;
+            }
+            if (i == 0) sums[(fold * MT + mt) * 4 + c] = part;
+        }
+    __syncthreads();
+
+    for (int kt0 = split; kt0 < tiles; kt0 += DEPTH * splits) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int kt = kt0 + d * splits;
+            if (kt < tiles) {
+#pragma unroll
+                for (int f = 0; f < kFolds; ++f) {
+                    Frag wf[FOLD];
+#pragma unroll
+                    for (int j = 0; j < FOLD; ++j) wf[j] = decode_codes<Frag>(w[d][f * FOLD + j]);
+                    const float z = ASYM ? a.zero_const + (float)zero[d][f] : a.zero_const;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        f32x4 part = sums[((kt * kFolds + f) * MT + mt) * 4 + c];
+                        if constexpr (ASYM) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) part[r] *= z;
+                        }
+#pragma unroll
+                        for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+                            for (int p = 0; p < P; ++p)
+                                part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + kt * 256 + (f * FOLD + j) * 64), wf[j], part);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[mt][r] = __builtin_fmaf(scale[d][f], part[r], acc[mt][r]);
+                    }
+                }
+                if (kt + DEPTH * splits < tiles) load(d, kt + DEPTH * splits);
+            }
+        }
+    }
+
+    f32x4* red = reinterpret_cast<f32x4*>(lds);  // [wave][MT][64], over the activations
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) red[(wave * MT + mt) * kWave + lane] = acc[mt];
+    __syncthreads();
+    for (int o = threadIdx.x; o < per_group * MT * kWave; o += kLdsThreads) {
+        const int unit = o / (MT * kWave), q = o % (MT * kWave);
+        const int64_t n = ((int64_t)blockIdx.x * per_group + unit) * kTileRows + (q & 15);
+        const int row = q / kWave * 16 + (q >> 4 & 3) * 4;
+        if (n >= a.n || row >= m) continue;
+        f32x4 v = red[unit * splits * MT * kWave + q];
+        for (int s = 1; s < splits; ++s) {
+            const f32x4 u = red[(unit * splits + s) * MT * kWave + q];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += u[r];
+        }
+        const float b = a.bias ? load_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
+        T* y = static_cast<T*>(a.y) + row * a.ldy + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (row + r < m) y[r * a.ldy] = store_cast<T>(v[r] + b);
+    }
+}
+
 // ----------------------------------------------------------------------------------------------------------- packing --
 __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restrict__ codes, int64_t n, int64_t k,
                                                            int32_t qmin, int64_t tiles, int64_t words,
@@ -247,16 +461,49 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
 // ------------------------------------------------------------------------------------------------------------- host --
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+#ifndef W1
+#define W1 8
+#endif
+#ifndef W2
+#define W2 8
+#endif
+template <typename T, int FOLD, int MT, int NT, int WAVES>
+int launch_few(const Int4Args& a, hipStream_t stream) {
+    const int waves = (int)(a.tiles < WAVES ? a.tiles : WAVES);
+    int4_linear_kernel<T, FOLD, MT, NT, WAVES><<<dim3((unsigned)ceil_div(a.ntiles, NT), (unsigned)ceil_div(a.m, 16 * MT)),
+                                                 waves * kWave, (size_t)waves * NT * MT * 1024, stream>>>(a);
+    return check_launch("ahq_int4_linear");
+}
+template <typename T, int FOLD, int MT, bool ASYM>
+int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stream) {
+    constexpr int kDepth = 2;
+    const auto kernel = int4_linear_lds_kernel<T, FOLD, MT, kDepth, ASYM>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
+    }
+    // as many waves to a row tile as one workgroup on each of the 256 compute units gives
+    int splits = kLdsWaves;
+    while (splits > 1 && (splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / splits) > 256)) splits /= 2;
+    kernel<<<(unsigned)ceil_div(a.ntiles, kLdsWaves / splits), kLdsThreads, lds, stream>>>(a, splits, (int)row_bytes);
+    return check_launch("ahq_int4_linear");
+}
+template <typename T, int FOLD, int MT>
+int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stream) {
+    return a.zero ? launch_lds<T, FOLD, MT, true>(a, row_bytes, lds, stream) : launch_lds<T, FOLD, MT, false>(a, row_bytes, lds, stream);
+}
+
 template <typename T, int FOLD>
 int launch_few(const Int4Args& a, hipStream_t stream) {
-    const int64_t ntiles = a.npad / kTileRows;
-    const int waves = a.tiles >= 16 ? 8 : a.tiles >= 4 ? 4 : 1;
-    if (a.m <= 16) {
-        int4_linear_kernel<T, FOLD, 1, 1><<<dim3((unsigned)ntiles, (unsigned)ceil_div(a.m, 16)), waves * kWave, waves * 1024, stream>>>(a);
-    } else {
-        int4_linear_kernel<T, FOLD, 2, 2><<<dim3((unsigned)ceil_div(ntiles, 2), (unsigned)ceil_div(a.m, 32)), waves * kWave, waves * 4096, stream>>>(a);
+    const size_t row_bytes = (size_t)a.tiles * 256 + 16;
+    const size_t xbytes = (size_t)a.m * row_bytes * Int4Traits<T>::kParts + (size_t)a.tiles * (4 / FOLD) * (a.m > 16 ? 128 : 64), red = (size_t)kLdsWaves * 1024 * (a.m > 16 ? 2 : 1);
+    const size_t lds = xbytes > red ? xbytes : red;
+    if (a.m <= 32 && lds <= 160 * 1024) {
+        if (a.m <= 16) return launch_lds<T, FOLD, 1>(a, row_bytes, lds, stream);
+        return launch_lds<T, FOLD, 2>(a, row_bytes, lds, stream);
     }
-    return check_launch("ahq_int4_linear");
+    if (a.m <= 16) return launch_few<T, FOLD, 1, 1, W1>(a, stream);
+    return launch_few<T, FOLD, 2, 2, W2>(a, stream);
 }
 
 template <typename T>
@@ -286,27 +533,28 @@ extern "C" int ahq_int4_pack(const int8_t* codes, int64_t n, int64_t k, int32_t 
     return check_launch("ahq_int4_pack");
 }
 
-extern "C" int ahq_int4_linear(int32_t dtype, const void* x, int64_t m, int64_t ldx, const void* packed, int64_t n,
-                               int64_t k, int64_t group, const float* scale, const int8_t* zero, float zero_const,
+extern "C" int ahq_int4_linear(const ahq_int4_weight* w, int32_t dtype, const void* x, int64_t m, int64_t ldx,
                                const void* bias, void* y, int64_t ldy, void* stream) {
     using namespace ahq;
+    if (!w || !w->packed || !w->scale) return set_error("null weight"), AHQ_ERR_INVALID;
+    const int64_t n = w->n, k = w->k, group = w->group;
     if (dtype < AHQ_F32 || dtype > AHQ_BF16) return set_error("bad dtype"), AHQ_ERR_INVALID;
     if (m < 0 || ahq_int4_packed_bytes(n, k) == 0) return set_error("bad shape"), AHQ_ERR_INVALID;
-    if (m == 0) return AHQ_OK;
-    if (!x || !packed || !scale || !y) return set_error("null argument"), AHQ_ERR_INVALID;
-    if (ldx < k || ldy < n) return set_error("row strides smaller than the rows"), AHQ_ERR_INVALID;
     if (group <= 0 || group > k || k % group) return set_error("the group must divide the row"), AHQ_ERR_INVALID;
     if (group != k && group % 32) return set_error("groups are multiples of 32 columns or the whole row"), AHQ_ERR_UNSUPPORTED;
-    if (((uintptr_t)packed | (uintptr_t)scale | (uintptr_t)zero) % 16)
+    if (((uintptr_t)w->packed | (uintptr_t)w->scale | (uintptr_t)w->zero) % 16)
         return set_error("packed weights, scales and zero points must be 16-byte aligned"), AHQ_ERR_INVALID;
+    if (m == 0) return AHQ_OK;
+    if (!x || !y) return set_error("null argument"), AHQ_ERR_INVALID;
+    if (ldx < k || ldy < n) return set_error("row strides smaller than the rows"), AHQ_ERR_INVALID;
     const size_t e = dtype == AHQ_F32 ? 4 : 2;
     if (((uintptr_t)x | (uintptr_t)y | (uintptr_t)bias) % e) return set_error("misaligned tensor"), AHQ_ERR_INVALID;
-    if (m > (1ll << 30)) return set_error("too many activations"), AHQ_ERR_UNSUPPORTED;
+    if (m > (1ll << 20)) return set_error("more than 2^20 activations in one call"), AHQ_ERR_UNSUPPORTED;
     Int4Args a;
-    a.x = x, a.w = static_cast<const uint8_t*>(packed), a.scale = scale, a.zero = zero, a.bias = bias, a.y = y;
+    a.x = x, a.w = static_cast<const uint8_t*>(w->packed), a.scale = w->scale, a.zero = w->zero, a.bias = bias, a.y = y;
     a.m = m, a.n = n, a.k = k, a.ldx = ldx, a.ldy = ldy;
-    a.tiles = ceil_div(k, kTileCols), a.npad = ceil_div(n, kTileRows) * kTileRows, a.groups = k / group;
-    a.zero_const = zero_const;
+    a.tiles = ceil_div(k, kTileCols), a.ntiles = ceil_div(n, kTileRows), a.groups = k / group;
+    a.zero_const = w->zero_const;
     // The scale is applied every 32, 64 or 128 columns: as rarely as one scale lasts (128 keeps the group sums short
     // where a scale covers a whole row).
     const int fold = group == k || group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;

@@ -1,22 +1,27 @@
 // A key/value cache held in 8 bits, and the attention that reads it.
 //
-// Stored: codes in [-127, 127] and, for every block of `block` tokens (16, 32 or 64) of a sequence and head, the largest
-// magnitude `amax` among them; a code stands for code * amax / 127.  Keys lie as [sequence, head, token, channel].  Values
-// lie as [sequence, head, tile of 64 tokens, channel, token of the tile]: the product of the probabilities and the values
-// sums over tokens, and a lane of a matrix instruction then finds the 16 tokens it needs of one channel in one 16-byte
-// load.
+// Stored: codes in [-127, 127], as bytes code + 128, and for every block of `block` tokens (16, 32 or 64) of a sequence and
+// head the largest magnitude `amax` among them; a code stands for code * amax / 127.  Keys lie as [sequence, head, token,
+// channel].  Values lie as [sequence, head, tile of 64 tokens, channel, token of the tile]: the product of the
+// probabilities and the values sums over tokens, and a lane of a matrix instruction then finds the 16 tokens it needs of
+// one channel in one 16-byte load.
 //
 // Writing (kv_append_kernel): a workgroup owns one block of one head.  amax = max(what the block had, |new tokens|), code =
 // rint(127 x / amax), half to even and exact; where amax grows, the codes the block had become rint(code * old / new).
 //
-// Reading (kv_attend_kernel): one pass over the tokens with the running maximum and sum of the softmax.  Rows of a tile
-// are the query heads of one key head (and the queries behind each other, where there are several).  A wave takes 64
-// tokens at a time: scores = keys (A) x queries (B) on the matrix cores, so that lane 16 c + i of the result holds 16
-// tokens of row i.  Keys are handed to the instruction in an order that makes those the tokens 16 c .. 16 c + 15 of the
-// tile: that is the B operand of the next product, values (A) x probabilities (B), without any exchange between lanes.
-// Codes are exact in bfloat16; queries are used exactly (float16 as two, float32 as three bfloat16 parts); the block's
-// scales multiply scores and probabilities in float32; the probabilities enter the second product as two bfloat16 parts
-// (16 bits, 2^-17 relative) for 16-bit queries and as three for float32 ones.  Everything else is float32.
+// Reading (kv_attend_kernel): one pass over the tokens with a running reference and sum of the softmax.  Rows are the query
+// heads of one key head, query after query.  A wave takes 64 tokens at a time: scores = keys (A) x queries (B) on the
+// matrix cores, so that lane 16 c + i of the result holds 16 tokens of row i.  Keys are handed to the instruction in an
+// order that makes those the tokens 16 c .. 16 c + 15 of the tile: that is the B operand of the next product, values (A) x
+// probabilities (B), without any exchange between lanes.
+//
+// Both products run in float16 with float32 sums.  Codes are exact in it: a byte b next to the byte 0x64 is the number
+// 1024 + b, and one packed addition of -1152 makes two codes of two bytes.  A query row is multiplied by the power of two
+// that brings its largest value to 2^13 .. 2^14, which keeps 16-bit queries exact (bfloat16 down to 2^-30 of the row's
+// largest value); float32 queries become two parts, 22 bits.  Probabilities carry the scale of their values' block:
+// with x = score + log2(scale), weights are 2^(x - reference), the reference being such that the largest is at most
+// kTop = 2^14, so float16 holds them to 2^-12 (two parts for float32 queries: 2^-23) and down to 2^-38 of the largest;
+// the softmax's denominator sums weight / scale in float32.  Scales below 2^-80 count as 2^-80 there.
 
 #include "../../include/aimet_amd_serving.h"
 #include "ahq_host.h"
@@ -25,12 +30,13 @@
 namespace ahq {
 
 constexpr int kKvTile = 64;
+constexpr int kCodeBias = 128;
 
 // ------------------------------------------------------------------------------------------------------------ append --
 struct KvAppendArgs {
     const void* x[2];        // new keys, new values
     int64_t sb[2], sh[2], st[2];  // strides in elements: sequence, head, token
-    int8_t* codes[2];
+    uint8_t* codes[2];
     float* amax[2];
     const int32_t* start;    // null: start0 for every sequence
     const int32_t* counts;   // null: count0
@@ -146,23 +152,23 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
     const CodeRule rule = code_rule(amax, sizeof(T) == 2);
     const int first = rescale ? 0 : old_end;  // first token whose codes are stored
 
-    int8_t* keys = a.codes[which] + ((int64_t)bh * a.capacity + p0) * D;
+    uint8_t* keys = a.codes[which] + ((int64_t)bh * a.capacity + p0) * D;
     // tile of 64 tokens that holds this block, and the block's place in it
-    int8_t* tile = a.codes[which] + ((int64_t)bh * a.capacity + p0 / kKvTile * kKvTile) * D + p0 % kKvTile;
-    __shared__ alignas(16) int8_t stage[D * kPitch];
+    uint8_t* tile = a.codes[which] + ((int64_t)bh * a.capacity + p0 / kKvTile * kKvTile) * D + p0 % kKvTile;
+    __shared__ alignas(16) uint8_t stage[D * kPitch];
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
         const int id = it * kThreads + threadIdx.x, t = id / (D / 8), d = id % (D / 8) * 8;
         if (t < first || t >= new_end) continue;
-        union { int8_t b[8]; u32x2_t w; } out;
+        union { uint8_t b[8]; u32x2_t w; } out;
         if (t >= old_end) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out.b[e] = (int8_t)to_code(v[it][e], rule);
+            for (int e = 0; e < 8; ++e) out.b[e] = (uint8_t)(to_code(v[it][e], rule) + kCodeBias);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int q = which ? tile[(d + e) * kKvTile + t] : keys[(int64_t)t * D + d + e];
-                out.b[e] = (int8_t)(int)__builtin_rint((double)q * (double)before / (double)amax);
+                const int q = (which ? tile[(d + e) * kKvTile + t] : keys[(int64_t)t * D + d + e]) - kCodeBias;
+                out.b[e] = (uint8_t)((int)__builtin_rint((double)q * (double)before / (double)amax) + kCodeBias);
             }
         }
         if (which == 0) {
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
         for (int id = threadIdx.x; id < D * (BT / 16); id += kThreads) {
             const int d = id / (BT / 16), t = id % (BT / 16) * 16;
             const uint32_t* from = reinterpret_cast<const uint32_t*>(stage + d * kPitch + t);
-            int8_t* to = tile + d * kKvTile + t;
+            uint8_t* to = tile + d * kKvTile + t;
             if (first <= t && t + 16 <= new_end) {
                 *reinterpret_cast<u32x4_t*>(to) = u32x4_t{from[0], from[1], from[2], from[3]};
             } else {
@@ -192,7 +198,7 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
 
 // -------------------------------------------------------------------------------------------------------- dequantize --
 struct KvValuesArgs {
-    const int8_t* codes[2];
+    const uint8_t* codes[2];
     const float* amax[2];
     void* out[2];  // [sequence, head, length, D]
     int32_t capacity, length, block;
@@ -204,10 +210,10 @@ __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
     const int which = blockIdx.z, tile = blockIdx.x;
     const int64_t bh = blockIdx.y;
     const int p0 = tile * kKvTile;
-    const int8_t* codes = a.codes[which] + (bh * a.capacity + p0) * D;
+    const uint8_t* codes = a.codes[which] + (bh * a.capacity + p0) * D;
     const float* amax = a.amax[which] + bh * (a.capacity / a.block);
     T* out = static_cast<T*>(a.out[which]) + (bh * a.length + p0) * D;
-    __shared__ alignas(16) int8_t stage[D * kPitch];
+    __shared__ alignas(16) uint8_t stage[D * kPitch];
     if (which) {
         for (int id = threadIdx.x; id < D * 4; id += kBlock) {
             const u32x4_t w = *reinterpret_cast<const u32x4_t*>(codes + id * 16);
@@ -221,7 +227,7 @@ __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
         const int t = id / (D / 8), d = id % (D / 8) * 8;
         if (p0 + t >= a.length) break;
         const float s = amax[(p0 + t) / a.block] / 127.0f;
-        union { int8_t b[8]; u32x2_t w; } in;
+        union { uint8_t b[8]; u32x2_t w; } in;
         if (which) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) in.b[e] = stage[(d + e) * kPitch + t];
@@ -233,7 +239,7 @@ __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
         for (int u = 0; u < 8 / kPer; ++u) {
             Pack<T, kPer> w;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) w.v[e] = store_cast<T>((float)in.b[u * kPer + e] * s);
+            for (int e = 0; e < kPer; ++e) w.v[e] = store_cast<T>((float)(in.b[u * kPer + e] - kCodeBias) * s);
             store_pack<T, kPer>(out + (int64_t)t * D + d + u * kPer, w);
         }
     }
@@ -244,56 +250,19 @@ struct KvAttendArgs {
     const void* q;
     void* out;
     int64_t qb, qh, qt, ob, oh, ot;  // strides in elements
-    const int8_t *k_codes, *v_codes;
+    const uint8_t *k_codes, *v_codes;
     const float *k_amax, *v_amax;
     const int32_t* lengths;  // null: length0
     const int32_t* counts;   // null: count0
     int32_t length0, count0;
     int32_t heads, groups, queries, capacity, block;
-    int32_t row_tiles, splits;
-    float scale;             // of the scores, times log2(e)
-    int32_t vec;             // rows of q start on 16-byte boundaries
-    float* part;             // [sequence * head][row tile][split][16][D], then [..][16][2]: maximum and sum
+    int32_t rows, row_tile;       // queries * groups; rows of a workgroup
+    int32_t splits, split_tiles;  // splits of the token axis, token tiles of each
+    float scale;                  // of the scores, times log2(e)
+    int32_t vec;                  // rows of q start on 16-byte boundaries
+    float* part;                  // [sequence * head][row][split][D], then [..][row][split][2]: reference and sum
     float* part_stat;
 };
-
-template <typename T> struct AttendTraits;
-template <> struct AttendTraits<bf16_t> { static constexpr int kQ = 1, kP = 2; };
-template <> struct AttendTraits<f16_t> { static constexpr int kQ = 2, kP = 2; };
-template <> struct AttendTraits<float> { static constexpr int kQ = 3, kP = 3; };
-
-// Eight codes as bfloat16: whole numbers up to 127 have no low half in float32.
-__device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t a, uint32_t b) {
-    u32x4_t w;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        w[e] = pack_high_halves((float)(int8_t)(a >> (16 * e)), (float)(int8_t)(a >> (16 * e + 8)));
-        w[2 + e] = pack_high_halves((float)(int8_t)(b >> (16 * e)), (float)(int8_t)(b >> (16 * e + 8)));
-    }
-    return __builtin_bit_cast(bf16x8, w);
-}
-
-template <typename T, int N>
-__device__ __forceinline__ void load_query(const T* p, bool live, bool vec, bf16x8* out) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if (live) {
-        constexpr int kPer = 16 / sizeof(T);
-        if (vec) {
-#pragma unroll
-            for (int u = 0; u < 8 / kPer; ++u) {
-                const Pack<T, kPer> w = load_pack<T, kPer>(p + u * kPer);
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) v[u * kPer + e] = load_f32(w.v[e]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = load_f32(p[e]);
-        }
-    }
-    split_bf16<N>(v, out);
-}
 
 struct SequenceView { int length, count; };
 __device__ __forceinline__ SequenceView view_sequence(const KvAttendArgs& a, int b) {
@@ -303,173 +272,390 @@ __device__ __forceinline__ SequenceView view_sequence(const KvAttendArgs& a, int
     t = t < 0 ? 0 : t > a.queries ? a.queries : t;
     return {n, t};
 }
+// Token tiles that hold something the rows up to `row` see.
+__device__ __forceinline__ int seen_tiles(const KvAttendArgs& a, const SequenceView& seq, int row) {
+    int t = row / a.groups;
+    if (t >= seq.count) t = seq.count - 1;
+    const int seen = seq.length - seq.count + t + 1;
+    return t < 0 || seen <= 0 ? 0 : (seen + kKvTile - 1) / kKvTile;
+}
+// Splits of the token axis that hold such tiles, for the workgroup's rows that `row` is one of.
+__device__ __forceinline__ int used_splits(const KvAttendArgs& a, const SequenceView& seq, int row) {
+    return (seen_tiles(a, seq, row / a.row_tile * a.row_tile + a.row_tile - 1) + a.split_tiles - 1) / a.split_tiles;
+}
 
+// Two codes of the low or of the high half of a word, exact in float16.
+__device__ __forceinline__ f16x2 two_codes(uint32_t w, uint32_t selector) {
+    const f16x2 biased = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, selector));
+    return biased + f16x2{(_Float16)-1152.0f, (_Float16)-1152.0f};
+}
+__device__ __forceinline__ f16x8 codes_to_f16(uint32_t a, uint32_t b) {
+    union { f16x2 h[4]; f16x8 v; } r;
+    r.h[0] = two_codes(a, 0x04010400u), r.h[1] = two_codes(a, 0x04030402u);
+    r.h[2] = two_codes(b, 0x04010400u), r.h[3] = two_codes(b, 0x04030402u);
+    return r.v;
+}
+// Eight values as a sum of N float16 fragments.
+template <int N>
+__device__ __forceinline__ void split_f16(const float* v, f16x8* out) {
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rest[e] = v[e];
+#pragma unroll
+    for (int p = 0; p < N; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            out[p][e] = (_Float16)rest[e];
+            if (p + 1 < N) rest[e] -= (float)out[p][e];
+        }
+}
+
+constexpr float kTop = 14.0f;                 // log2 of the largest weight
+constexpr float kLeastScale = 0x1p-80f;
 constexpr int kAttendWaves = 4;
 
-template <typename T, int D>
+// Loads are waited for in the order they were asked for, so a tile's scales come in front of its keys.
+template <int D>
+struct KvTile {
+    u32x4_t keys[4][D / 64];
+    float k_amax, v_amax;
+};
+
+// What a wave knows of its 16 * NR rows; a lane holds row 16 n + i of them and the channels 16 u + 4 c + r of its answer.
+template <typename T, int D, int NR>
+struct AttendRows {
+    static constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kSteps = D / 32, kOut = D / 16;
+    f16x8 q[kSteps][NR][kParts];
+    f32x4 o[kOut][NR];
+    float rescale[NR];  // what the row's power of two is undone with, times the scale of the scores
+    float reference[NR], top[NR], sum[NR];
+    int last[NR];       // the last token the row sees; below 0: none
+    int least;          // of the wave's rows that see anything, the least `last`
+
+    __device__ __forceinline__ void begin(const KvAttendArgs& a, const SequenceView& seq, int b, int h, int row0, int i, int c) {
+        least = 0x7fffffff;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const int row = row0 + 16 * n + i, t = row / a.groups;
+            last[n] = row < a.rows && t < seq.count ? seq.length - seq.count + t : -1;
+            const bool live = last[n] >= 0;
+            if (live && last[n] < least) least = last[n];
+            const T* at = static_cast<const T*>(a.q) + b * a.qb + (int64_t)(h * a.groups + row % a.groups) * a.qh + (int64_t)t * a.qt;
+            float v[kSteps][8];
+            float size = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const T* p = at + 64 * (s / 2) + 16 * c + 8 * (s % 2);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[s][e] = 0.0f;
+                if (live) {
+                    constexpr int kPer = 16 / sizeof(T);
+                    if (a.vec) {
+#pragma unroll
+                        for (int u = 0; u < 8 / kPer; ++u) {
+                            const Pack<T, kPer> w = load_pack<T, kPer>(p + u * kPer);
+#pragma unroll
+                            for (int e = 0; e < kPer; ++e) v[s][u * kPer + e] = load_f32(w.v[e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[s][e] = load_f32(p[e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) size = fmaxf(size, fabsf(v[s][e]));
+            }
+            size = fmaxf(size, __shfl_xor(size, 16, kWave));
+            size = fmaxf(size, __shfl_xor(size, 32, kWave));
+            // exponent of the largest value; zeros, infinities and the smallest numbers go as they are
+            int ex = (int)(f32_to_bits(size) >> 23);
+            if (size == 0.0f || ex >= 255) ex = 140;
+            if (ex < 16) ex = 16;
+            const float up = bits_to_f32((uint32_t)(267 - ex) << 23);
+            rescale[n] = bits_to_f32((uint32_t)(ex - 13) << 23) * a.scale;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[s][e] *= up;
+                split_f16<kParts>(v[s], q[s][n]);
+            }
+            reference[n] = 0.0f, top[n] = -__builtin_inff(), sum[n] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kOut; ++u) o[u][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int m = 1; m < 16; m *= 2) {
+            const int other = __shfl_xor(least, m, kWave);
+            least = other < least ? other : least;
+        }
+        least = __builtin_amdgcn_readfirstlane(least);
+    }
+
+    // One tile of 64 tokens; `prefetch` is called once the tile's keys and scales are no longer needed.
+    template <typename Prefetch>
+    __device__ __forceinline__ void work(const KvTile<D>& tile, const u32x4_t* values, int p0, int c, Prefetch prefetch) {
+        const float k_scale = tile.k_amax / 127.0f;
+        const float v_scale = fmaxf(tile.v_amax / 127.0f, kLeastScale);
+        const float v_log = __builtin_amdgcn_logf(v_scale);
+        const float v_inverse = 1.0f / v_scale;
+        f32x4 x[4][NR];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n) x[s][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) {
+                const u32x4_t w = tile.keys[s][u / 2];
+                const f16x8 kf = u % 2 ? codes_to_f16(w[2], w[3]) : codes_to_f16(w[0], w[1]);
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf, q[u][n][p], x[s][n]);
+            }
+        }
+        prefetch();
+        f16x8 pf[2][NR][kParts];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float factor = k_scale * rescale[n], shift = v_log - reference[n];
+            float most = -__builtin_inff();
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[s][n][r] = __builtin_fmaf(x[s][n][r], factor, shift);
+            float inverse = v_inverse;
+            if (p0 + kKvTile - 1 > least) {  // some row's last token lies in this tile
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (p0 + 16 * c + 4 * s + r > last[n]) x[s][n][r] = -__builtin_inff();
+                if (p0 + 16 * c > last[n]) inverse = 0.0f;
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) most = fmaxf(most, x[s][n][r]);
+            most = fmaxf(most, __shfl_xor(most, 16, kWave));
+            most = fmaxf(most, __shfl_xor(most, 32, kWave));
+            const bool raise = most > top[n];
+            if (__any(raise)) {  // seldom once a few tiles are done
+                const float by = raise ? most - kTop : 0.0f;
+                const float fade = !raise ? 1.0f : top[n] == kTop ? __builtin_amdgcn_exp2f(-by) : 0.0f;
+                if (raise) top[n] = kTop;
+                reference[n] += by;
+                sum[n] *= fade;
+#pragma unroll
+                for (int u = 0; u < kOut; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[u][n][r] *= fade;
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[s][n][r] -= by;
+            }
+            float total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(x[2 * w + e / 4][n][e % 4]);
+                    total += p[e];
+                }
+                split_f16<kParts>(p, pf[w][n]);
+            }
+            sum[n] = __builtin_fmaf(total, inverse, sum[n]);
+        }
+#pragma unroll
+        for (int u = 0; u < kOut; ++u) {
+            const f16x8 v0 = codes_to_f16(values[u][0], values[u][1]), v1 = codes_to_f16(values[u][2], values[u][3]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    o[u][n] = mma(v0, pf[0][n][p], o[u][n]);
+                    o[u][n] = mma(v1, pf[1][n][p], o[u][n]);
+                }
+        }
+    }
+};
+
+// TOKEN_WAVES = 4: the waves of a workgroup share its 16 * NR rows and take their token tiles in turn (few rows, long
+// caches: bound by the stream of codes); 1: each wave has 16 * NR rows of its own and all the tokens (prompts: bound by the
+// matrix cores and the vector work around them).
+template <typename T, int D, int NR, int TOKEN_WAVES>
 __global__ __launch_bounds__(kAttendWaves * kWave) void kv_attend_kernel(KvAttendArgs a) {
-    constexpr int NQ = AttendTraits<T>::kQ, NP = AttendTraits<T>::kP;
-    constexpr int kSteps = D / 32;   // matrix instructions along the channels
-    constexpr int kOut = D / 16;     // output tiles of 16 channels
+    constexpr int kOut = D / 16;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int i = lane & 15, c = lane >> 4;
-    const int split = blockIdx.x, row_tile = blockIdx.y;
-    const int64_t bh = blockIdx.z;
+    const int64_t bh = blockIdx.y;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+    const int split = blockIdx.z;
+    const int wg_row = (int)(gridDim.x - 1 - blockIdx.x) * a.row_tile;  // the rows that see most come first
     const SequenceView seq = view_sequence(a, b);
+    const int used = used_splits(a, seq, wg_row);
+    if (split >= used && split > 0) return;
 
-    const int rows = a.queries * a.groups;
-    const int row = row_tile * 16 + i;
-    const int t = row / a.groups;
-    // the last token this row sees; below 0: none
-    const int last = row < rows && t < seq.count ? seq.length - seq.count + t : -1;
-    int t_end = (row_tile * 16 + 15) / a.groups;
-    if (t_end >= seq.count) t_end = seq.count - 1;
-    const int seen = seq.length - seq.count + t_end + 1;  // tokens the tile's last row sees
-    const int tiles = t_end < 0 || seen <= 0 ? 0 : (seen + kKvTile - 1) / kKvTile;
-    const int per_split = (tiles + a.splits - 1) / a.splits;
-    const int first = split * per_split;
-    const int stop = first + per_split < tiles ? first + per_split : tiles;
+    const int row0 = wg_row + (TOKEN_WAVES == 1 ? wave * 16 * NR : 0);
+    const int tiles = row0 < a.rows ? seen_tiles(a, seq, row0 + 16 * NR - 1) : 0;
+    const int first = split * a.split_tiles + (TOKEN_WAVES == 1 ? 0 : wave);
+    const int stop = (split + 1) * a.split_tiles < tiles ? (split + 1) * a.split_tiles : tiles;
 
-    bf16x8 q[kSteps][NQ];
-    {
-        const bool live = last >= 0;
-        const T* base = static_cast<const T*>(a.q) + b * a.qb + (int64_t)(h * a.groups + row % a.groups) * a.qh + (int64_t)t * a.qt;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) load_query<T, NQ>(base + 64 * (s / 2) + 16 * c + 8 * (s % 2), live, a.vec, q[s]);
-    }
-    f32x4 o[kOut];
-#pragma unroll
-    for (int u = 0; u < kOut; ++u) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float top = -__builtin_inff(), sum = 0.0f;
-
-    const int8_t* keys = a.k_codes + bh * a.capacity * D;
-    const int8_t* values = a.v_codes + bh * a.capacity * D;
+    AttendRows<T, D, NR> rows;
+    rows.begin(a, seq, b, h, row0, i, c);
+    const uint8_t* keys = a.k_codes + bh * a.capacity * D + 16 * c;
+    const uint8_t* values = a.v_codes + bh * a.capacity * D + i * kKvTile + 16 * c;
     const float* k_amax = a.k_amax + bh * (a.capacity / a.block);
     const float* v_amax = a.v_amax + bh * (a.capacity / a.block);
     const int key_row = (i >> 2) * 16 + (i & 3);  // token of A row i in the score tile s: key_row + 4 s
 
-    for (int tile = first + wave; tile < stop; tile += kAttendWaves) {
-        const int p0 = tile * kKvTile;
-        u32x4_t kw[4][D / 64];
+    // Keys of the next tile and values of this one are asked for before the work on this one begins.
+    KvTile<D> next;
+    const auto load = [&](int tile) {
+        const int block_at = (tile * kKvTile + 16 * c) / a.block;
+        next.k_amax = k_amax[block_at];
+        next.v_amax = v_amax[block_at];
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int u = 0; u < D / 64; ++u)
-                kw[s][u] = *reinterpret_cast<const u32x4_t*>(keys + (int64_t)(p0 + key_row + 4 * s) * D + 64 * u + 16 * c);
-        const int block_at = (p0 + 16 * c) / a.block;
-        const float k_scale = k_amax[block_at] / 127.0f * a.scale;
-        const float v_scale = v_amax[block_at] / 127.0f;
-        float sc[16];
-        float tile_top = -__builtin_inff();
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int u = 0; u < kSteps; ++u) {
-                const u32x4_t w = kw[s][u / 2];
-                const bf16x8 kf = u % 2 ? codes_to_bf16(w[2], w[3]) : codes_to_bf16(w[0], w[1]);
-#pragma unroll
-                for (int p = 0; p < NQ; ++p) acc = mma(kf, q[u][p], acc);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float v = p0 + 16 * c + 4 * s + r <= last ? acc[r] * k_scale : -__builtin_inff();
-                sc[4 * s + r] = v;
-                tile_top = fmaxf(tile_top, v);
-            }
-        }
-        tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 16, kWave));
-        tile_top = fmaxf(tile_top, __shfl_xor(tile_top, 32, kWave));
-        const float now = fmaxf(top, tile_top);
-        const float base = now == -__builtin_inff() ? 0.0f : now;
-        const float fade = __builtin_amdgcn_exp2f(top - base);
-        top = now;
-        sum *= fade;
+                next.keys[s][u] = *reinterpret_cast<const u32x4_t*>(keys + (int64_t)(tile * kKvTile + key_row + 4 * s) * D + 64 * u);
+    };
+    if (first < stop) load(first);
+    for (int tile = first; tile < stop; tile += TOKEN_WAVES) {
+        u32x4_t vw[kOut];
 #pragma unroll
         for (int u = 0; u < kOut; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[u][r] *= fade;
-        bf16x8 pf[2][NP];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool hidden = p0 + 16 * c + 8 * w + e > last;
-                const float v = hidden ? 0.0f : __builtin_amdgcn_exp2f(sc[8 * w + e] - base);
-                sum += v;
-                p[e] = hidden ? 0.0f : v * v_scale;
-            }
-            split_bf16<NP>(p, pf[w]);
-        }
-#pragma unroll
-        for (int u = 0; u < kOut; ++u) {
-            const u32x4_t w = *reinterpret_cast<const u32x4_t*>(values + (int64_t)p0 * D + (16 * u + i) * kKvTile + 16 * c);
-            const bf16x8 v0 = codes_to_bf16(w[0], w[1]), v1 = codes_to_bf16(w[2], w[3]);
-#pragma unroll
-            for (int p = 0; p < NP; ++p) o[u] = mma(v0, pf[0][p], o[u]);
-#pragma unroll
-            for (int p = 0; p < NP; ++p) o[u] = mma(v1, pf[1][p], o[u]);
-        }
+            vw[u] = *reinterpret_cast<const u32x4_t*>(values + (int64_t)tile * kKvTile * D + 16 * u * kKvTile);
+        rows.work(next, vw, tile * kKvTile, c, [&] {
+            if (tile + TOKEN_WAVES < stop) load(tile + TOKEN_WAVES);
+        });
     }
-    sum += __shfl_xor(sum, 16, kWave);
-    sum += __shfl_xor(sum, 32, kWave);
+    float sum[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        sum[n] = rows.sum[n];
+        sum[n] += __shfl_xor(sum[n], 16, kWave);
+        sum[n] += __shfl_xor(sum[n], 32, kWave);
+        if (rows.last[n] < 0) sum[n] = 0.0f;
+        if (rows.top[n] != kTop) rows.reference[n] = -__builtin_inff();  // nothing seen here
+    }
 
-    // the waves' results are joined through LDS, in wave order
-    constexpr int kPitch = 17;
-    extern __shared__ float joined[];  // [wave][D][17], then [wave][16][2]
-    float* stats = joined + kAttendWaves * D * kPitch;
+    if constexpr (TOKEN_WAVES == 1) {
 #pragma unroll
-    for (int u = 0; u < kOut; ++u)
+        for (int n = 0; n < NR; ++n) {
+            const int row = row0 + 16 * n + i;
+            if (row >= a.rows) continue;
+            if (used <= 1) {
+                const float inverse = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+                T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * c;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) joined[(wave * D + 16 * u + 4 * c + r) * kPitch + i] = o[u][r];
-    if (c == 0) stats[(wave * 16 + i) * 2] = top, stats[(wave * 16 + i) * 2 + 1] = sum;
-    __syncthreads();
-    for (int id = threadIdx.x; id < 16 * D; id += kAttendWaves * kWave) {
-        const int rr = id / D, d = id % D;
-        float best = -__builtin_inff();
+                for (int u = 0; u < kOut; ++u)
 #pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) best = fmaxf(best, stats[(w * 16 + rr) * 2]);
-        const float base = best == -__builtin_inff() ? 0.0f : best;
-        float total = 0.0f, value = 0.0f;
+                    for (int r = 0; r < 4; ++r) to[16 * u + r] = store_cast<T>(sum[n] == 0.0f ? 0.0f : rows.o[u][n][r] * inverse);
+            } else {
+                const int64_t at = (bh * a.rows + row) * a.splits + split;
 #pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(stats[(w * 16 + rr) * 2] - base);
-            total += f * stats[(w * 16 + rr) * 2 + 1];
-            value += f * joined[(w * D + d) * kPitch + rr];
+                for (int u = 0; u < kOut; ++u) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * u + 4 * c) = rows.o[u][n];
+                if (c == 0) a.part_stat[at * 2] = rows.reference[n], a.part_stat[at * 2 + 1] = sum[n];
+            }
         }
-        const int out_row = row_tile * 16 + rr;
-        if (out_row >= rows) continue;
-        if (a.splits == 1) {
-            T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + out_row % a.groups) * a.oh + (int64_t)(out_row / a.groups) * a.ot;
-            to[d] = store_cast<T>(total == 0.0f ? 0.0f : value / total);
-        } else {
-            const int64_t at = ((bh * a.row_tiles + row_tile) * a.splits + split) * 16 + rr;
-            a.part[at * D + d] = value;
-            if (d == 0) a.part_stat[at * 2] = best, a.part_stat[at * 2 + 1] = total;
+    } else {
+        // the waves' results are joined through LDS, in wave order
+        constexpr int kRows = 16 * NR, kPitch = kRows + 1;
+        extern __shared__ float joined[];  // [wave][D][kPitch], then [wave][kRows][2]
+        float* stats = joined + kAttendWaves * D * kPitch;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+#pragma unroll
+            for (int u = 0; u < kOut; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) joined[(wave * D + 16 * u + 4 * c + r) * kPitch + 16 * n + i] = rows.o[u][n][r];
+            if (c == 0) stats[(wave * kRows + 16 * n + i) * 2] = rows.reference[n], stats[(wave * kRows + 16 * n + i) * 2 + 1] = sum[n];
+        }
+        __syncthreads();
+        for (int id = threadIdx.x; id < kRows * D; id += kAttendWaves * kWave) {
+            const int rr = id / D, d = id % D;
+            const int row = wg_row + rr;
+            if (row >= a.rows) break;
+            float best = -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < kAttendWaves; ++w) best = fmaxf(best, stats[(w * kRows + rr) * 2]);
+            const float base = best == -__builtin_inff() ? 0.0f : best;
+            float total = 0.0f, value = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kAttendWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(stats[(w * kRows + rr) * 2] - base);
+                total += f * stats[(w * kRows + rr) * 2 + 1];
+                value += f * joined[(w * D + d) * kPitch + rr];
+            }
+            if (used <= 1) {
+                T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot;
+                to[d] = store_cast<T>(total == 0.0f ? 0.0f : value / total);
+            } else {
+                const int64_t at = (bh * a.rows + row) * a.splits + split;
+                a.part[at * D + d] = value;
+                if (d == 0) a.part_stat[at * 2] = best, a.part_stat[at * 2 + 1] = total;
+            }
         }
     }
 }
 
-// One workgroup per row: the splits' results are added in their order.
+// One workgroup per row joins the splits: the weights of all of them first, then 1024 / D splits at a time with 16 bytes
+// a lane, their sums through LDS in a fixed order.  Rows that one split answered are done already.
+constexpr int kJoinThreads = 256;
 template <typename T, int D>
-__global__ __launch_bounds__(D) void kv_join_kernel(KvAttendArgs a) {
-    const int row = blockIdx.x, d = threadIdx.x;
+__global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttendArgs a) {
+    constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes;
+    const int row = blockIdx.x;
     const int64_t bh = blockIdx.y;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-    const int64_t at = (bh * a.row_tiles + row / 16) * a.splits * 16 + row % 16;
+    const SequenceView seq = view_sequence(a, b);
+    const int used = used_splits(a, seq, row);
+    if (used <= 1) return;
+    const int64_t at = (bh * a.rows + row) * a.splits;
+    const float* stat = a.part_stat + at * 2;
+    const float* part = a.part + at * D;
+    __shared__ float smem[kJoinThreads / kWave];
+    __shared__ float weight[kJoinThreads];
+    __shared__ f32x4 sums[kRows][kLanes];
     float best = -__builtin_inff();
-    for (int s = 0; s < a.splits; ++s) best = fmaxf(best, a.part_stat[(at + (int64_t)s * 16) * 2]);
+    for (int s = threadIdx.x; s < used; s += kJoinThreads) best = fmaxf(best, stat[(int64_t)s * 2]);
+    best = block_reduce(best, OpMaxF(), smem);
     const float base = best == -__builtin_inff() ? 0.0f : best;
-    float total = 0.0f, value = 0.0f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(a.part_stat[(at + (int64_t)s * 16) * 2] - base);
-        total += f * a.part_stat[(at + (int64_t)s * 16) * 2 + 1];
-        value += f * a.part[(at + (int64_t)s * 16) * D + d];
+    float total = 0.0f;
+    f32x4 value = {0.f, 0.f, 0.f, 0.f};
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    for (int s0 = 0; s0 < used; s0 += kJoinThreads) {
+        const int s = s0 + threadIdx.x;
+        __syncthreads();
+        if (s < used) {
+            const float f = __builtin_amdgcn_exp2f(stat[(int64_t)s * 2] - base);
+            weight[threadIdx.x] = f;
+            total += f * stat[(int64_t)s * 2 + 1];
+        }
+        __syncthreads();
+        const int n = used - s0 < kJoinThreads ? used - s0 : kJoinThreads;
+#pragma unroll 4
+        for (int j = group; j < n; j += kRows) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)(s0 + j) * D + 4 * lane);
+            const float f = weight[j];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) value[r] = __builtin_fmaf(f, v[r], value[r]);
+        }
     }
-    T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot;
-    to[d] = store_cast<T>(total == 0.0f ? 0.0f : value / total);
+    total = block_reduce(total, OpAddF(), smem);
+    sums[group][lane] = value;
+    __syncthreads();
+    if (group) return;
+    for (int j = 1; j < kRows; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) value[r] += sums[j][lane][r];
+    T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * lane;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) to[r] = store_cast<T>(total == 0.0f ? 0.0f : value[r] / total);
 }
 
 // -------------------------------------------------------------------------------------------------------------- host --
@@ -518,39 +704,58 @@ int launch_values(const KvValuesArgs& a, int64_t bh, int32_t dim, hipStream_t s)
     return dim == 64 ? launch_values<T, 64>(a, bh, s) : dim == 128 ? launch_values<T, 128>(a, bh, s) : launch_values<T, 256>(a, bh, s);
 }
 
-// Splits of the token axis: enough workgroups to fill the chip four times over, at least four tiles (one for each wave)
-// to a split.
-inline int32_t attend_splits(int64_t bh, int64_t row_tiles, int64_t tokens) {
+// How a call is shared out.  Few rows (decoding): 16 to a workgroup, whose four waves share the tokens.  More rows: each
+// wave its own 32 (float32 queries, 256 channels: 16), so that a tile of codes is turned into float16 once for all of them.
+// The token axis is split until there are two workgroups for each of the 256 compute units (which is what runs there at
+// once), in one round of equal shares with one length for all sequences; where lengths differ (and are known to the device
+// alone) shares a third as long even them out.  A share is at least four tiles.
+struct AttendPlan { int32_t token_waves, row_tile, splits, split_tiles; };
+inline AttendPlan plan_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q) {
+    const int64_t bh = (int64_t)cache->batch * cache->heads, rows = (int64_t)q->queries * (q->query_heads / cache->heads);
+    const int64_t tokens = q->lengths ? cache->capacity : q->length_all;
     const int64_t tiles = (tokens + kKvTile - 1) / kKvTile;
-    int64_t n = (1024 + bh * row_tiles - 1) / (bh * row_tiles);
-    const int64_t most = (tiles + kAttendWaves - 1) / kAttendWaves;
-    n = n > most ? most : n;
-    return (int32_t)(n < 1 ? 1 : n);
+    AttendPlan p;
+    p.token_waves = rows <= 32 ? 4 : 1;
+    const int wave_rows = q->dtype == AHQ_F32 || cache->head_dim == 256 ? 16 : 32;
+    p.row_tile = p.token_waves == 4 ? 16 : kAttendWaves * wave_rows;
+    const int64_t room = 512 * (q->lengths ? 3 : 1), wgs = bh * ((rows + p.row_tile - 1) / p.row_tile);
+    int64_t n = (wgs * tiles + room - 1) / room;
+    n = (n + 3) / 4 * 4;
+    p.split_tiles = (int32_t)(n < 4 ? 4 : n);
+    n = (tiles + p.split_tiles - 1) / p.split_tiles;
+    p.splits = (int32_t)(n < 1 ? 1 : n);
+    return p;
 }
 
 template <typename T, int D>
-int launch_attend(const KvAttendArgs& a, int64_t bh, hipStream_t s) {
-    constexpr size_t lds = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float);
-    if (lds > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_attend_kernel<T, D>),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
+int launch_attend(const KvAttendArgs& a, const AttendPlan& p, int64_t bh, hipStream_t s) {
+    const dim3 grid((unsigned)((a.rows + p.row_tile - 1) / p.row_tile), (unsigned)bh, (unsigned)p.splits);
+    if (p.token_waves == 4) {
+        constexpr size_t lds = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float);
+        const auto kernel = kv_attend_kernel<T, D, 1, 4>;
+        if (lds > 65536) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
+        }
+        kernel<<<grid, kAttendWaves * kWave, lds, s>>>(a);
+    } else {
+        constexpr int NR = sizeof(T) == 4 || D == 256 ? 1 : 2;
+        kv_attend_kernel<T, D, NR, 1><<<grid, kAttendWaves * kWave, 0, s>>>(a);
     }
-    kv_attend_kernel<T, D><<<dim3(a.splits, a.row_tiles, (unsigned)bh), kAttendWaves * kWave, lds, s>>>(a);
     const int rc = check_launch("ahq_kv_attend");
-    if (rc != AHQ_OK || a.splits == 1) return rc;
-    kv_join_kernel<T, D><<<dim3(a.queries * a.groups, (unsigned)bh), D, 0, s>>>(a);
+    if (rc != AHQ_OK || p.splits == 1) return rc;
+    kv_join_kernel<T, D><<<dim3((unsigned)a.rows, (unsigned)bh), kJoinThreads, 0, s>>>(a);
     return check_launch("ahq_kv_attend");
 }
 template <typename T>
-int launch_attend(const KvAttendArgs& a, int64_t bh, int32_t dim, hipStream_t s) {
-    return dim == 64 ? launch_attend<T, 64>(a, bh, s) : dim == 128 ? launch_attend<T, 128>(a, bh, s) : launch_attend<T, 256>(a, bh, s);
+int launch_attend(const KvAttendArgs& a, const AttendPlan& p, int64_t bh, int32_t dim, hipStream_t s) {
+    return dim == 64 ? launch_attend<T, 64>(a, p, bh, s) : dim == 128 ? launch_attend<T, 128>(a, p, bh, s) : launch_attend<T, 256>(a, p, bh, s);
 }
 
 inline bool attend_shape(const ahq_kv_cache* cache, const ahq_kv_queries* q) {
     if (!q || q->query_heads <= 0 || q->queries < 0) return set_error("bad query shape"), false;
     if (q->query_heads % cache->heads) return set_error("query heads must be a multiple of the cache's heads"), false;
-    if ((int64_t)q->queries * (q->query_heads / cache->heads) > 65535ll * 16) return set_error("too many queries in one call"), false;
+    if ((int64_t)q->queries * (q->query_heads / cache->heads) >= 1ll << 20) return set_error("too many queries in one call"), false;
     return true;
 }
 
@@ -606,10 +811,10 @@ extern "C" int ahq_kv_dequantize(const ahq_kv_cache* cache, int32_t dtype, int32
 extern "C" size_t ahq_kv_attend_workspace_bytes(const ahq_kv_cache* cache, const ahq_kv_queries* q) {
     using namespace ahq;
     if (!check_cache(cache) || !attend_shape(cache, q) || !supported(cache) || q->queries == 0) return 0;
-    const int64_t bh = (int64_t)cache->batch * cache->heads;
-    const int64_t row_tiles = ((int64_t)q->queries * (q->query_heads / cache->heads) + 15) / 16;
-    const int32_t splits = attend_splits(bh, row_tiles, q->lengths ? cache->capacity : q->length_all);
-    return splits == 1 ? 0 : (size_t)(bh * row_tiles * splits * 16) * (cache->head_dim + 2) * sizeof(float);
+    const AttendPlan p = plan_attend(cache, q);
+    if (p.splits == 1) return 0;
+    const size_t rows = (size_t)cache->batch * cache->heads * q->queries * (q->query_heads / cache->heads);
+    return rows * p.splits * (cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q, void* workspace, size_t workspace_bytes,
@@ -626,6 +831,8 @@ extern "C" int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q,
     const int64_t e = q->dtype == AHQ_F32 ? 4 : 2;
     if (((uintptr_t)q->q | (uintptr_t)q->out) % e) return set_error("misaligned tensor"), AHQ_ERR_INVALID;
     const int64_t bh = (int64_t)cache->batch * cache->heads;
+    const AttendPlan p = plan_attend(cache, q);
+    if (p.splits > 65535) return set_error("too many splits of the token axis"), AHQ_ERR_UNSUPPORTED;
     KvAttendArgs a;
     a.q = q->q, a.out = q->out;
     a.qb = q->q_stride_batch, a.qh = q->q_stride_head, a.qt = q->q_stride_query;
@@ -634,14 +841,13 @@ extern "C" int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q,
     a.lengths = q->lengths, a.counts = q->counts, a.length0 = q->length_all, a.count0 = q->count_all;
     a.heads = cache->heads, a.groups = q->query_heads / cache->heads, a.queries = q->queries;
     a.capacity = cache->capacity, a.block = cache->block;
-    a.row_tiles = (int32_t)(((int64_t)a.queries * a.groups + 15) / 16);
-    a.splits = attend_splits(bh, a.row_tiles, q->lengths ? cache->capacity : q->length_all);
+    a.rows = a.queries * a.groups, a.row_tile = p.row_tile, a.splits = p.splits, a.split_tiles = p.split_tiles;
     a.scale = q->scale * 1.44269504088896340736f;
     a.vec = (uintptr_t)q->q % 16 == 0 && a.qb * e % 16 == 0 && a.qh * e % 16 == 0 && a.qt * e % 16 == 0;
     a.part = static_cast<float*>(workspace);
-    a.part_stat = a.part + (size_t)bh * a.row_tiles * a.splits * 16 * cache->head_dim;
+    a.part_stat = a.part + (size_t)bh * a.rows * a.splits * cache->head_dim;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (q->dtype == AHQ_F32) return launch_attend<float>(a, bh, cache->head_dim, s);
-    if (q->dtype == AHQ_F16) return launch_attend<f16_t>(a, bh, cache->head_dim, s);
-    return launch_attend<bf16_t>(a, bh, cache->head_dim, s);
+    if (q->dtype == AHQ_F32) return launch_attend<float>(a, p, bh, cache->head_dim, s);
+    if (q->dtype == AHQ_F16) return launch_attend<f16_t>(a, p, bh, cache->head_dim, s);
+    return launch_attend<bf16_t>(a, p, bh, cache->head_dim, s);
 }

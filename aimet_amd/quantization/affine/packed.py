@@ -33,8 +33,8 @@ def _refuse_gradients(what: str, *tensors) -> None:
 class PackedWeight:
     """The codes of a weight [out_features, in_features] with at most 16 levels, packed for ``packed_linear``.
 
-    Attributes: ``codes`` (uint8, the library's layout), ``scale`` (float32 [groups, out_features padded to 16]),
-    ``zero`` (int8 of the same shape, or None where one zero point serves all), ``zero_const``, ``shape``, ``group``
+    Attributes: ``codes`` (uint8, the library's layout), ``scale`` (float32 [out_features / 16, groups, 16],
+    channels in sixteens and padded to them), ``zero`` (int8 of the same shape, or None where one zero point serves all), ``zero_const``, ``shape``, ``group``
     (columns that share a scale)."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], zero_const: float,
@@ -47,11 +47,19 @@ class PackedWeight:
             raise RuntimeError(f"{tuple(codes.shape)} bytes of {codes.dtype} are no packed weight of shape {self.shape}")
         if self.group <= 0 or k % self.group or (self.group != k and self.group % 32):
             raise RuntimeError(f"groups must be a multiple of 32 columns that divides {k}, or all of them; got {group}")
-        expected = (k // self.group, -(-n // 16) * 16)
+        expected = (-(-n // 16), k // self.group, 16)
         for name, t, dtype in (("scale", scale, torch.float32), ("zero", zero, torch.int8)):
             if t is not None and (tuple(t.shape) != expected or t.dtype != dtype or not t.is_contiguous()
                                   or t.device != codes.device):
                 raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {expected} on {codes.device}")
+        self._struct = _lib.Int4Weight(n, k, self.group, codes.data_ptr(), scale.data_ptr(), _lib.ptr(zero), self.zero_const)
+
+    def __getstate__(self):
+        # the structure handed to the library holds addresses: copies and pickles make their own
+        return {k: v for k, v in self.__dict__.items() if k != "_struct"}
+
+    def __setstate__(self, state):
+        self.__init__(*(state[k] for k in ("codes", "scale", "zero", "zero_const", "shape", "group")))
 
     @property
     def device(self) -> torch.device:
@@ -84,9 +92,14 @@ class PackedWeight:
         if not -128 <= qmin <= 112:
             raise RuntimeError(f"qmin must be in [-128, 112]; got {qmin}")
         npad = -(-n // 16) * 16
-        # the padding repeats nothing: its rows have the scale 0 and are never stored
-        scales = torch.zeros(groups, npad, dtype=torch.float32, device=codes.device)
-        scales[:, :n] = scale.detach().t()
+
+        def in_sixteens(t, dtype):
+            # rows of the padding have the scale 0 and are never stored
+            out = torch.zeros(npad, groups, dtype=dtype, device=codes.device)
+            out[:n] = t
+            return out.view(npad // 16, 16, groups).transpose(1, 2).contiguous()
+
+        scales = in_sixteens(scale.detach(), torch.float32)
         zero, zero_const = None, qmin + float(zero_point_shift)
         if offset is not None:
             off = offset.detach().float()
@@ -98,8 +111,7 @@ class PackedWeight:
             else:
                 if o_lo + qmin < -128 or o_hi + qmin > 127:
                     raise RuntimeError(f"offset + qmin in [{o_lo + qmin}, {o_hi + qmin}] does not fit 8 bits")
-                zero = torch.zeros(groups, npad, dtype=torch.int8, device=codes.device)
-                zero[:, :n] = (off + qmin).t().to(torch.int8)
+                zero = in_sixteens(off + qmin, torch.int8)
                 zero_const = float(zero_point_shift)
         lib = _lib.load()
         nbytes = lib.ahq_int4_packed_bytes(n, k)
@@ -166,8 +178,7 @@ def packed_linear(x: torch.Tensor, weight: PackedWeight, bias: Optional[torch.Te
         rows = rows.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    args = (_lib.DTYPE_CODE[x.dtype], rows.data_ptr(), m, rows.stride(0) if m > 1 else k, weight.codes.data_ptr(), n, k,
-            weight.group, weight.scale.data_ptr(), _lib.ptr(weight.zero), weight.zero_const, _lib.ptr(bias),
+    args = (weight._struct, _lib.DTYPE_CODE[x.dtype], rows.data_ptr(), m, rows.stride(0) if m > 1 else k, _lib.ptr(bias),
             y.data_ptr(), n)
     if device.index == torch.cuda.current_device():
         status = _lib.load().ahq_int4_linear(*args, _lib.current_stream(device))

@@ -48,14 +48,27 @@ class QuantizedKVCache:
         self.batch, self.kv_heads, self.head_dim, self.block_tokens = batch, kv_heads, head_dim, block_tokens
         self.capacity = -(-capacity // 64) * 64  # in whole tiles of 64 tokens
         blocks = self.capacity // block_tokens
-        self.k_codes = torch.zeros(batch, kv_heads, self.capacity, head_dim, dtype=torch.int8, device=device)
+        # bytes hold code + 128
+        self.k_codes = torch.full((batch, kv_heads, self.capacity, head_dim), 128, dtype=torch.uint8, device=device)
         # values lie with the 64 tokens of a tile next to each other, channel by channel
-        self.v_codes = torch.zeros(batch, kv_heads, self.capacity // 64, head_dim, 64, dtype=torch.int8, device=device)
+        self.v_codes = torch.full((batch, kv_heads, self.capacity // 64, head_dim, 64), 128, dtype=torch.uint8, device=device)
         self.k_amax = torch.zeros(batch, kv_heads, blocks, dtype=torch.float32, device=device)
         self.v_amax = torch.zeros(batch, kv_heads, blocks, dtype=torch.float32, device=device)
         self.device = self.k_codes.device
-        self._struct = _lib.KvCache(batch, kv_heads, self.capacity, head_dim, block_tokens, self.k_codes.data_ptr(),
-                                    self.v_codes.data_ptr(), self.k_amax.data_ptr(), self.v_amax.data_ptr())
+        self._bind()
+
+    def _bind(self) -> None:
+        self._struct = _lib.KvCache(self.batch, self.kv_heads, self.capacity, self.head_dim, self.block_tokens,
+                                    self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_amax.data_ptr(),
+                                    self.v_amax.data_ptr())
+
+    def __getstate__(self):
+        # the structure handed to the library holds addresses: copies and pickles make their own
+        return {k: v for k, v in self.__dict__.items() if k != "_struct"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     def _per_sequence(self, n: PerSequence, what: str, most: int) -> Tuple[Optional[int], int]:
         """(device pointer or None, value for all sequences) of a whole number or an int32 tensor [batch]."""

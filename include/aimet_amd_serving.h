@@ -18,35 +18,42 @@ extern "C" {
  * Inference on the codes a calibrated 4-bit weight quantizer describes (AT/nn/fake_quant.py's QuantizedLinear with the
  * weight's encoding applied on the fly instead of a quantize-dequantized copy; no kernel of the reference does this).
  *
- *   y[m][j] = sum_g scale[g][j] * ( sum_{k in group g} x[m][k] * (code[j][k] - qmin + zero[g][j] + zero_const) ) + bias[j]
+ *   y[m][j] = sum_g scale[j][g] * ( sum_{k in group g} x[m][k] * (code[j][k] - qmin + zero[j][g] + zero_const) ) + bias[j]
  *
  * ahq_int4_pack lays out the codes of an [n][k] weight (row-major bytes, each in [qmin, qmin + 15]; only the low four
  * bits of code - qmin are kept) as ahq_int4_linear reads them, ahq_int4_packed_bytes(n, k) bytes (0: bad shape; k is at
  * most 2^20).
  * ahq_int4_linear: x is [m][k] of `dtype` with rows ldx elements apart, y [m][n] with rows ldy apart, both dense along
- * the row.  `group` columns share a scale: a multiple of 32 that divides k, or k.  scale: float [k / group][n rounded
- * up to 16] (the padding is read and not used: any finite value); zero: int8 of the same shape (4-byte reads), or NULL
- * for zero_const alone; both 16-byte aligned.  bias: n values of `dtype`, or NULL.  Products and sums are float32 with
- * exact factors; y is rounded once.  Results do not depend on m or on the other rows' values beyond the order of the sums.
+ * the row; m is at most 2^20.  bias: n values of `dtype`, or NULL.  Products and sums are float32 with exact factors; y is
+ * rounded once.
  */
+typedef struct {
+    int64_t n, k;        /* output and input channels */
+    int64_t group;       /* columns that share a scale: a multiple of 32 that divides k, or k */
+    const void* packed;  /* ahq_int4_pack's output; like scale and zero 16-byte aligned */
+    const float* scale;  /* [ceil(n / 16)][k / group][16]: channel 16 i + j at [i][.][j]; padding: any finite value */
+    const int8_t* zero;  /* same shape, or NULL for zero_const alone */
+    float zero_const;
+} ahq_int4_weight;
+
 size_t ahq_int4_packed_bytes(int64_t n, int64_t k);
 int ahq_int4_pack(const int8_t* codes, int64_t n, int64_t k, int32_t qmin, void* packed, void* stream);
-int ahq_int4_linear(int32_t dtype, const void* x, int64_t m, int64_t ldx, const void* packed, int64_t n, int64_t k,
-                    int64_t group, const float* scale, const int8_t* zero, float zero_const, const void* bias, void* y,
-                    int64_t ldy, void* stream);
+int ahq_int4_linear(const ahq_int4_weight* w, int32_t dtype, const void* x, int64_t m, int64_t ldx, const void* bias,
+                    void* y, int64_t ldy, void* stream);
 
 /* ---------------------------------------------------------------- 8-bit key/value cache ----------------------------
  * A cache of keys and values as codes in [-127, 127] with the largest magnitude (`amax`, float) of every block of
  * `block` tokens (16, 32 or 64) of a sequence and head: a code stands for code * amax / 127 (the symmetric grid of
  * the 8-bit quantizers without its lowest code).  head_dim: 64, 128 or 256; capacity: tokens per sequence, a
- * multiple of 64.  All arrays are the caller's; a new cache is cleared to zero.
+ * multiple of 64.  All arrays are the caller's; a new cache has code bytes 128 (the code 0; a byte holds code + 128) and
+ * maxima 0.
  *   k_codes [batch][heads][capacity][head_dim]
  *   v_codes [batch][heads][capacity / 64][head_dim][64]     (16-byte aligned, as k_codes)
  *   k_amax, v_amax [batch][heads][capacity / block]
  */
 typedef struct {
     int32_t batch, heads, capacity, head_dim, block;
-    int8_t *k_codes, *v_codes;
+    uint8_t *k_codes, *v_codes;
     float *k_amax, *v_amax;
 } ahq_kv_cache;
 

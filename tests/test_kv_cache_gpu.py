@@ -52,7 +52,7 @@ class Model:
 def _codes(cache):
     """Stored codes, keys and values alike as [B, H, C, D]."""
     v = cache.v_codes.transpose(3, 4).reshape(cache.k_codes.shape)
-    return cache.k_codes.cpu().double(), v.cpu().double()
+    return cache.k_codes.cpu().double() - 128, v.cpu().double() - 128
 
 
 def _same(cache, models):
@@ -163,15 +163,17 @@ def test_append_strides(device, dtype):
 
 # -------------------------------------------------------------------------------------------------------- attention --
 def _reference(cache, q, lengths, counts, scale):
-    """(answer, sum of probability times magnitude, largest sum of |q k| of the row), in 64 bits."""
-    k, v = (x.cpu() for x in cache.dequantize())  # exact codes; code * amax / 127 in float32: 2^-23 relative
+    """(answer, sum of probability times magnitude, largest sum of |q k| of the row, largest probability times scale of
+    the values' block), in 64 bits."""
     kc, vc = _codes(cache)
     k = kc * (cache.k_amax.cpu().double() / 127).repeat_interleave(cache.block_tokens, 2)[..., None]
     v = vc * (cache.v_amax.cpu().double() / 127).repeat_interleave(cache.block_tokens, 2)[..., None]
     qd = q.cpu().double()
     b, hq, t, d = qd.shape
     g = hq // cache.kv_heads
-    out, size, most = torch.zeros_like(qd), torch.zeros_like(qd), torch.zeros(b, hq, t, 1, dtype=torch.float64)
+    out, size = torch.zeros_like(qd), torch.zeros_like(qd)
+    most, heavy = torch.zeros(b, hq, t, 1, dtype=torch.float64), torch.zeros(b, hq, t, 1, dtype=torch.float64)
+    v_scale = (cache.v_amax.cpu().double() / 127).repeat_interleave(cache.block_tokens, 2)
     for i in range(b):
         n, c = max(0, min(int(lengths[i]), cache.capacity)), max(0, min(int(counts[i]), t))
         for h in range(hq):
@@ -181,8 +183,9 @@ def _reference(cache, q, lengths, counts, scale):
             p = torch.softmax(s.masked_fill(~seen, -1e300), 1) * seen if n else s
             out[i, h], size[i, h] = p @ v[i, h // g, :n], p @ v[i, h // g, :n].abs()
             if n:
+                heavy[i, h] = (p * v_scale[i, h // g, None, :n]).amax(1, keepdim=True)
                 most[i, h] = (qd[i, h].abs() @ k[i, h // g, :n].abs().T * abs(scale)).amax(1, keepdim=True)
-    return out, size, most
+    return out, size, most, heavy
 
 
 def _attend_check(cache, q, lengths, counts=None, scale=None, given=()):
@@ -190,29 +193,29 @@ def _attend_check(cache, q, lengths, counts=None, scale=None, given=()):
     n = [lengths] * b if isinstance(lengths, int) else lengths
     c = [t] * b if counts is None else [counts] * b if isinstance(counts, int) else counts
     out = cache.attend(q, *(given or (lengths, counts)), scale)
-    want, size, most = _reference(cache, q, n, c, 1 / math.sqrt(d) if scale is None else scale)
+    want, size, most, heavy = _reference(cache, q, n, c, 1 / math.sqrt(d) if scale is None else scale)
     eps = torch.finfo(q.dtype).eps / 2
-    # scores: exact products, float32 sums of d terms (2^-23 each, up to three parts) and three more roundings; a
-    # probability is off by twice that and by 2^-21 of its exponential; the parts keep 16 bits of 16-bit queries'
-    # probabilities (2^-17 left) or all 24; sums of up to 2^-23 a token tile of 32
-    parts = 3 if q.dtype == torch.float32 else 2
+    # scores: queries in full or in two parts of 11 bits (2^-23), float32 sums of d products (2^-23 each) and four more
+    # roundings; a probability is off by twice that and by 2^-19 (exponential, logarithm of the scale); as float16 it is
+    # off by 2^-12 for 16-bit queries, by 2^-23 as two parts; sums of up to 2^-23 a token tile of 32
+    wide = q.dtype == torch.float32
     tiles = cache.capacity / 32
-    score = (33 * parts * d / 32 + 4) * 2.0 ** -23 * most
-    bound = eps * want.abs() + (2 * score + 2.0 ** -20 + (2.0 ** -16 if parts == 2 else 0.0) + (33 * parts + tiles) * 2.0 ** -22) * size
+    score = (33 * (2 if wide else 1) * d / 32 + 5) * 2.0 ** -23 * most
+    bound = eps * want.abs() + (2 * score + 2.0 ** -19 + (2.0 ** -22 if wide else 2.0 ** -11) + (66 + tiles) * 2.0 ** -22) * size
     bound += torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
-    # a probability below 2^-126 of the largest, a part of one (2^-8 of it at least) or its product with a code of at most
-    # 127 may fall below float32's normal numbers and count as 0: at most 2^-126 * 127 of the largest scale a token,
-    # three parts, twice
-    bound += 6 * max(n) * 2.0 ** -126 * 127 * cache.v_amax.double().nan_to_num(0.0, 0.0).max().item()
+    # weights (probability times scale) are float16 numbers of which the largest is at least 2^13: steps of 2^-24 near zero
+    # take away at most half a step, 2^-38 of the largest, for each token, times a code of at most 127
+    bound += max(n) * 2.0 ** -38 * 127 * heavy.nan_to_num(0.0, 0.0)
     err = (out.cpu().double() - want).abs()
     assert out.dtype == q.dtype and out.shape == q.shape
     worst = tuple(x.item() for x in torch.unravel_index((err / bound).argmax(), err.shape))
     assert bool((err <= bound).all()), f"{(err / bound).max().item()} of the bound at {worst}: {out[worst].item()}, {want[worst].item()}"
-    # as many float32 roundings as a random walk, relative to the whole answer; a score's scale is formed by three more
-    # (quotient, two products) of 2^-24, and an error of the score is the same error of the probability, relative to it
+    # the roundings as a random walk, relative to the whole answer: float16's of the weights (rms 2^-12 / sqrt(3) at most),
+    # and for a score the sums' and its scale's (four of 2^-24); an error of the score is the same error of the probability,
+    # relative to it
     if want.norm() > 0:
         rel = err.norm().item() / want.norm().item()
-        assert rel <= eps + (2.0 ** -16 if parts == 2 else 2.0 ** -19) + 4 * 2.0 ** -24 * most.max().item(), rel
+        assert rel <= eps + (2.0 ** -19 if wide else 2.0 ** -12) * max(1.0, (size.norm() / want.norm()).item()) + 5 * 2.0 ** -24 * most.max().item(), rel
     return out
 
 
@@ -313,9 +316,9 @@ def test_attend_does_not_read_behind_the_length(device, queries):
     cache = _filled(1, 1, 200, 64, 32, torch.float32, device)
     q = _queries(1, 2, queries, 64, torch.float32, device)
     want = cache.attend(q, 100)
-    cache.k_codes[:, :, 100:] = 127
-    cache.v_codes[:, :, 2:] = -127
-    cache.v_codes[:, :, 1, :, 36:] = -127
+    cache.k_codes[:, :, 100:] = 255
+    cache.v_codes[:, :, 2:] = 0
+    cache.v_codes[:, :, 1, :, 36:] = 0
     cache.k_amax[:, :, 4:] = float("nan")
     cache.v_amax[:, :, 4:] = float("inf")
     assert torch.equal(cache.attend(q, 100), want)
@@ -356,17 +359,17 @@ def test_offsets_past_32_bits(device):
     k, v = _tokens(1, heads, t, d, torch.float32, 0, device), _tokens(1, heads, t, d, torch.float32, 1, device)
     start = cache.capacity - t
     cache.append(k, v, start)
-    kq, vq = (x[:, :, -64:].clone() for x in (cache.k_codes[:, :, -t:], cache.v_codes[:, :, -1].transpose(2, 3)))
+    kq, vq = (x[:, :, -64:].double() - 128 for x in (cache.k_codes[:, :, -t:], cache.v_codes[:, :, -1].transpose(2, 3)))
     assert bool(kq.any()) and bool(vq.any())
     for h in (0, 31):
         for x, codes, amax in ((k, kq, cache.k_amax), (v, vq, cache.v_amax)):
             want = (x[0, h, -64:].double() * 127 / amax[0, h, -1].double()).round()
-            assert torch.equal(codes[0, h].double(), want)
+            assert torch.equal(codes[0, h], want)
     q = _queries(1, heads, 1, d, torch.float32, device)
     out = cache.attend(q, cache.capacity)
     # all other tokens have the score 0 and the value 0
-    kd = cache.k_codes[0, :, -192:].double() * (cache.k_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
-    vd = cache.v_codes[0, :, -3:].transpose(2, 3).reshape(heads, 192, d).double() * (cache.v_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
+    kd = (cache.k_codes[0, :, -192:].double() - 128) * (cache.k_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
+    vd = (cache.v_codes[0, :, -3:].transpose(2, 3).reshape(heads, 192, d).double() - 128) * (cache.v_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
     s = (kd @ q[0].double().transpose(1, 2))[..., 0] / math.sqrt(d)
     p = torch.exp(s)
     want = (p[:, None] @ vd)[:, 0] / (p.sum(1, keepdim=True) + cache.capacity - 192)
@@ -411,6 +414,17 @@ def test_another_stream_and_graph(device):
     _attend_check(eager, q, other.tolist(), given=(other, None))
 
 
+def test_copies_are_their_own(device):
+    import copy
+
+    cache = _filled(1, 2, 40, 64, 16, torch.float32, device)
+    twin = copy.deepcopy(cache)
+    q = _queries(1, 2, 1, 64, torch.float32, device)
+    want = cache.attend(q, 40)
+    twin.append(_tokens(1, 2, 24, 64, torch.float32, 8, device), _tokens(1, 2, 24, 64, torch.float32, 9, device), 10)
+    assert torch.equal(cache.attend(q, 40), want) and not torch.equal(twin.attend(q, 40), want)
+
+
 def test_refusals(device):
     cache = QuantizedKVCache(2, 2, 128, 64, 32, device)
     k = torch.randn(2, 2, 4, 64, device=device)
@@ -429,7 +443,7 @@ def test_refusals(device):
             cache.append(k, k, 0, counts=counts)
     with pytest.raises(RuntimeError, match="no backward"):
         cache.append(k.clone().requires_grad_(True), k, 0)
-    assert not bool(cache.k_codes.any()) and not bool(cache.v_amax.any())
+    assert bool((cache.k_codes == 128).all()) and not bool(cache.v_amax.any())
     q = torch.randn(2, 4, 1, 64, device=device)
     for bad in (q[:1], q[:, :3], q[:, :0], q[..., :32], q.double(), q[0]):
         with pytest.raises(RuntimeError):

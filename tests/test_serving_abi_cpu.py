@@ -33,7 +33,7 @@ def test_header_and_bindings_agree(lib, tmp_path):
     header = re.sub(r"/\*.*?\*/", "", open(path).read(), flags=re.S)
     declared = set(re.findall(r"\b(ahq_[a-z0-9_]+)\s*\(", header))
     assert declared == set(_lib._SERVING_SIGNATURES) and all(hasattr(lib, name) for name in declared)
-    mirrors = {"ahq_kv_cache": _lib.KvCache, "ahq_kv_tokens": _lib.KvTokens, "ahq_kv_queries": _lib.KvQueries}
+    mirrors = {"ahq_int4_weight": _lib.Int4Weight, "ahq_kv_cache": _lib.KvCache, "ahq_kv_tokens": _lib.KvTokens, "ahq_kv_queries": _lib.KvQueries}
     assert set(re.findall(r"^\} (ahq_\w+);", header, flags=re.M)) == set(mirrors)
     if shutil.which("gcc") is None:
         pytest.skip("no C compiler")
@@ -67,15 +67,16 @@ def test_int4_refusals(lib):
 
     def linear(**kw):
         a = {**good, **kw}
-        return lib.ahq_int4_linear(a["dtype"], a["x"], a["m"], a["ldx"], a["w"], a["n"], a["k"], a["group"], a["scale"],
-                                   a["zero"], a["zc"], a["bias"], a["y"], a["ldy"], None)
+        w = _lib.Int4Weight(a["n"], a["k"], a["group"], a["w"], a["scale"], a["zero"], a["zc"])
+        return lib.ahq_int4_linear(w, a["dtype"], a["x"], a["m"], a["ldx"], a["bias"], a["y"], a["ldy"], None)
 
     for bad in (dict(dtype=3), dict(dtype=-1), dict(x=None), dict(w=None), dict(scale=None), dict(y=None), dict(m=-1),
                 dict(n=0), dict(k=0), dict(ldx=63), dict(ldy=31), dict(group=0), dict(group=48), dict(group=128),
                 dict(w=p + 8), dict(scale=p + 4), dict(zero=p + 2), dict(x=p + 1), dict(y=p + 2), dict(bias=p + 1)):
         assert linear(**bad) == 1, bad
+    assert lib.ahq_int4_linear(None, 0, p, 1, 64, None, p, 32, None) == 1
     assert linear(group=16) == _lib.AHQ_ERR_UNSUPPORTED and b"32" in lib.ahq_last_error()
-    assert linear(m=(1 << 30) + 1) == _lib.AHQ_ERR_UNSUPPORTED
+    assert linear(m=(1 << 20) + 1) == _lib.AHQ_ERR_UNSUPPORTED
     assert linear(m=0, x=None, y=None) == 0
 
 
@@ -136,7 +137,8 @@ def test_attend_workspace(lib):
     long = _cache(capacity=1 << 17)
     need = lib.ahq_kv_attend_workspace_bytes(long, _queries(length=1 << 17))
     assert need > 0 and need % (16 * (64 + 2) * 4) == 0
-    assert lib.ahq_kv_attend_workspace_bytes(long, _queries(lengths=4096)) == need  # by the capacity
+    assert lib.ahq_kv_attend_workspace_bytes(long, _queries(lengths=4096)) >= need  # by the capacity
+    assert lib.ahq_kv_attend_workspace_bytes(long, _queries(length=256)) == 0
     assert lib.ahq_kv_attend(long, _queries(length=1 << 17), None, 0, None) == _lib.AHQ_ERR_WORKSPACE
     assert lib.ahq_kv_attend(long, _queries(length=1 << 17), 4096, need - 1, None) == _lib.AHQ_ERR_WORKSPACE
 
