@@ -1,10 +1,10 @@
 // A key/value cache held in 8 bits, and the attention that reads it.
 //
 // Stored: codes in [-127, 127], as bytes code + 128, and for every block of `block` tokens (16, 32 or 64) of a sequence and
-// head the largest magnitude `amax` among them; a code stands for code * amax / 127.  Keys lie as [sequence, head, token,
-// channel].  Values lie as [sequence, head, tile of 64 tokens, channel, token of the tile]: the product of the
-// probabilities and the values sums over tokens, and a lane of a matrix instruction then finds the 16 tokens it needs of
-// one channel in one 16-byte load.
+// head the largest magnitude `amax` among them; a code stands for code * amax / 127.  Both lie as [sequence, head, tile of
+// 64 tokens], and inside a tile in pieces of 1 KB that one load of a wave takes whole, 16 bytes a lane, in the order of the
+// operands of a 16 x 16 x 32 matrix instruction (key_offset, value_offset): lane 16 c + i of a keys' piece holds 16 channels
+// of one token, of a values' piece 16 tokens of one channel.
 //
 // Writing (kv_append_kernel): a workgroup owns one block of one head.  amax = max(what the block had, |new tokens|), code =
 // rint(127 x / amax), half to even and exact; where amax grows, the codes the block had become rint(code * old / new).
@@ -31,6 +31,18 @@ namespace ahq {
 
 constexpr int kKvTile = 64;
 constexpr int kCodeBias = 128;
+
+// Place of a code in its tile of 64 tokens.  Keys: piece (s, u) holds the channels 64 u .. of the tokens 16 g + 4 s + r, lane
+// 16 c + 4 g + r those from 64 u + 16 c on.  Values: piece u holds the channels 16 u + i, lane 16 c + i the tokens from
+// 16 c on.
+template <int D>
+__device__ __forceinline__ int key_offset(int token, int channel) {
+    const int s = token >> 2 & 3, i = (token >> 4) * 4 + (token & 3);
+    return (((s * (D / 64) + (channel >> 6)) * 4 + (channel >> 4 & 3)) * 16 + i) * 16 + (channel & 15);
+}
+__device__ __forceinline__ int value_offset(int token, int channel) {
+    return (((channel >> 4) * 4 + (token >> 4)) * 16 + (channel & 15)) * 16 + (token & 15);
+}
 
 // ------------------------------------------------------------------------------------------------------------ append --
 struct KvAppendArgs {
@@ -101,7 +113,6 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
     constexpr int kVecs = BT * D / 8;
     constexpr int kThreads = kVecs < 512 ? kVecs : 512;
     constexpr int kItems = kVecs / kThreads;
-    constexpr int kPitch = BT + 4;
     const int which = blockIdx.z;
     const int bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads;
     const TokenRange range = new_tokens(a.start, a.start0, a.counts, a.count0, a.tokens, a.capacity, b);
@@ -152,10 +163,9 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
     const CodeRule rule = code_rule(amax, sizeof(T) == 2);
     const int first = rescale ? 0 : old_end;  // first token whose codes are stored
 
-    uint8_t* keys = a.codes[which] + ((int64_t)bh * a.capacity + p0) * D;
-    // tile of 64 tokens that holds this block, and the block's place in it
-    uint8_t* tile = a.codes[which] + ((int64_t)bh * a.capacity + p0 / kKvTile * kKvTile) * D + p0 % kKvTile;
-    __shared__ alignas(16) uint8_t stage[D * kPitch];
+    uint8_t* tile = a.codes[which] + ((int64_t)bh * a.capacity + p0 / kKvTile * kKvTile) * D;
+    const int t0 = p0 % kKvTile;  // the block's first token in its tile
+    __shared__ alignas(16) uint8_t stage[D * kKvTile];  // an image of the tile
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
         const int id = it * kThreads + threadIdx.x, t = id / (D / 8), d = id % (D / 8) * 8;
@@ -167,32 +177,34 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int q = (which ? tile[(d + e) * kKvTile + t] : keys[(int64_t)t * D + d + e]) - kCodeBias;
+                const int q = tile[which ? value_offset(t0 + t, d + e) : key_offset<D>(t0 + t, d + e)] - kCodeBias;
                 out.b[e] = (uint8_t)((int)__builtin_rint((double)q * (double)before / (double)amax) + kCodeBias);
             }
         }
         if (which == 0) {
-            *reinterpret_cast<u32x2_t*>(keys + (int64_t)t * D + d) = out.w;
+            *reinterpret_cast<u32x2_t*>(stage + key_offset<D>(t0 + t, d)) = out.w;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) stage[(d + e) * kPitch + t] = out.b[e];
+            for (int e = 0; e < 8; ++e) stage[value_offset(t0 + t, d + e)] = out.b[e];
         }
     }
-    if (which == 1) {
-        __syncthreads();
-        for (int id = threadIdx.x; id < D * (BT / 16); id += kThreads) {
-            const int d = id / (BT / 16), t = id % (BT / 16) * 16;
-            const uint32_t* from = reinterpret_cast<const uint32_t*>(stage + d * kPitch + t);
-            uint8_t* to = tile + d * kKvTile + t;
+    __syncthreads();
+    // 16 bytes at a time: 16 channels of a token, or 16 tokens of a channel
+    for (int id = threadIdx.x; id < D * BT / 16; id += kThreads) {
+        if (which == 0) {
+            const int t = id % BT, at = key_offset<D>(t0 + t, id / BT * 16);
+            if (t >= first && t < new_end) *reinterpret_cast<u32x4_t*>(tile + at) = *reinterpret_cast<const u32x4_t*>(stage + at);
+        } else {
+            const int t = id / D * 16, at = value_offset(t0 + t, id % D);
             if (first <= t && t + 16 <= new_end) {
-                *reinterpret_cast<u32x4_t*>(to) = u32x4_t{from[0], from[1], from[2], from[3]};
+                *reinterpret_cast<u32x4_t*>(tile + at) = *reinterpret_cast<const u32x4_t*>(stage + at);
             } else {
                 for (int e = 0; e < 16; ++e)
-                    if (t + e >= first && t + e < new_end) to[e] = stage[d * kPitch + t + e];
+                    if (t + e >= first && t + e < new_end) tile[at + e] = stage[at + e];
             }
         }
     }
-    // read by other threads before the first barrier above, so it is written behind the last one
+    // read by all threads before the first barrier above, so it is written behind one
     if (threadIdx.x == 0) *amax_at = amax;
 }
 
@@ -206,23 +218,16 @@ struct KvValuesArgs {
 
 template <typename T, int D>
 __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
-    constexpr int kPitch = kKvTile + 4;
     const int which = blockIdx.z, tile = blockIdx.x;
     const int64_t bh = blockIdx.y;
     const int p0 = tile * kKvTile;
     const uint8_t* codes = a.codes[which] + (bh * a.capacity + p0) * D;
     const float* amax = a.amax[which] + bh * (a.capacity / a.block);
     T* out = static_cast<T*>(a.out[which]) + (bh * a.length + p0) * D;
-    __shared__ alignas(16) uint8_t stage[D * kPitch];
-    if (which) {
-        for (int id = threadIdx.x; id < D * 4; id += kBlock) {
-            const u32x4_t w = *reinterpret_cast<const u32x4_t*>(codes + id * 16);
-            uint32_t* to = reinterpret_cast<uint32_t*>(stage + id / 4 * kPitch + id % 4 * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) to[e] = w[e];
-        }
-        __syncthreads();
-    }
+    __shared__ alignas(16) uint8_t stage[D * kKvTile];
+    for (int id = threadIdx.x; id < D * 4; id += kBlock)
+        *reinterpret_cast<u32x4_t*>(stage + id * 16) = *reinterpret_cast<const u32x4_t*>(codes + id * 16);
+    __syncthreads();
     for (int id = threadIdx.x; id < kKvTile * (D / 8); id += kBlock) {
         const int t = id / (D / 8), d = id % (D / 8) * 8;
         if (p0 + t >= a.length) break;
@@ -230,9 +235,9 @@ __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
         union { uint8_t b[8]; u32x2_t w; } in;
         if (which) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) in.b[e] = stage[(d + e) * kPitch + t];
+            for (int e = 0; e < 8; ++e) in.b[e] = stage[value_offset(t, d + e)];
         } else {
-            in.w = *reinterpret_cast<const u32x2_t*>(codes + (int64_t)t * D + d);
+            in.w = *reinterpret_cast<const u32x2_t*>(stage + key_offset<D>(t, d));
         }
         constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
@@ -255,11 +260,12 @@ struct KvAttendArgs {
     const int32_t* lengths;  // null: length0
     const int32_t* counts;   // null: count0
     int32_t length0, count0;
-    int32_t heads, groups, queries, capacity, block;
+    int32_t heads, groups, queries, capacity, block_shift;
     int32_t rows, row_tile;       // queries * groups; rows of a workgroup
     int32_t splits, split_tiles;  // splits of the token axis, token tiles of each
     float scale;                  // of the scores, times log2(e)
     int32_t vec;                  // rows of q start on 16-byte boundaries
+    int32_t stream;               // the codes are more than the caches keep: non-temporal loads
     float* part;                  // [sequence * head][row][split][D], then [..][row][split][2]: reference and sum
     float* part_stat;
 };
@@ -341,31 +347,34 @@ struct AttendRows {
             last[n] = row < a.rows && t < seq.count ? seq.length - seq.count + t : -1;
             const bool live = last[n] >= 0;
             if (live && last[n] < least) least = last[n];
-            const T* at = static_cast<const T*>(a.q) + b * a.qb + (int64_t)(h * a.groups + row % a.groups) * a.qh + (int64_t)t * a.qt;
+            // rows that see nothing read the first query's place and count as zero
+            const T* at = static_cast<const T*>(a.q) + b * a.qb + (int64_t)(h * a.groups + (live ? row % a.groups : 0)) * a.qh + (int64_t)(live ? t : 0) * a.qt + 16 * c;
             float v[kSteps][8];
+            if (a.vec) {
+                constexpr int kPer = 16 / sizeof(T);
+                Pack<T, kPer> raw[kSteps][8 / kPer];
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int u = 0; u < 8 / kPer; ++u) raw[s][u] = load_pack<T, kPer>(at + 64 * (s / 2) + 8 * (s % 2) + u * kPer);
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[s][e] = load_f32(raw[s][e / kPer].v[e % kPer]);
+            } else {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[s][e] = load_f32(at[64 * (s / 2) + 8 * (s % 2) + e]);
+            }
             float size = 0.0f;
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const T* p = at + 64 * (s / 2) + 16 * c + 8 * (s % 2);
+            for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[s][e] = 0.0f;
-                if (live) {
-                    constexpr int kPer = 16 / sizeof(T);
-                    if (a.vec) {
-#pragma unroll
-                        for (int u = 0; u < 8 / kPer; ++u) {
-                            const Pack<T, kPer> w = load_pack<T, kPer>(p + u * kPer);
-#pragma unroll
-                            for (int e = 0; e < kPer; ++e) v[s][u * kPer + e] = load_f32(w.v[e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[s][e] = load_f32(p[e]);
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    v[s][e] = live ? v[s][e] : 0.0f;
+                    size = fmaxf(size, fabsf(v[s][e]));
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) size = fmaxf(size, fabsf(v[s][e]));
-            }
             size = fmaxf(size, __shfl_xor(size, 16, kWave));
             size = fmaxf(size, __shfl_xor(size, 32, kWave));
             // exponent of the largest value; zeros, infinities and the smallest numbers go as they are
@@ -395,10 +404,10 @@ struct AttendRows {
     // One tile of 64 tokens; `prefetch` is called once the tile's keys and scales are no longer needed.
     template <typename Prefetch>
     __device__ __forceinline__ void work(const KvTile<D>& tile, const u32x4_t* values, int p0, int c, Prefetch prefetch) {
-        const float k_scale = tile.k_amax / 127.0f;
-        const float v_scale = fmaxf(tile.v_amax / 127.0f, kLeastScale);
+        const float k_scale = tile.k_amax * (1.0f / 127.0f);
+        const float v_scale = fmaxf(tile.v_amax * (1.0f / 127.0f), kLeastScale);
         const float v_log = __builtin_amdgcn_logf(v_scale);
-        const float v_inverse = 1.0f / v_scale;
+        const float v_inverse = __builtin_amdgcn_rcpf(v_scale);
         f32x4 x[4][NR];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -485,10 +494,13 @@ struct AttendRows {
 // TOKEN_WAVES = 4: the waves of a workgroup share its 16 * NR rows and take their token tiles in turn (few rows, long
 // caches: bound by the stream of codes); 1: each wave has 16 * NR rows of its own and all the tokens (prompts: bound by the
 // matrix cores and the vector work around them).
+#ifndef OCC
+#define OCC 2
+#endif
 template <typename T, int D, int NR, int TOKEN_WAVES>
-__global__ __launch_bounds__(kAttendWaves * kWave) void kv_attend_kernel(KvAttendArgs a) {
+__global__ __launch_bounds__(kAttendWaves * kWave, D * NR <= 128 ? OCC : 1) void kv_attend_kernel(KvAttendArgs a) {
     constexpr int kOut = D / 16;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i = lane & 15, c = lane >> 4;
     const int64_t bh = blockIdx.y;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
@@ -503,35 +515,40 @@ __global__ __launch_bounds__(kAttendWaves * kWave) void kv_attend_kernel(KvAtten
     const int first = split * a.split_tiles + (TOKEN_WAVES == 1 ? 0 : wave);
     const int stop = (split + 1) * a.split_tiles < tiles ? (split + 1) * a.split_tiles : tiles;
 
-    AttendRows<T, D, NR> rows;
-    rows.begin(a, seq, b, h, row0, i, c);
-    const uint8_t* keys = a.k_codes + bh * a.capacity * D + 16 * c;
-    const uint8_t* values = a.v_codes + bh * a.capacity * D + i * kKvTile + 16 * c;
-    const float* k_amax = a.k_amax + bh * (a.capacity / a.block);
-    const float* v_amax = a.v_amax + bh * (a.capacity / a.block);
-    const int key_row = (i >> 2) * 16 + (i & 3);  // token of A row i in the score tile s: key_row + 4 s
+    // addresses: a scalar base for the tile, an offset of the lane and constants
+    const uint8_t* keys = a.k_codes + bh * a.capacity * D;
+    const uint8_t* values = a.v_codes + bh * a.capacity * D;
+    const float* k_amax = a.k_amax + bh * (a.capacity >> a.block_shift);
+    const float* v_amax = a.v_amax + bh * (a.capacity >> a.block_shift);
+    const int amax_at = 16 * c >> a.block_shift;
 
     // Keys of the next tile and values of this one are asked for before the work on this one begins.
     KvTile<D> next;
+    const auto piece = [&](const uint8_t* from, int n) {
+        const u32x4_t* at = reinterpret_cast<const u32x4_t*>(from + (lane * 16 + n * 1024));
+        return a.stream ? __builtin_nontemporal_load(at) : *at;
+    };
     const auto load = [&](int tile) {
-        const int block_at = (tile * kKvTile + 16 * c) / a.block;
-        next.k_amax = k_amax[block_at];
-        next.v_amax = v_amax[block_at];
+        const float* ks = k_amax + ((int64_t)tile * kKvTile >> a.block_shift);
+        const float* vs = v_amax + ((int64_t)tile * kKvTile >> a.block_shift);
+        next.k_amax = ks[amax_at];
+        next.v_amax = vs[amax_at];
+        const uint8_t* from = keys + (int64_t)tile * (kKvTile * D);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int u = 0; u < D / 64; ++u)
-                next.keys[s][u] = *reinterpret_cast<const u32x4_t*>(keys + (int64_t)(tile * kKvTile + key_row + 4 * s) * D + 64 * u);
+            for (int u = 0; u < D / 64; ++u) next.keys[s][u] = piece(from, s * (D / 64) + u);
     };
     if (first < stop) load(first);
+    AttendRows<T, D, NR> rows;
+    rows.begin(a, seq, b, h, row0, i, c);
     for (int tile = first; tile < stop; tile += TOKEN_WAVES) {
         u32x4_t vw[kOut];
+        const uint8_t* from = values + (int64_t)tile * (kKvTile * D);
 #pragma unroll
-        for (int u = 0; u < kOut; ++u)
-            vw[u] = *reinterpret_cast<const u32x4_t*>(values + (int64_t)tile * kKvTile * D + 16 * u * kKvTile);
-        rows.work(next, vw, tile * kKvTile, c, [&] {
-            if (tile + TOKEN_WAVES < stop) load(tile + TOKEN_WAVES);
-        });
+        for (int u = 0; u < kOut; ++u) vw[u] = piece(from, u);
+        // behind the last tile that one is loaded again: a load that may be left out would have to be waited for at once
+        rows.work(next, vw, tile * kKvTile, c, [&] { load(tile + TOKEN_WAVES < stop ? tile + TOKEN_WAVES : tile); });
     }
     float sum[NR];
 #pragma unroll
@@ -840,10 +857,11 @@ extern "C" int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q,
     a.k_codes = cache->k_codes, a.v_codes = cache->v_codes, a.k_amax = cache->k_amax, a.v_amax = cache->v_amax;
     a.lengths = q->lengths, a.counts = q->counts, a.length0 = q->length_all, a.count0 = q->count_all;
     a.heads = cache->heads, a.groups = q->query_heads / cache->heads, a.queries = q->queries;
-    a.capacity = cache->capacity, a.block = cache->block;
+    a.capacity = cache->capacity, a.block_shift = cache->block == 16 ? 4 : cache->block == 32 ? 5 : 6;
     a.rows = a.queries * a.groups, a.row_tile = p.row_tile, a.splits = p.splits, a.split_tiles = p.split_tiles;
     a.scale = q->scale * 1.44269504088896340736f;
     a.vec = (uintptr_t)q->q % 16 == 0 && a.qb * e % 16 == 0 && a.qh * e % 16 == 0 && a.qt * e % 16 == 0;
+    a.stream = bh * a.capacity * cache->head_dim >= kStreamLoadBytes;
     a.part = static_cast<float*>(workspace);
     a.part_stat = a.part + (size_t)bh * a.rows * a.splits * cache->head_dim;
     const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -48,10 +48,11 @@ class QuantizedKVCache:
         self.batch, self.kv_heads, self.head_dim, self.block_tokens = batch, kv_heads, head_dim, block_tokens
         self.capacity = -(-capacity // 64) * 64  # in whole tiles of 64 tokens
         blocks = self.capacity // block_tokens
-        # bytes hold code + 128
-        self.k_codes = torch.full((batch, kv_heads, self.capacity, head_dim), 128, dtype=torch.uint8, device=device)
-        # values lie with the 64 tokens of a tile next to each other, channel by channel
-        self.v_codes = torch.full((batch, kv_heads, self.capacity // 64, head_dim, 64), 128, dtype=torch.uint8, device=device)
+        # bytes hold code + 128, a tile of 64 tokens in the order in which the matrix cores take it
+        self.k_codes = torch.full((batch, kv_heads, self.capacity // 64, 4, head_dim // 64, 4, 16, 16), 128,
+                                  dtype=torch.uint8, device=device)
+        self.v_codes = torch.full((batch, kv_heads, self.capacity // 64, head_dim // 16, 4, 16, 16), 128,
+                                  dtype=torch.uint8, device=device)
         self.k_amax = torch.zeros(batch, kv_heads, blocks, dtype=torch.float32, device=device)
         self.v_amax = torch.zeros(batch, kv_heads, blocks, dtype=torch.float32, device=device)
         self.device = self.k_codes.device
@@ -103,6 +104,13 @@ class QuantizedKVCache:
             with torch.cuda.device(self.device):
                 status = fn(*args, _lib.current_stream(self.device))
         _lib.check(status, name)
+
+    def codes(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The stored codes of keys and values as two int8 tensors [batch, kv_heads, capacity, head_dim]."""
+        shape = (self.batch, self.kv_heads, self.capacity, self.head_dim)
+        k = self.k_codes.unflatten(6, (4, 4)).permute(0, 1, 2, 6, 3, 7, 4, 5, 8)  # tile, g, s, r, u, c, e
+        v = self.v_codes.permute(0, 1, 2, 4, 6, 3, 5)                             # tile, c, e, u, i
+        return tuple((x.reshape(shape).to(torch.int16) - 128).to(torch.int8) for x in (k, v))
 
     def append(self, k: torch.Tensor, v: torch.Tensor, start: PerSequence,
                counts: Optional[PerSequence] = None) -> None:

@@ -47,8 +47,10 @@ int ahq_int4_linear(const ahq_int4_weight* w, int32_t dtype, const void* x, int6
  * the 8-bit quantizers without its lowest code).  head_dim: 64, 128 or 256; capacity: tokens per sequence, a
  * multiple of 64.  All arrays are the caller's; a new cache has code bytes 128 (the code 0; a byte holds code + 128) and
  * maxima 0.
- *   k_codes [batch][heads][capacity][head_dim]
- *   v_codes [batch][heads][capacity / 64][head_dim][64]     (16-byte aligned, as k_codes)
+ *   k_codes [batch][heads][capacity / 64][4][head_dim / 64][4][16][16]: [.][s][u][c][4 g + r][e] is token 16 g + 4 s + r of
+ *           the tile of 64, channel 64 u + 16 c + e
+ *   v_codes [batch][heads][capacity / 64][head_dim / 16][4][16][16]: [.][u][c][i][e] is token 16 c + e, channel 16 u + i
+ *           (both 16-byte aligned)
  *   k_amax, v_amax [batch][heads][capacity / block]
  */
 typedef struct {

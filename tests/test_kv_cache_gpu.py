@@ -50,9 +50,8 @@ class Model:
 
 
 def _codes(cache):
-    """Stored codes, keys and values alike as [B, H, C, D]."""
-    v = cache.v_codes.transpose(3, 4).reshape(cache.k_codes.shape)
-    return cache.k_codes.cpu().double() - 128, v.cpu().double() - 128
+    """Stored codes of keys and values in 64 bits, [B, H, C, D]."""
+    return tuple(x.cpu().double() for x in cache.codes())
 
 
 def _same(cache, models):
@@ -158,7 +157,8 @@ def test_append_strides(device, dtype):
         assert torch.equal(cache.k_codes, want.k_codes) and torch.equal(cache.v_codes, want.v_codes)
     # one token for all heads and sequences
     cache.append(k[:1, :1, :1].expand(b, h, 1, d), v[:1, :1, :1].expand(b, h, 1, d), 32)
-    assert torch.equal(cache.k_codes[1, 2, 32], cache.k_codes[0, 0, 32]) and bool(cache.k_codes[0, 0, 32].any())
+    k, _ = cache.codes()
+    assert torch.equal(k[1, 2, 32], k[0, 0, 32]) and bool(k[0, 0, 32].any())
 
 
 # -------------------------------------------------------------------------------------------------------- attention --
@@ -316,9 +316,12 @@ def test_attend_does_not_read_behind_the_length(device, queries):
     cache = _filled(1, 1, 200, 64, 32, torch.float32, device)
     q = _queries(1, 2, queries, 64, torch.float32, device)
     want = cache.attend(q, 100)
-    cache.k_codes[:, :, 100:] = 255
+    cache.k_codes[:, :, 2:] = 255  # tokens from 128 on
     cache.v_codes[:, :, 2:] = 0
-    cache.v_codes[:, :, 1, :, 36:] = 0
+    cache.k_codes[:, :, 1, :, :, :, 12:] = 255  # tokens 112 to 127
+    cache.v_codes[:, :, 1, :, 3] = 0
+    cache.k_codes[:, :, 1, 1:, :, :, 8:12] = 255  # tokens 100 to 111
+    cache.v_codes[:, :, 1, :, 2, :, 4:] = 0
     cache.k_amax[:, :, 4:] = float("nan")
     cache.v_amax[:, :, 4:] = float("inf")
     assert torch.equal(cache.attend(q, 100), want)
@@ -359,7 +362,10 @@ def test_offsets_past_32_bits(device):
     k, v = _tokens(1, heads, t, d, torch.float32, 0, device), _tokens(1, heads, t, d, torch.float32, 1, device)
     start = cache.capacity - t
     cache.append(k, v, start)
-    kq, vq = (x[:, :, -64:].double() - 128 for x in (cache.k_codes[:, :, -t:], cache.v_codes[:, :, -1].transpose(2, 3)))
+    end = QuantizedKVCache(1, heads, 192, d, 64, device)  # the last three tiles
+    end.k_codes, end.v_codes = cache.k_codes[:, :, -3:], cache.v_codes[:, :, -3:]
+    kd, vd = (x[0].double() for x in end.codes())
+    kq, vq = kd[None, :, -64:], vd[None, :, -64:]
     assert bool(kq.any()) and bool(vq.any())
     for h in (0, 31):
         for x, codes, amax in ((k, kq, cache.k_amax), (v, vq, cache.v_amax)):
@@ -368,8 +374,8 @@ def test_offsets_past_32_bits(device):
     q = _queries(1, heads, 1, d, torch.float32, device)
     out = cache.attend(q, cache.capacity)
     # all other tokens have the score 0 and the value 0
-    kd = (cache.k_codes[0, :, -192:].double() - 128) * (cache.k_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
-    vd = (cache.v_codes[0, :, -3:].transpose(2, 3).reshape(heads, 192, d).double() - 128) * (cache.v_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
+    kd = kd * (cache.k_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
+    vd = vd * (cache.v_amax[0, :, -3:].double() / 127).repeat_interleave(64, 1)[..., None]
     s = (kd @ q[0].double().transpose(1, 2))[..., 0] / math.sqrt(d)
     p = torch.exp(s)
     want = (p[:, None] @ vd)[:, 0] / (p.sum(1, keepdim=True) + cache.capacity - 192)
