@@ -265,7 +265,7 @@ struct KvAttendArgs {
     int32_t splits, split_tiles;  // splits of the token axis, token tiles of each
     float scale;                  // of the scores, times log2(e)
     int32_t vec;                  // rows of q start on 16-byte boundaries
-    int32_t stream;               // the codes are more than the caches keep: non-temporal loads
+    int32_t vec_out;              // rows of the answers start on boundaries of four elements
     float* part;                  // [sequence * head][row][split][D], then [..][row][split][2]: reference and sum
     float* part_stat;
 };
@@ -319,13 +319,6 @@ __device__ __forceinline__ void split_f16(const float* v, f16x8* out) {
 constexpr float kTop = 14.0f;                 // log2 of the largest weight
 constexpr float kLeastScale = 0x1p-80f;
 constexpr int kAttendWaves = 4;
-
-// Loads are waited for in the order they were asked for, so a tile's scales come in front of its keys.
-template <int D>
-struct KvTile {
-    u32x4_t keys[4][D / 64];
-    float k_amax, v_amax;
-};
 
 // What a wave knows of its 16 * NR rows; a lane holds row 16 n + i of them and the channels 16 u + 4 c + r of its answer.
 template <typename T, int D, int NR>
@@ -401,11 +394,12 @@ struct AttendRows {
         least = __builtin_amdgcn_readfirstlane(least);
     }
 
-    // One tile of 64 tokens; `prefetch` is called once the tile's keys and scales are no longer needed.
-    template <typename Prefetch>
-    __device__ __forceinline__ void work(const KvTile<D>& tile, const u32x4_t* values, int p0, int c, Prefetch prefetch) {
-        const float k_scale = tile.k_amax * (1.0f / 127.0f);
-        const float v_scale = fmaxf(tile.v_amax * (1.0f / 127.0f), kLeastScale);
+    // One tile of 64 tokens from p0 on: `key` and `value` give a lane's 16 bytes of a piece, `between` is called once the
+    // keys and scales are no longer needed.
+    template <typename Key, typename Value, typename Between>
+    __device__ __forceinline__ void work(Key key, Value value, float k_amax, float v_amax, int p0, int c, Between between) {
+        const float k_scale = k_amax * (1.0f / 127.0f);
+        const float v_scale = fmaxf(v_amax * (1.0f / 127.0f), kLeastScale);
         const float v_log = __builtin_amdgcn_logf(v_scale);
         const float v_inverse = __builtin_amdgcn_rcpf(v_scale);
         f32x4 x[4][NR];
@@ -414,16 +408,19 @@ struct AttendRows {
 #pragma unroll
             for (int n = 0; n < NR; ++n) x[s][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < kSteps; ++u) {
-                const u32x4_t w = tile.keys[s][u / 2];
-                const f16x8 kf = u % 2 ? codes_to_f16(w[2], w[3]) : codes_to_f16(w[0], w[1]);
+            for (int u = 0; u < D / 64; ++u) {
+                const u32x4_t w = key(s, u);
 #pragma unroll
-                for (int n = 0; n < NR; ++n)
+                for (int half = 0; half < 2; ++half) {
+                    const f16x8 kf = codes_to_f16(w[2 * half], w[2 * half + 1]);
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf, q[u][n][p], x[s][n]);
+                    for (int n = 0; n < NR; ++n)
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf, q[2 * u + half][n][p], x[s][n]);
+                }
             }
         }
-        prefetch();
+        between();
         f16x8 pf[2][NR][kParts];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -479,7 +476,8 @@ struct AttendRows {
         }
 #pragma unroll
         for (int u = 0; u < kOut; ++u) {
-            const f16x8 v0 = codes_to_f16(values[u][0], values[u][1]), v1 = codes_to_f16(values[u][2], values[u][3]);
+            const u32x4_t w = value(u);
+            const f16x8 v0 = codes_to_f16(w[0], w[1]), v1 = codes_to_f16(w[2], w[3]);
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -491,15 +489,153 @@ struct AttendRows {
     }
 };
 
-// TOKEN_WAVES = 4: the waves of a workgroup share its 16 * NR rows and take their token tiles in turn (few rows, long
-// caches: bound by the stream of codes); 1: each wave has 16 * NR rows of its own and all the tokens (prompts: bound by the
-// matrix cores and the vector work around them).
-#ifndef OCC
-#define OCC 2
-#endif
-template <typename T, int D, int NR, int TOKEN_WAVES>
-__global__ __launch_bounds__(kAttendWaves * kWave, D * NR <= 128 ? OCC : 1) void kv_attend_kernel(KvAttendArgs a) {
+// The rows' answers, or their share of them where the token axis is split: from a wave's registers.
+template <typename T, int D, int NR>
+__device__ __forceinline__ void store_rows(const KvAttendArgs& a, const AttendRows<T, D, NR>& rows, const float* sum, int64_t bh,
+                                           int row0, int split, bool whole, int i, int c) {
+    const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int row = row0 + 16 * n + i;
+        if (row >= a.rows) continue;
+        if (whole) {
+            const float inverse = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+            T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * c;
+#pragma unroll
+            for (int u = 0; u < D / 16; ++u) {
+                Pack<T, 4> out;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out.v[r] = store_cast<T>(sum[n] == 0.0f ? 0.0f : rows.o[u][n][r] * inverse);
+                if (a.vec_out) {
+                    store_pack<T, 4>(to + 16 * u, out);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) to[16 * u + r] = out.v[r];
+                }
+            }
+        } else {
+            const int64_t at = (bh * a.rows + row) * a.splits + split;
+#pragma unroll
+            for (int u = 0; u < D / 16; ++u) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * u + 4 * c) = rows.o[u][n];
+            if (c == 0) a.part_stat[at * 2] = rows.reference[n], a.part_stat[at * 2 + 1] = sum[n];
+        }
+    }
+}
+
+// Sums over the lanes of a row; rows that saw nothing have the reference -infinity and the sum 0.
+template <typename T, int D, int NR>
+__device__ __forceinline__ void finish_rows(AttendRows<T, D, NR>& rows, float* sum) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        sum[n] = rows.sum[n];
+        sum[n] += __shfl_xor(sum[n], 16, kWave);
+        sum[n] += __shfl_xor(sum[n], 32, kWave);
+        if (rows.last[n] < 0) sum[n] = 0.0f;
+        if (rows.top[n] != kTop) rows.reference[n] = -__builtin_inff();
+    }
+}
+
+// Few rows, long caches (decoding): the four waves of a workgroup share its 16 rows and take their token tiles in turn.
+// Bound by the stream of codes: keys of the next tile and values of this one are asked for before the work on this one
+// begins.  STREAM: the codes are more than the caches keep, so they are read past them.
+template <typename T, int D, bool STREAM>
+__global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_attend_kernel(KvAttendArgs a) {
     constexpr int kOut = D / 16;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int i = lane & 15, c = lane >> 4;
+    const int64_t bh = blockIdx.y;
+    const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+    const int split = blockIdx.z, row0 = blockIdx.x * 16;
+    const SequenceView seq = view_sequence(a, b);
+    const int used = used_splits(a, seq, row0);
+    if (split >= used && split > 0) return;
+
+    const int tiles = seen_tiles(a, seq, row0 + 15);
+    const int first = split * a.split_tiles + wave;
+    const int stop = (split + 1) * a.split_tiles < tiles ? (split + 1) * a.split_tiles : tiles;
+    const uint8_t* keys = a.k_codes + bh * a.capacity * D;
+    const uint8_t* values = a.v_codes + bh * a.capacity * D;
+    const float* k_amax = a.k_amax + bh * (a.capacity >> a.block_shift);
+    const float* v_amax = a.v_amax + bh * (a.capacity >> a.block_shift);
+    const int amax_at = 16 * c >> a.block_shift;
+
+    // Loads are waited for in the order they were asked for, so a tile's scales come in front of its keys.
+    u32x4_t kw[4][D / 64];
+    float k_next = 0.0f, v_next = 0.0f;
+    const auto piece = [&](const uint8_t* from, int n) {
+        const u32x4_t* at = reinterpret_cast<const u32x4_t*>(from + (lane * 16 + n * 1024));
+        if constexpr (STREAM) return __builtin_nontemporal_load(at);
+        else return *at;
+    };
+    const auto load = [&](int tile) {
+        k_next = k_amax[((int64_t)tile * kKvTile >> a.block_shift) + amax_at];
+        v_next = v_amax[((int64_t)tile * kKvTile >> a.block_shift) + amax_at];
+        const uint8_t* from = keys + (int64_t)tile * (kKvTile * D);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int u = 0; u < D / 64; ++u) kw[s][u] = piece(from, s * (D / 64) + u);
+    };
+    if (first < stop) load(first);
+    AttendRows<T, D, 1> rows;
+    rows.begin(a, seq, b, h, row0, i, c);
+    for (int tile = first; tile < stop; tile += kAttendWaves) {
+        u32x4_t vw[kOut];
+        const uint8_t* from = values + (int64_t)tile * (kKvTile * D);
+#pragma unroll
+        for (int u = 0; u < kOut; ++u) vw[u] = piece(from, u);
+        // behind the last tile that one is loaded again: a load that may be left out would have to be waited for at once
+        rows.work([&](int s, int u) { return kw[s][u]; }, [&](int u) { return vw[u]; }, k_next, v_next, tile * kKvTile, c,
+                  [&] { load(tile + kAttendWaves < stop ? tile + kAttendWaves : tile); });
+    }
+    float sum[1];
+    finish_rows(rows, sum);
+
+    // the waves' results are joined through LDS, in wave order
+    constexpr int kPitch = 17;
+    extern __shared__ float joined[];  // [wave][D][17], then [wave][16][2]
+    float* stats = joined + kAttendWaves * D * kPitch;
+#pragma unroll
+    for (int u = 0; u < kOut; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) joined[(wave * D + 16 * u + 4 * c + r) * kPitch + i] = rows.o[u][0][r];
+    if (c == 0) stats[(wave * 16 + i) * 2] = rows.reference[0], stats[(wave * 16 + i) * 2 + 1] = sum[0];
+    __syncthreads();
+    for (int id = threadIdx.x; id < 16 * D; id += kAttendWaves * kWave) {
+        const int rr = id / D, d = id % D;
+        const int row = row0 + rr;
+        if (row >= a.rows) break;
+        float best = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < kAttendWaves; ++w) best = fmaxf(best, stats[(w * 16 + rr) * 2]);
+        const float base = best == -__builtin_inff() ? 0.0f : best;
+        float total = 0.0f, value = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttendWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(stats[(w * 16 + rr) * 2] - base);
+            total += f * stats[(w * 16 + rr) * 2 + 1];
+            value += f * joined[(w * D + d) * kPitch + rr];
+        }
+        if (used <= 1) {
+            T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot;
+            to[d] = store_cast<T>(total == 0.0f ? 0.0f : value / total);
+        } else {
+            const int64_t at = (bh * a.rows + row) * a.splits + split;
+            a.part[at * D + d] = value;
+            if (d == 0) a.part_stat[at * 2] = best, a.part_stat[at * 2 + 1] = total;
+        }
+    }
+}
+
+// Many rows (prompts): each wave has 16 * NR rows of its own, and the workgroup takes the token tiles one after the other
+// through two LDS buffers; the next tile is on its way to registers while this one is worked on.  Bound by the vector
+// work between the two products (conversion of codes, exponentials).
+template <typename T, int D, int NR, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArgs a) {
+    constexpr int kThreads = WAVES * kWave;
+    constexpr int kPieces = D * kKvTile / 16;             // of 16 bytes, of keys and of values each
+    constexpr int kPer = 2 * kPieces / kThreads;
+    static_assert(2 * kPieces % kThreads == 0, "whole tiles");
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i = lane & 15, c = lane >> 4;
     const int64_t bh = blockIdx.y;
@@ -510,114 +646,50 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D * NR <= 128 ? OCC : 1) void
     const int used = used_splits(a, seq, wg_row);
     if (split >= used && split > 0) return;
 
-    const int row0 = wg_row + (TOKEN_WAVES == 1 ? wave * 16 * NR : 0);
-    const int tiles = row0 < a.rows ? seen_tiles(a, seq, row0 + 16 * NR - 1) : 0;
-    const int first = split * a.split_tiles + (TOKEN_WAVES == 1 ? 0 : wave);
-    const int stop = (split + 1) * a.split_tiles < tiles ? (split + 1) * a.split_tiles : tiles;
-
-    // addresses: a scalar base for the tile, an offset of the lane and constants
-    const uint8_t* keys = a.k_codes + bh * a.capacity * D;
-    const uint8_t* values = a.v_codes + bh * a.capacity * D;
+    const int row0 = wg_row + wave * 16 * NR;
+    const int first = split * a.split_tiles;
+    const auto limit = [&](int row) {
+        const int tiles = seen_tiles(a, seq, row);
+        return first + a.split_tiles < tiles ? first + a.split_tiles : tiles;
+    };
+    const int stop = limit(wg_row + a.row_tile - 1);
+    const int mine = row0 < a.rows ? limit(row0 + 16 * NR - 1) : 0;
+    const u32x4_t* keys = reinterpret_cast<const u32x4_t*>(a.k_codes + bh * a.capacity * D);
+    const u32x4_t* values = reinterpret_cast<const u32x4_t*>(a.v_codes + bh * a.capacity * D);
     const float* k_amax = a.k_amax + bh * (a.capacity >> a.block_shift);
     const float* v_amax = a.v_amax + bh * (a.capacity >> a.block_shift);
     const int amax_at = 16 * c >> a.block_shift;
+    extern __shared__ u32x4_t buffers[];  // [2][keys, values][kPieces]
 
-    // Keys of the next tile and values of this one are asked for before the work on this one begins.
-    KvTile<D> next;
-    const auto piece = [&](const uint8_t* from, int n) {
-        const u32x4_t* at = reinterpret_cast<const u32x4_t*>(from + (lane * 16 + n * 1024));
-        return a.stream ? __builtin_nontemporal_load(at) : *at;
-    };
+    u32x4_t coming[kPer];
+    float k_next = 0.0f, v_next = 0.0f;
     const auto load = [&](int tile) {
-        const float* ks = k_amax + ((int64_t)tile * kKvTile >> a.block_shift);
-        const float* vs = v_amax + ((int64_t)tile * kKvTile >> a.block_shift);
-        next.k_amax = ks[amax_at];
-        next.v_amax = vs[amax_at];
-        const uint8_t* from = keys + (int64_t)tile * (kKvTile * D);
+        k_next = k_amax[((int64_t)tile * kKvTile >> a.block_shift) + amax_at];
+        v_next = v_amax[((int64_t)tile * kKvTile >> a.block_shift) + amax_at];
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int u = 0; u < D / 64; ++u) next.keys[s][u] = piece(from, s * (D / 64) + u);
+        for (int n = 0; n < kPer; ++n) {
+            const int at = n * kThreads + threadIdx.x;
+            coming[n] = at < kPieces ? keys[(int64_t)tile * kPieces + at] : values[(int64_t)tile * kPieces + at - kPieces];
+        }
     };
     if (first < stop) load(first);
     AttendRows<T, D, NR> rows;
     rows.begin(a, seq, b, h, row0, i, c);
-    for (int tile = first; tile < stop; tile += TOKEN_WAVES) {
-        u32x4_t vw[kOut];
-        const uint8_t* from = values + (int64_t)tile * (kKvTile * D);
+    for (int tile = first; tile < stop; ++tile) {
+        u32x4_t* buffer = buffers + (tile & 1) * 2 * kPieces;
+        const float k_now = k_next, v_now = v_next;
 #pragma unroll
-        for (int u = 0; u < kOut; ++u) vw[u] = piece(from, u);
-        // behind the last tile that one is loaded again: a load that may be left out would have to be waited for at once
-        rows.work(next, vw, tile * kKvTile, c, [&] { load(tile + TOKEN_WAVES < stop ? tile + TOKEN_WAVES : tile); });
+        for (int n = 0; n < kPer; ++n) buffer[n * kThreads + threadIdx.x] = coming[n];
+        // one barrier a tile: this buffer was last read two tiles ago, in front of the previous barrier
+        __syncthreads();
+        load(tile + 1 < stop ? tile + 1 : tile);
+        if (tile < mine)
+            rows.work([&](int s, int u) { return buffer[(s * (D / 64) + u) * kWave + lane]; },
+                      [&](int u) { return buffer[kPieces + u * kWave + lane]; }, k_now, v_now, tile * kKvTile, c, [] {});
     }
     float sum[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        sum[n] = rows.sum[n];
-        sum[n] += __shfl_xor(sum[n], 16, kWave);
-        sum[n] += __shfl_xor(sum[n], 32, kWave);
-        if (rows.last[n] < 0) sum[n] = 0.0f;
-        if (rows.top[n] != kTop) rows.reference[n] = -__builtin_inff();  // nothing seen here
-    }
-
-    if constexpr (TOKEN_WAVES == 1) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-            const int row = row0 + 16 * n + i;
-            if (row >= a.rows) continue;
-            if (used <= 1) {
-                const float inverse = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
-                T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * c;
-#pragma unroll
-                for (int u = 0; u < kOut; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) to[16 * u + r] = store_cast<T>(sum[n] == 0.0f ? 0.0f : rows.o[u][n][r] * inverse);
-            } else {
-                const int64_t at = (bh * a.rows + row) * a.splits + split;
-#pragma unroll
-                for (int u = 0; u < kOut; ++u) *reinterpret_cast<f32x4*>(a.part + at * D + 16 * u + 4 * c) = rows.o[u][n];
-                if (c == 0) a.part_stat[at * 2] = rows.reference[n], a.part_stat[at * 2 + 1] = sum[n];
-            }
-        }
-    } else {
-        // the waves' results are joined through LDS, in wave order
-        constexpr int kRows = 16 * NR, kPitch = kRows + 1;
-        extern __shared__ float joined[];  // [wave][D][kPitch], then [wave][kRows][2]
-        float* stats = joined + kAttendWaves * D * kPitch;
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-#pragma unroll
-            for (int u = 0; u < kOut; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) joined[(wave * D + 16 * u + 4 * c + r) * kPitch + 16 * n + i] = rows.o[u][n][r];
-            if (c == 0) stats[(wave * kRows + 16 * n + i) * 2] = rows.reference[n], stats[(wave * kRows + 16 * n + i) * 2 + 1] = sum[n];
-        }
-        __syncthreads();
-        for (int id = threadIdx.x; id < kRows * D; id += kAttendWaves * kWave) {
-            const int rr = id / D, d = id % D;
-            const int row = wg_row + rr;
-            if (row >= a.rows) break;
-            float best = -__builtin_inff();
-#pragma unroll
-            for (int w = 0; w < kAttendWaves; ++w) best = fmaxf(best, stats[(w * kRows + rr) * 2]);
-            const float base = best == -__builtin_inff() ? 0.0f : best;
-            float total = 0.0f, value = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kAttendWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f(stats[(w * kRows + rr) * 2] - base);
-                total += f * stats[(w * kRows + rr) * 2 + 1];
-                value += f * joined[(w * D + d) * kPitch + rr];
-            }
-            if (used <= 1) {
-                T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot;
-                to[d] = store_cast<T>(total == 0.0f ? 0.0f : value / total);
-            } else {
-                const int64_t at = (bh * a.rows + row) * a.splits + split;
-                a.part[at * D + d] = value;
-                if (d == 0) a.part_stat[at * 2] = best, a.part_stat[at * 2 + 1] = total;
-            }
-        }
-    }
+    finish_rows(rows, sum);
+    store_rows(a, rows, sum, bh, row0, split, used <= 1, i, c);
 }
 
 // One workgroup per row joins the splits: the weights of all of them first, then 1024 / D splits at a time with 16 bytes
@@ -721,21 +793,21 @@ int launch_values(const KvValuesArgs& a, int64_t bh, int32_t dim, hipStream_t s)
     return dim == 64 ? launch_values<T, 64>(a, bh, s) : dim == 128 ? launch_values<T, 128>(a, bh, s) : launch_values<T, 256>(a, bh, s);
 }
 
-// How a call is shared out.  Few rows (decoding): 16 to a workgroup, whose four waves share the tokens.  More rows: each
-// wave its own 32 (float32 queries, 256 channels: 16), so that a tile of codes is turned into float16 once for all of them.
-// The token axis is split until there are two workgroups for each of the 256 compute units (which is what runs there at
-// once), in one round of equal shares with one length for all sequences; where lengths differ (and are known to the device
+// How a call is shared out.  Up to 32 rows (decoding): 16 to a workgroup, whose four waves share the tokens.  More rows: each
+// of four or eight waves its own 32 (float32 queries, 256 channels: 16), so that a tile of codes is turned into float16
+// once for all of them.  The token axis is split until every compute unit has eight waves, which is what runs there at
+// once, in one round of equal shares with one length for all sequences; where lengths differ (and are known to the device
 // alone) shares a third as long even them out.  A share is at least four tiles.
-struct AttendPlan { int32_t token_waves, row_tile, splits, split_tiles; };
+struct AttendPlan { int32_t waves, row_tile, splits, split_tiles; };
 inline AttendPlan plan_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q) {
     const int64_t bh = (int64_t)cache->batch * cache->heads, rows = (int64_t)q->queries * (q->query_heads / cache->heads);
     const int64_t tokens = q->lengths ? cache->capacity : q->length_all;
     const int64_t tiles = (tokens + kKvTile - 1) / kKvTile;
-    AttendPlan p;
-    p.token_waves = rows <= 32 ? 4 : 1;
     const int wave_rows = q->dtype == AHQ_F32 || cache->head_dim == 256 ? 16 : 32;
-    p.row_tile = p.token_waves == 4 ? 16 : kAttendWaves * wave_rows;
-    const int64_t room = 512 * (q->lengths ? 3 : 1), wgs = bh * ((rows + p.row_tile - 1) / p.row_tile);
+    AttendPlan p;
+    p.waves = rows <= 32 ? 0 : rows <= 4 * wave_rows ? 4 : 8;  // 0: waves share the tokens
+    p.row_tile = p.waves == 0 ? 16 : p.waves * wave_rows;
+    const int64_t room = (p.waves == 8 ? 256 : 512) * (q->lengths ? 3 : 1), wgs = bh * ((rows + p.row_tile - 1) / p.row_tile);
     int64_t n = (wgs * tiles + room - 1) / room;
     n = (n + 3) / 4 * 4;
     p.split_tiles = (int32_t)(n < 4 ? 4 : n);
@@ -744,22 +816,30 @@ inline AttendPlan plan_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q
     return p;
 }
 
+template <typename Kernel>
+int launch_with_lds(Kernel kernel, const dim3& grid, int threads, size_t lds, const KvAttendArgs& a, hipStream_t s) {
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
+    }
+    kernel<<<grid, threads, lds, s>>>(a);
+    return check_launch("ahq_kv_attend");
+}
+
 template <typename T, int D>
 int launch_attend(const KvAttendArgs& a, const AttendPlan& p, int64_t bh, hipStream_t s) {
     const dim3 grid((unsigned)((a.rows + p.row_tile - 1) / p.row_tile), (unsigned)bh, (unsigned)p.splits);
-    if (p.token_waves == 4) {
-        constexpr size_t lds = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float);
-        const auto kernel = kv_attend_kernel<T, D, 1, 4>;
-        if (lds > 65536) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
-        }
-        kernel<<<grid, kAttendWaves * kWave, lds, s>>>(a);
-    } else {
-        constexpr int NR = sizeof(T) == 4 || D == 256 ? 1 : 2;
-        kv_attend_kernel<T, D, NR, 1><<<grid, kAttendWaves * kWave, 0, s>>>(a);
-    }
-    const int rc = check_launch("ahq_kv_attend");
+    constexpr int NR = sizeof(T) == 4 || D == 256 ? 1 : 2;
+    constexpr size_t joined = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float), buffers = 4 * (size_t)D * kKvTile;
+    int rc;
+    if (p.waves == 0 && bh * a.capacity * D >= kStreamLoadBytes)
+        rc = launch_with_lds(kv_attend_kernel<T, D, true>, grid, kAttendWaves * kWave, joined, a, s);
+    else if (p.waves == 0)
+        rc = launch_with_lds(kv_attend_kernel<T, D, false>, grid, kAttendWaves * kWave, joined, a, s);
+    else if (p.waves == 4)
+        rc = launch_with_lds(kv_prompt_kernel<T, D, NR, 4>, grid, 4 * kWave, buffers, a, s);
+    else
+        rc = launch_with_lds(kv_prompt_kernel<T, D, NR, 8>, grid, 8 * kWave, buffers, a, s);
     if (rc != AHQ_OK || p.splits == 1) return rc;
     kv_join_kernel<T, D><<<dim3((unsigned)a.rows, (unsigned)bh), kJoinThreads, 0, s>>>(a);
     return check_launch("ahq_kv_attend");
@@ -861,7 +941,7 @@ extern "C" int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q,
     a.rows = a.queries * a.groups, a.row_tile = p.row_tile, a.splits = p.splits, a.split_tiles = p.split_tiles;
     a.scale = q->scale * 1.44269504088896340736f;
     a.vec = (uintptr_t)q->q % 16 == 0 && a.qb * e % 16 == 0 && a.qh * e % 16 == 0 && a.qt * e % 16 == 0;
-    a.stream = bh * a.capacity * cache->head_dim >= kStreamLoadBytes;
+    a.vec_out = (uintptr_t)q->out % (4 * e) == 0 && a.ob % 4 == 0 && a.oh % 4 == 0 && a.ot % 4 == 0;
     a.part = static_cast<float*>(workspace);
     a.part_stat = a.part + (size_t)bh * a.rows * a.splits * cache->head_dim;
     const hipStream_t s = static_cast<hipStream_t>(stream);
