@@ -19,9 +19,10 @@
 // 1024 + b, and one packed addition of -1152 makes two codes of two bytes.  A query row is multiplied by the power of two
 // that brings its largest value to 2^13 .. 2^14, which keeps 16-bit queries exact (bfloat16 down to 2^-30 of the row's
 // largest value); float32 queries become two parts, 22 bits.  Probabilities carry the scale of their values' block:
-// with x = score + log2(scale), weights are 2^(x - reference), the reference being such that the largest is at most
-// kTop = 2^14, so float16 holds them to 2^-12 (two parts for float32 queries: 2^-23) and down to 2^-38 of the largest;
-// the softmax's denominator sums weight / scale in float32.  Scales below 2^-80 count as 2^-80 there.
+// with x = score + log2(scale), weights are 2^(x - reference), the reference being such that the largest weight so far lies
+// between 2^10 and 2^15 (it is moved, and the sums with it, only when a weight passes 2^15), so float16 holds them to
+// 2^-12 (two parts for float32 queries: 2^-23) and down to 2^-34 of the largest; the softmax's denominator sums
+// weight / scale in float32.  Scales below 2^-80 count as 2^-80 there.
 
 #include "../../include/aimet_amd_serving.h"
 #include "ahq_host.h"
@@ -301,6 +302,7 @@ __device__ __forceinline__ f16x8 codes_to_f16(uint32_t a, uint32_t b) {
     r.h[2] = two_codes(b, 0x04010400u), r.h[3] = two_codes(b, 0x04030402u);
     return r.v;
 }
+__device__ __forceinline__ f16x8 half_piece(const u32x4_t& w, int half) { return codes_to_f16(w[2 * half], w[2 * half + 1]); }
 // Eight values as a sum of N float16 fragments.
 template <int N>
 __device__ __forceinline__ void split_f16(const float* v, f16x8* out) {
@@ -316,7 +318,7 @@ __device__ __forceinline__ void split_f16(const float* v, f16x8* out) {
         }
 }
 
-constexpr float kTop = 14.0f;                 // log2 of the largest weight
+constexpr float kTop = 15.0f, kStart = 10.0f;  // log2 of the largest weight: at most, and where the reference is set to
 constexpr float kLeastScale = 0x1p-80f;
 constexpr int kAttendWaves = 4;
 
@@ -394,8 +396,8 @@ struct AttendRows {
         least = __builtin_amdgcn_readfirstlane(least);
     }
 
-    // One tile of 64 tokens from p0 on: `key` and `value` give a lane's 16 bytes of a piece, `between` is called once the
-    // keys and scales are no longer needed.
+    // One tile of 64 tokens from p0 on: `key(s, u)` and `value(u, w)` give operands, `between` is called once the keys and
+    // scales are no longer needed.
     template <typename Key, typename Value, typename Between>
     __device__ __forceinline__ void work(Key key, Value value, float k_amax, float v_amax, int p0, int c, Between between) {
         const float k_scale = k_amax * (1.0f / 127.0f);
@@ -408,16 +410,12 @@ struct AttendRows {
 #pragma unroll
             for (int n = 0; n < NR; ++n) x[s][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < D / 64; ++u) {
-                const u32x4_t w = key(s, u);
+            for (int u = 0; u < kSteps; ++u) {
+                const f16x8 kf = key(s, u);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const f16x8 kf = codes_to_f16(w[2 * half], w[2 * half + 1]);
+                for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int n = 0; n < NR; ++n)
-#pragma unroll
-                        for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf, q[2 * u + half][n][p], x[s][n]);
-                }
+                    for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf, q[u][n][p], x[s][n]);
             }
         }
         between();
@@ -447,7 +445,7 @@ struct AttendRows {
             most = fmaxf(most, __shfl_xor(most, 32, kWave));
             const bool raise = most > top[n];
             if (__any(raise)) {  // seldom once a few tiles are done
-                const float by = raise ? most - kTop : 0.0f;
+                const float by = raise ? most - kStart : 0.0f;
                 const float fade = !raise ? 1.0f : top[n] == kTop ? __builtin_amdgcn_exp2f(-by) : 0.0f;
                 if (raise) top[n] = kTop;
                 reference[n] += by;
@@ -476,8 +474,7 @@ struct AttendRows {
         }
 #pragma unroll
         for (int u = 0; u < kOut; ++u) {
-            const u32x4_t w = value(u);
-            const f16x8 v0 = codes_to_f16(w[0], w[1]), v1 = codes_to_f16(w[2], w[3]);
+            const f16x8 v0 = value(u, 0), v1 = value(u, 1);
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -585,8 +582,8 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
 #pragma unroll
         for (int u = 0; u < kOut; ++u) vw[u] = piece(from, u);
         // behind the last tile that one is loaded again: a load that may be left out would have to be waited for at once
-        rows.work([&](int s, int u) { return kw[s][u]; }, [&](int u) { return vw[u]; }, k_next, v_next, tile * kKvTile, c,
-                  [&] { load(tile + kAttendWaves < stop ? tile + kAttendWaves : tile); });
+        rows.work([&](int s, int u) { return half_piece(kw[s][u / 2], u % 2); }, [&](int u, int w) { return half_piece(vw[u], w); },
+                  k_next, v_next, tile * kKvTile, c, [&] { load(tile + kAttendWaves < stop ? tile + kAttendWaves : tile); });
     }
     float sum[1];
     finish_rows(rows, sum);
@@ -628,8 +625,8 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
 }
 
 // Many rows (prompts): each wave has 16 * NR rows of its own, and the workgroup takes the token tiles one after the other
-// through two LDS buffers; the next tile is on its way to registers while this one is worked on.  Bound by the vector
-// work between the two products (conversion of codes, exponentials).
+// through two LDS buffers, turned into float16 once for all its waves; the next tile is on its way to registers while this
+// one is worked on.  Bound by the matrix cores and the vector work between the two products together.
 template <typename T, int D, int NR, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArgs a) {
     constexpr int kThreads = WAVES * kWave;
@@ -659,7 +656,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArg
     const float* k_amax = a.k_amax + bh * (a.capacity >> a.block_shift);
     const float* v_amax = a.v_amax + bh * (a.capacity >> a.block_shift);
     const int amax_at = 16 * c >> a.block_shift;
-    extern __shared__ u32x4_t buffers[];  // [2][keys, values][kPieces]
+    extern __shared__ f16x8 buffers[];  // [2][keys, values][piece of 64 lanes][half][64]
 
     u32x4_t coming[kPer];
     float k_next = 0.0f, v_next = 0.0f;
@@ -676,16 +673,19 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArg
     AttendRows<T, D, NR> rows;
     rows.begin(a, seq, b, h, row0, i, c);
     for (int tile = first; tile < stop; ++tile) {
-        u32x4_t* buffer = buffers + (tile & 1) * 2 * kPieces;
+        f16x8* buffer = buffers + (tile & 1) * 4 * kPieces;
         const float k_now = k_next, v_now = v_next;
 #pragma unroll
-        for (int n = 0; n < kPer; ++n) buffer[n * kThreads + threadIdx.x] = coming[n];
+        for (int n = 0; n < kPer; ++n)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                buffer[(n * WAVES + wave) * 2 * kWave + half * kWave + lane] = half_piece(coming[n], half);
         // one barrier a tile: this buffer was last read two tiles ago, in front of the previous barrier
         __syncthreads();
         load(tile + 1 < stop ? tile + 1 : tile);
         if (tile < mine)
-            rows.work([&](int s, int u) { return buffer[(s * (D / 64) + u) * kWave + lane]; },
-                      [&](int u) { return buffer[kPieces + u * kWave + lane]; }, k_now, v_now, tile * kKvTile, c, [] {});
+            rows.work([&](int s, int u) { return buffer[(s * (D / 32) + u) * kWave + lane]; },
+                      [&](int u, int w) { return buffer[2 * kPieces + (2 * u + w) * kWave + lane]; }, k_now, v_now, tile * kKvTile, c, [] {});
     }
     float sum[NR];
     finish_rows(rows, sum);
@@ -830,7 +830,7 @@ template <typename T, int D>
 int launch_attend(const KvAttendArgs& a, const AttendPlan& p, int64_t bh, hipStream_t s) {
     const dim3 grid((unsigned)((a.rows + p.row_tile - 1) / p.row_tile), (unsigned)bh, (unsigned)p.splits);
     constexpr int NR = sizeof(T) == 4 || D == 256 ? 1 : 2;
-    constexpr size_t joined = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float), buffers = 4 * (size_t)D * kKvTile;
+    constexpr size_t joined = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float), buffers = 8 * (size_t)D * kKvTile;
     int rc;
     if (p.waves == 0 && bh * a.capacity * D >= kStreamLoadBytes)
         rc = launch_with_lds(kv_attend_kernel<T, D, true>, grid, kAttendWaves * kWave, joined, a, s);

@@ -203,9 +203,9 @@ def _attend_check(cache, q, lengths, counts=None, scale=None, given=()):
     score = (33 * (2 if wide else 1) * d / 32 + 5) * 2.0 ** -23 * most
     bound = eps * want.abs() + (2 * score + 2.0 ** -19 + (2.0 ** -22 if wide else 2.0 ** -11) + (66 + tiles) * 2.0 ** -22) * size
     bound += torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
-    # weights (probability times scale) are float16 numbers of which the largest is at least 2^13: steps of 2^-24 near zero
-    # take away at most half a step, 2^-38 of the largest, for each token, times a code of at most 127
-    bound += max(n) * 2.0 ** -38 * 127 * heavy.nan_to_num(0.0, 0.0)
+    # weights (probability times scale) are float16 numbers of which the largest is at least 2^10: steps of 2^-24 near zero
+    # take away at most half a step, 2^-35 of the largest, for each token, times a code of at most 127
+    bound += max(n) * 2.0 ** -35 * 127 * heavy.nan_to_num(0.0, 0.0)
     err = (out.cpu().double() - want).abs()
     assert out.dtype == q.dtype and out.shape == q.shape
     worst = tuple(x.item() for x in torch.unravel_index((err / bound).argmax(), err.shape))
