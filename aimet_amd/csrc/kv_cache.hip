@@ -318,6 +318,14 @@ __device__ __forceinline__ void split_f16(const float* v, f16x8* out) {
         }
 }
 
+// Largest value over the four lanes of a row, which are 16 apart.
+__device__ __forceinline__ float row_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(f32_to_bits(v), f32_to_bits(v), false, false);
+    v = fmaxf(bits_to_f32(a[0]), bits_to_f32(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(f32_to_bits(v), f32_to_bits(v), false, false);
+    return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
+}
+
 constexpr float kTop = 15.0f, kStart = 10.0f;  // log2 of the largest weight: at most, and where the reference is set to
 constexpr float kLeastScale = 0x1p-80f;
 constexpr int kAttendWaves = 4;
@@ -370,8 +378,7 @@ struct AttendRows {
                     v[s][e] = live ? v[s][e] : 0.0f;
                     size = fmaxf(size, fabsf(v[s][e]));
                 }
-            size = fmaxf(size, __shfl_xor(size, 16, kWave));
-            size = fmaxf(size, __shfl_xor(size, 32, kWave));
+            size = row_max(size);
             // exponent of the largest value; zeros, infinities and the smallest numbers go as they are
             int ex = (int)(f32_to_bits(size) >> 23);
             if (size == 0.0f || ex >= 255) ex = 140;
@@ -397,28 +404,41 @@ struct AttendRows {
     }
 
     // One tile of 64 tokens from p0 on: `key(s, u)` and `value(u, w)` give operands, `between` is called once the keys and
-    // scales are no longer needed.
-    template <typename Key, typename Value, typename Between>
+    // scales are no longer needed.  AHEAD: operands come from LDS and are asked for one group of products early, in an
+    // order that the compiler keeps (its own waits for each one right behind its load).
+    template <bool AHEAD, typename Key, typename Value, typename Between>
     __device__ __forceinline__ void work(Key key, Value value, float k_amax, float v_amax, int p0, int c, Between between) {
         const float k_scale = k_amax * (1.0f / 127.0f);
         const float v_scale = fmaxf(v_amax * (1.0f / 127.0f), kLeastScale);
         const float v_log = __builtin_amdgcn_logf(v_scale);
         const float v_inverse = __builtin_amdgcn_rcpf(v_scale);
         f32x4 x[4][NR];
+        f16x8 kf[2][kSteps];
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) kf[0][u] = key(0, u);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
+            if (s < 3) {
+#pragma unroll
+                for (int u = 0; u < kSteps; ++u) kf[(s + 1) % 2][u] = key(s + 1, u);
+            }
+            if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int n = 0; n < NR; ++n) x[s][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < kSteps; ++u) {
-                const f16x8 kf = key(s, u);
+            for (int u = 0; u < kSteps; ++u)
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf, q[u][n][p], x[s][n]);
-            }
+                    for (int p = 0; p < kParts; ++p) x[s][n] = mma(kf[s % 2][u], q[u][n][p], x[s][n]);
+            if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
         }
         between();
+        f16x8 vf[3][2];
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) vf[u][0] = value(u, 0), vf[u][1] = value(u, 1);
+        }
         f16x8 pf[2][NR][kParts];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -441,8 +461,7 @@ struct AttendRows {
             for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) most = fmaxf(most, x[s][n][r]);
-            most = fmaxf(most, __shfl_xor(most, 16, kWave));
-            most = fmaxf(most, __shfl_xor(most, 32, kWave));
+            most = row_max(most);
             const bool raise = most > top[n];
             if (__any(raise)) {  // seldom once a few tiles are done
                 const float by = raise ? most - kStart : 0.0f;
@@ -474,13 +493,18 @@ struct AttendRows {
         }
 #pragma unroll
         for (int u = 0; u < kOut; ++u) {
-            const f16x8 v0 = value(u, 0), v1 = value(u, 1);
+            if constexpr (AHEAD) {
+                if (u + 2 < kOut) vf[(u + 2) % 3][0] = value(u + 2, 0), vf[(u + 2) % 3][1] = value(u + 2, 1);
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                vf[u % 3][0] = value(u, 0), vf[u % 3][1] = value(u, 1);
+            }
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int p = 0; p < kParts; ++p) {
-                    o[u][n] = mma(v0, pf[0][n][p], o[u][n]);
-                    o[u][n] = mma(v1, pf[1][n][p], o[u][n]);
+                    o[u][n] = mma(vf[u % 3][0], pf[0][n][p], o[u][n]);
+                    o[u][n] = mma(vf[u % 3][1], pf[1][n][p], o[u][n]);
                 }
         }
     }
@@ -540,9 +564,9 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
     constexpr int kOut = D / 16;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i = lane & 15, c = lane >> 4;
-    const int64_t bh = blockIdx.y;
+    const int64_t bh = blockIdx.x;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-    const int split = blockIdx.z, row0 = blockIdx.x * 16;
+    const int split = blockIdx.z, row0 = blockIdx.y * 16;
     const SequenceView seq = view_sequence(a, b);
     const int used = used_splits(a, seq, row0);
     if (split >= used && split > 0) return;
@@ -582,7 +606,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
 #pragma unroll
         for (int u = 0; u < kOut; ++u) vw[u] = piece(from, u);
         // behind the last tile that one is loaded again: a load that may be left out would have to be waited for at once
-        rows.work([&](int s, int u) { return half_piece(kw[s][u / 2], u % 2); }, [&](int u, int w) { return half_piece(vw[u], w); },
+        rows.template work<false>([&](int s, int u) { return half_piece(kw[s][u / 2], u % 2); }, [&](int u, int w) { return half_piece(vw[u], w); },
                   k_next, v_next, tile * kKvTile, c, [&] { load(tile + kAttendWaves < stop ? tile + kAttendWaves : tile); });
     }
     float sum[1];
@@ -635,10 +659,11 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArg
     static_assert(2 * kPieces % kThreads == 0, "whole tiles");
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i = lane & 15, c = lane >> 4;
-    const int64_t bh = blockIdx.y;
+    const int64_t bh = blockIdx.x;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
     const int split = blockIdx.z;
-    const int wg_row = (int)(gridDim.x - 1 - blockIdx.x) * a.row_tile;  // the rows that see most come first
+    // the rows that see most come first, those of all heads, so that the workgroups that end the call are short ones
+    const int wg_row = (int)(gridDim.y - 1 - blockIdx.y) * a.row_tile;
     const SequenceView seq = view_sequence(a, b);
     const int used = used_splits(a, seq, wg_row);
     if (split >= used && split > 0) return;
@@ -684,7 +709,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArg
         __syncthreads();
         load(tile + 1 < stop ? tile + 1 : tile);
         if (tile < mine)
-            rows.work([&](int s, int u) { return buffer[(s * (D / 32) + u) * kWave + lane]; },
+            rows.template work<true>([&](int s, int u) { return buffer[(s * (D / 32) + u) * kWave + lane]; },
                       [&](int u, int w) { return buffer[2 * kPieces + (2 * u + w) * kWave + lane]; }, k_now, v_now, tile * kKvTile, c, [] {});
     }
     float sum[NR];
@@ -828,7 +853,7 @@ int launch_with_lds(Kernel kernel, const dim3& grid, int threads, size_t lds, co
 
 template <typename T, int D>
 int launch_attend(const KvAttendArgs& a, const AttendPlan& p, int64_t bh, hipStream_t s) {
-    const dim3 grid((unsigned)((a.rows + p.row_tile - 1) / p.row_tile), (unsigned)bh, (unsigned)p.splits);
+    const dim3 grid((unsigned)bh, (unsigned)((a.rows + p.row_tile - 1) / p.row_tile), (unsigned)p.splits);
     constexpr int NR = sizeof(T) == 4 || D == 256 ? 1 : 2;
     constexpr size_t joined = (size_t)kAttendWaves * (D * 17 + 32) * sizeof(float), buffers = 8 * (size_t)D * kKvTile;
     int rc;
