@@ -113,169 +113,7 @@ struct Int4Args {
     int32_t vec_x, vec_y;
 };
 
-// ------------------------------------------------------------------------------------------------- few activations --
-// What a wave reads for one 128-column tile of NT row tiles: codes, scales and zero points of its folds and, where one
-// tile of activations is all there is, those too.
-template <typename T, int FOLD, int MT, int NT, bool WITH_X>
-struct Int4Stage {
-    u32x4_t w[NT];
-    f32x4 scale[4 / FOLD][NT];
-    uint32_t zero[4 / FOLD][NT];
-    typename Int4Traits<T>::Raw x[WITH_X ? 4 : 1];
-};
-
-// A workgroup owns 16 * NT rows of the weight and 16 * MT activations; its waves take the 128-column tiles in turn and
-// their sums are added through LDS in wave order.  FOLD: matrix instructions (of 32 columns) whose sum shares a scale.
-// Bound by the stream of codes: a wave asks for its next tile before it works on the present one.
-template <typename T, int FOLD, int MT, int NT, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave) void int4_linear_kernel(Int4Args a) {
-    typedef typename Int4Traits<T>::Frag Frag;
-    constexpr int P = Int4Traits<T>::kParts;
-    constexpr bool kWithX = MT == 1;
-    typedef Int4Stage<T, FOLD, MT, NT, kWithX> Stage;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
-    const int i = lane & 15, c = lane >> 4;
-    const int64_t tile0 = (int64_t)blockIdx.x * NT;
-    const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
-    const Frag ones = ones_fragment<Frag>();
-    const T* rows[MT];
-    int64_t cols[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int64_t m = m0 + 16 * mt + i;
-        rows[mt] = static_cast<const T*>(a.x) + (m < a.m ? m : 0) * a.ldx;
-        cols[mt] = m < a.m ? a.k : 0;  // rows behind the last one count as zero
-    }
-    const u32x4_t* wp[NT];
-    const float* sp[NT];
-    const int8_t* zp[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int64_t t = tile0 + nt < a.ntiles ? tile0 + nt : a.ntiles - 1;
-        wp[nt] = reinterpret_cast<const u32x4_t*>(a.w + t * a.tiles * kTileBytes) + lane;
-        sp[nt] = a.scale + t * a.groups * kTileRows + 4 * c;
-        zp[nt] = a.zero + t * a.groups * kTileRows + 4 * c;
-    }
-    f32x4 acc[NT][MT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    const auto load = [&](Stage& st, int64_t kt) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) st.w[nt] = wp[nt][kt * (kTileBytes / 16)];
-        if constexpr (kWithX) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) st.x[j] = load_raw<T>(rows[0], kt * kTileCols + 32 * j + 8 * c, cols[0], a.vec_x);
-        }
-#pragma unroll
-        for (int f = 0; f < 4 / FOLD; ++f) {
-            const uint64_t fold = (uint64_t)(kt * (4 / FOLD) + f);
-            int64_t g = (int64_t)((fold * a.fold_inverse) >> 32);
-            g = g < a.groups ? g : a.groups - 1;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                st.scale[f][nt] = *reinterpret_cast<const f32x4*>(sp[nt] + g * kTileRows);
-                if (a.zero) st.zero[f][nt] = *reinterpret_cast<const uint32_t*>(zp[nt] + g * kTileRows);
-            }
-        }
-    };
-    const auto compute = [&](const Stage& st, int64_t kt) {
-#pragma unroll
-        for (int f = 0; f < 4 / FOLD; ++f) {
-            Frag xf[FOLD][MT][P];
-            f32x4 sum[MT];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                sum[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < FOLD; ++j) {
-                    if constexpr (kWithX)
-                        raw_to_fragments<T>(st.x[f * FOLD + j], xf[j][mt]);
-                    else
-                        raw_to_fragments<T>(load_raw<T>(rows[mt], kt * kTileCols + 32 * (f * FOLD + j) + 8 * c, cols[mt], a.vec_x), xf[j][mt]);
-                }
-#pragma unroll
-                for (int j = 0; j < FOLD; ++j)
-#pragma unroll
-                    for (int p = 0; p < P; ++p) sum[mt] = mma(ones, xf[j][mt][p], sum[mt]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                f32x4 z = {a.zero_const, a.zero_const, a.zero_const, a.zero_const};
-                if (a.zero) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) z[r] += (float)(int8_t)(st.zero[f][nt] >> (8 * r));
-                }
-                Frag wf[FOLD];
-#pragma unroll
-                for (int j = 0; j < FOLD; ++j) wf[j] = decode_codes<Frag>(st.w[nt][f * FOLD + j]);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    f32x4 part;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) part[r] = z[r] * sum[mt][r];
-#pragma unroll
-                    for (int j = 0; j < FOLD; ++j)
-#pragma unroll
-                        for (int p = 0; p < P; ++p) part = mma(wf[j], xf[j][mt][p], part);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[nt][mt][r] = __builtin_fmaf(st.scale[f][nt][r], part[r], acc[nt][mt][r]);
-                }
-            }
-        }
-    };
-    if (wave < a.tiles) {
-        Stage even, odd;
-        load(even, wave);
-        for (int64_t kt = wave;;) {
-            if (kt + waves < a.tiles) load(odd, kt + waves);
-            compute(even, kt);
-            kt += waves;
-            if (kt >= a.tiles) break;
-            if (kt + waves < a.tiles) load(even, kt + waves);
-            compute(odd, kt);
-            kt += waves;
-            if (kt >= a.tiles) break;
-        }
-    }
-
-    extern __shared__ f32x4 red[];  // [waves][NT * MT][64]
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) red[(wave * NT * MT + nt * MT + mt) * kWave + lane] = acc[nt][mt];
-    __syncthreads();
-    for (int o = threadIdx.x; o < NT * MT * kWave; o += blockDim.x) {
-        f32x4 v = red[o];
-        for (int w = 1; w < waves; ++w) {
-            const f32x4 u = red[w * NT * MT * kWave + o];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += u[r];
-        }
-        const int l = o & (kWave - 1), q = o / kWave;
-        const int64_t n = (tile0 + q / MT) * kTileRows + 4 * (l >> 4), m = m0 + 16 * (q % MT) + (l & 15);
-        if (m >= a.m || n >= a.n) continue;
-        T* y = static_cast<T*>(a.y) + m * a.ldy + n;
-        const T* bias = static_cast<const T*>(a.bias);
-        Pack<T, 4> out;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float b = bias && n + r < a.n ? load_f32(bias[n + r]) : 0.0f;
-            out.v[r] = store_cast<T>(v[r] + b);
-        }
-        if (a.vec_y && n + 4 <= a.n) {
-            store_pack<T, 4>(y, out);
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (n + r < a.n) y[r] = out.v[r];
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------------- few activations, all of them in LDS --
+// ------------------------------------------------------------------------------------------------------- few activations --
 // For activations that fit LDS (decoding: one to a few tokens).  One workgroup of 16 waves to a compute unit; `splits`
 // waves share a row tile and take its 128-column tiles in turn, so a workgroup owns 16 / splits row tiles.  Activations
 // are the A operand here, the weight's rows the columns of the result: a lane's results belong to one channel, whose scale
@@ -436,6 +274,221 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
     }
 }
 
+// ------------------------------------------------------------------------------------------------------ many activations --
+// Prompts.  A workgroup computes 16 * MT activations x 128 channels with eight waves: two halves of the channels times four
+// groups that take the 64-column steps of the row in turn, each with activations of its own in LDS (two buffers, in the
+// order of the matrix operands), so that two waves on each SIMD overlap matrix and vector work and a 2048 x 2048 result
+// already fills the chip.  Per step and wave: 8 * MT matrix instructions, 56 vector instructions to turn codes into
+// operands and 16 * MT to scale the finished group sums (every 64 columns at least): the two kinds nearly balance.  The
+// wave that brings activations in sums them, with one matrix instruction a fragment.  The groups' results are added
+// through LDS, in a fixed order.
+constexpr int kGroups = 4, kManyWaves = 2 * kGroups, kManyRows = 128;
+
+template <typename T, int MT> struct ManyLayout {
+    static constexpr int kParts = Int4Traits<T>::kParts;
+    static constexpr int kStage = 2 * MT * kParts * kWave;            // operands (16 bytes) of a 64-column step
+    static constexpr int kSums = 2 * MT * 4;                          // f32x4 of the two halves' sums
+    static constexpr size_t kBytes = (size_t)kGroups * 2 * (kStage + kSums) * 16;
+    static constexpr size_t kJoin = (size_t)(kGroups / 2) * 2 * MT * 4 * kWave * 16;
+    static constexpr size_t kLds = kBytes > kJoin ? kBytes : kJoin;
+};
+
+template <typename T, int FOLD, int MT, bool ASYM>
+__global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel(Int4Args a, int mblocks, int nblocks) {
+    typedef typename Int4Traits<T>::Frag Frag;
+    typedef ManyLayout<T, MT> Layout;
+    constexpr int P = Int4Traits<T>::kParts;
+    constexpr int NT = 4;                  // row tiles of a wave
+    constexpr int kFolds = 2 / FOLD;       // of a step
+    constexpr int kMine = MT / 2;          // activation tiles that a wave brings in
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int i = lane & 15, c = lane >> 4;
+    const int half = wave & 1, group = wave >> 1;
+    // Blocks on one XCD (every eighth workgroup) form a band of four activation blocks: they share activations and
+    // weights in its L2.
+    const int total = mblocks * nblocks, per_xcd = (total + 7) / 8;
+    const int order = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (order >= total || (int)(blockIdx.x >> 3) >= per_xcd) return;
+    const int band = order / (4 * nblocks), band_rows = mblocks - 4 * band < 4 ? mblocks - 4 * band : 4;
+    const int in_band = order - band * 4 * nblocks;
+    const int mblock = 4 * band + in_band % band_rows, nblock = in_band / band_rows;
+    const int64_t m0 = (int64_t)mblock * (16 * MT);
+    const int64_t tile0 = (int64_t)nblock * (kManyRows / kTileRows) + half * NT;
+
+    extern __shared__ u32x4_t lds[];
+    Frag* stages = reinterpret_cast<Frag*>(lds) + (size_t)group * 2 * Layout::kStage;
+    f32x4* sums = reinterpret_cast<f32x4*>(lds) + (size_t)kGroups * 2 * Layout::kStage + group * 2 * Layout::kSums;
+
+    const T* rows[kMine];
+#pragma unroll
+    for (int t = 0; t < kMine; ++t) {
+        const int64_t m = m0 + 16 * (half * kMine + t) + i;  // rows behind the last one repeat it and are not stored
+        rows[t] = static_cast<const T*>(a.x) + (m < a.m ? m : a.m - 1) * a.ldx;
+    }
+    const u32x4_t* wp[NT];
+    const float* sp[NT];
+    const int8_t* zp[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int64_t t = tile0 + nt < a.ntiles ? tile0 + nt : a.ntiles - 1;
+        wp[nt] = reinterpret_cast<const u32x4_t*>(a.w + t * a.tiles * kTileBytes) + lane;
+        sp[nt] = a.scale + t * a.groups * kTileRows + i;
+        zp[nt] = ASYM ? a.zero + t * a.groups * kTileRows + i : nullptr;
+    }
+    const int tiles = (int)a.tiles, groups = (int)a.groups;
+    const int rounds = (tiles + kGroups - 1) / kGroups;  // the same for all waves: they meet at barriers
+
+    typename Int4Traits<T>::Raw raw[kMine][2];
+    const auto fetch = [&](int step) {  // 64-column steps
+#pragma unroll
+        for (int t = 0; t < kMine; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) raw[t][j] = load_raw<T>(rows[t], (int64_t)step * 64 + 32 * j + 8 * c, a.k, a.vec_x);
+    };
+    const Frag ones = ones_fragment<Frag>();
+    const auto put = [&](int buffer) {
+#pragma unroll
+        for (int t = 0; t < kMine; ++t) {
+            f32x4 part[kFolds];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                Frag f[P];
+                raw_to_fragments<T>(raw[t][j], f);
+                if (j % FOLD == 0) part[j / FOLD] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    stages[buffer * Layout::kStage + ((j * MT + half * kMine + t) * P + p) * kWave + lane] = f[p];
+                    part[j / FOLD] = mma(f[p], ones, part[j / FOLD]);
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < kFolds; ++f) {
+                if constexpr (!ASYM) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) part[f][r] *= a.zero_const;
+                }
+                if (i == 0) sums[buffer * Layout::kSums + (f * MT + half * kMine + t) * 4 + c] = part[f];
+            }
+        }
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    u32x4_t next_w[NT];
+    const auto fetch_w = [&](int tile) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) next_w[nt] = wp[nt][tile * (kTileBytes / 16)];
+    };
+    const auto at_most = [&](int tile) { return tile < tiles ? tile : tiles - 1; };
+    fetch(2 * at_most(group));
+    fetch_w(at_most(group));
+    for (int round = 0; round < rounds; ++round) {
+        const int tile = round * kGroups + group;
+        u32x4_t w[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) w[nt] = next_w[nt];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {  // the two steps of a tile use the two buffers
+            put(s);
+            // one barrier a step: this buffer was last read two steps ago, in front of the previous barrier
+            __syncthreads();
+            float scale[kFolds][NT];
+            float zero[kFolds][NT];
+#pragma unroll
+            for (int f = 0; f < kFolds; ++f) {
+                int g = (int)(((uint64_t)(unsigned)((2 * at_most(tile) + s) * kFolds + f) * a.fold_inverse) >> 32);
+                g = g < groups ? g : groups - 1;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    scale[f][nt] = sp[nt][g * kTileRows];
+                    if constexpr (ASYM) zero[f][nt] = a.zero_const + (float)zp[nt][g * kTileRows];
+                }
+            }
+            if (s == 0) {
+                fetch(2 * at_most(tile) + 1);
+            } else {
+                fetch(2 * at_most(tile + kGroups));
+                fetch_w(at_most(tile + kGroups));
+            }
+            if (tile < tiles) {
+#pragma unroll
+                for (int f = 0; f < kFolds; ++f) {
+                    Frag wf[NT][FOLD];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < FOLD; ++j) wf[nt][j] = decode_codes<Frag>(w[nt][2 * s + f * FOLD + j]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        Frag xf[FOLD][P];
+#pragma unroll
+                        for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+                            for (int p = 0; p < P; ++p)
+                                xf[j][p] = stages[s * Layout::kStage + (((f * FOLD + j) * MT + mt) * P + p) * kWave + lane];
+                        const f32x4 sum = sums[s * Layout::kSums + (f * MT + mt) * 4 + c];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            f32x4 part = sum;
+                            if constexpr (ASYM) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) part[r] *= zero[f][nt];
+                            }
+#pragma unroll
+                            for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+                                for (int p = 0; p < P; ++p) part = mma(xf[j][p], wf[nt][j], part);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[mt][nt][r] = __builtin_fmaf(scale[f][nt], part[r], acc[mt][nt][r]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // groups 2 and 3 hand their sums to 0 and 1, then 1 to 0
+    f32x4* join = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int far = kGroups / 2; far >= 1; far /= 2) {
+        __syncthreads();
+        if (group >= far && group < 2 * far) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) join[(((group - far) * 2 + half) * MT * NT + mt * NT + nt) * kWave + lane] = acc[mt][nt];
+        }
+        __syncthreads();
+        if (group < far) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const f32x4 u = join[((group * 2 + half) * MT * NT + mt * NT + nt) * kWave + lane];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[mt][nt][r] += u[r];
+                }
+        }
+    }
+    if (group) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int64_t n = (tile0 + nt) * kTileRows + i;
+        if (n >= a.n) continue;
+        const float b = a.bias ? load_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t m = m0 + 16 * mt + 4 * c + r;
+                if (m < a.m) static_cast<T*>(a.y)[m * a.ldy + n] = store_cast<T>(acc[mt][nt][r] + b);
+            }
+    }
+}
+
 // ----------------------------------------------------------------------------------------------------------- packing --
 __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restrict__ codes, int64_t n, int64_t k,
                                                            int32_t qmin, int64_t tiles, int64_t words,
@@ -461,19 +514,6 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
 // ------------------------------------------------------------------------------------------------------------- host --
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-#ifndef W1
-#define W1 8
-#endif
-#ifndef W2
-#define W2 8
-#endif
-template <typename T, int FOLD, int MT, int NT, int WAVES>
-int launch_few(const Int4Args& a, hipStream_t stream) {
-    const int waves = (int)(a.tiles < WAVES ? a.tiles : WAVES);
-    int4_linear_kernel<T, FOLD, MT, NT, WAVES><<<dim3((unsigned)ceil_div(a.ntiles, NT), (unsigned)ceil_div(a.m, 16 * MT)),
-                                                 waves * kWave, (size_t)waves * NT * MT * 1024, stream>>>(a);
-    return check_launch("ahq_int4_linear");
-}
 template <typename T, int FOLD, int MT, bool ASYM>
 int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stream) {
     constexpr int kDepth = 2;
@@ -493,24 +533,57 @@ int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stre
     return a.zero ? launch_lds<T, FOLD, MT, true>(a, row_bytes, lds, stream) : launch_lds<T, FOLD, MT, false>(a, row_bytes, lds, stream);
 }
 
+template <typename T, int FOLD, int MT, bool ASYM>
+int launch_many(const Int4Args& a, hipStream_t stream) {
+    constexpr size_t lds = ManyLayout<T, MT>::kLds;
+    const auto kernel = int4_linear_many_kernel<T, FOLD, MT, ASYM>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
+    }
+    const int64_t mblocks = ceil_div(a.m, 16 * MT), nblocks = ceil_div(a.n, kManyRows);
+    if (mblocks * nblocks > (1 << 30)) return set_error("too many activations and channels in one call"), AHQ_ERR_UNSUPPORTED;
+    kernel<<<(unsigned)(ceil_div(mblocks * nblocks, 8) * 8), kManyWaves * kWave, lds, stream>>>(a, (int)mblocks, (int)nblocks);
+    return check_launch("ahq_int4_linear");
+}
+template <typename T, int FOLD, int MT>
+int launch_many(const Int4Args& a, hipStream_t stream) {
+    return a.zero ? launch_many<T, FOLD, MT, true>(a, stream) : launch_many<T, FOLD, MT, false>(a, stream);
+}
+
 template <typename T, int FOLD>
-int launch_few(const Int4Args& a, hipStream_t stream) {
+int launch_linear(Int4Args a, int64_t group, hipStream_t stream) {
+    // Folds per group, and the activations' room in LDS for the kernel of few activations.
+    const auto folds = [&](int64_t columns) {
+        const uint64_t n = group == a.k ? 1ull << 32 : (uint64_t)(group / columns);
+        a.fold_inverse = ((1ull << 32) + n - 1) / n;
+    };
     const size_t row_bytes = (size_t)a.tiles * 256 + 16;
-    const size_t xbytes = (size_t)a.m * row_bytes * Int4Traits<T>::kParts + (size_t)a.tiles * (4 / FOLD) * (a.m > 16 ? 128 : 64), red = (size_t)kLdsWaves * 1024 * (a.m > 16 ? 2 : 1);
-    const size_t lds = xbytes > red ? xbytes : red;
+    const size_t xbytes = (size_t)a.m * row_bytes * Int4Traits<T>::kParts + (size_t)a.tiles * (4 / FOLD) * (a.m > 16 ? 128 : 64);
+    const size_t red = (size_t)kLdsWaves * 1024 * (a.m > 16 ? 2 : 1), lds = xbytes > red ? xbytes : red;
     if (a.m <= 32 && lds <= 160 * 1024) {
+        folds(32 * FOLD);
         if (a.m <= 16) return launch_lds<T, FOLD, 1>(a, row_bytes, lds, stream);
         return launch_lds<T, FOLD, 2>(a, row_bytes, lds, stream);
     }
-    if (a.m <= 16) return launch_few<T, FOLD, 1, 1, W1>(a, stream);
-    return launch_few<T, FOLD, 2, 2, W2>(a, stream);
+    constexpr int kFold = FOLD == 1 ? 1 : 2;
+    folds(32 * kFold);
+    if constexpr (sizeof(T) == 2) {
+        // the largest block of activations that still gives most compute units a workgroup
+        const int64_t nblocks = ceil_div(a.n, kManyRows);
+        if (a.m > 64 && ceil_div(a.m, 128) * nblocks >= 192) return launch_many<T, kFold, 8>(a, stream);
+        if (a.m > 32 && ceil_div(a.m, 64) * nblocks >= 192) return launch_many<T, kFold, 4>(a, stream);
+    }
+    return launch_many<T, kFold, 2>(a, stream);
 }
 
 template <typename T>
-int launch_linear(const Int4Args& a, int fold, hipStream_t stream) {
-    if (fold == 1) return launch_few<T, 1>(a, stream);
-    if (fold == 2) return launch_few<T, 2>(a, stream);
-    return launch_few<T, 4>(a, stream);
+int launch_linear(const Int4Args& a, int64_t group, hipStream_t stream) {
+    // The scale is applied every 32, 64 or 128 columns: as rarely as one scale lasts (128 keeps the group sums short
+    // where a scale covers a whole row).
+    if (group == a.k || group % 128 == 0) return launch_linear<T, 4>(a, group, stream);
+    if (group % 64 == 0) return launch_linear<T, 2>(a, group, stream);
+    return launch_linear<T, 1>(a, group, stream);
 }
 
 }  // namespace ahq
@@ -555,15 +628,10 @@ extern "C" int ahq_int4_linear(const ahq_int4_weight* w, int32_t dtype, const vo
     a.m = m, a.n = n, a.k = k, a.ldx = ldx, a.ldy = ldy;
     a.tiles = ceil_div(k, kTileCols), a.ntiles = ceil_div(n, kTileRows), a.groups = k / group;
     a.zero_const = w->zero_const;
-    // The scale is applied every 32, 64 or 128 columns: as rarely as one scale lasts (128 keeps the group sums short
-    // where a scale covers a whole row).
-    const int fold = group == k || group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;
-    const uint64_t folds = group == k ? (uint64_t)a.tiles * 4 : (uint64_t)(group / (32 * fold));
-    a.fold_inverse = ((1ull << 32) + folds - 1) / folds;
     a.vec_x = (uintptr_t)x % 16 == 0 && (ldx * (int64_t)e) % 16 == 0;
     a.vec_y = (uintptr_t)y % (4 * e) == 0 && ldy % 4 == 0;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == AHQ_F32) return launch_linear<float>(a, fold, s);
-    if (dtype == AHQ_F16) return launch_linear<f16_t>(a, fold, s);
-    return launch_linear<bf16_t>(a, fold, s);
+    if (dtype == AHQ_F32) return launch_linear<float>(a, group, s);
+    if (dtype == AHQ_F16) return launch_linear<f16_t>(a, group, s);
+    return launch_linear<bf16_t>(a, group, s);
 }
