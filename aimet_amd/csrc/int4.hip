@@ -275,35 +275,40 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
 }
 
 // ------------------------------------------------------------------------------------------------------ many activations --
-// Prompts.  A workgroup computes 16 * MT activations x 128 channels with eight waves: two halves of the channels times four
-// groups that take the 64-column steps of the row in turn, each with activations of its own in LDS (two buffers, in the
-// order of the matrix operands), so that two waves on each SIMD overlap matrix and vector work and a 2048 x 2048 result
-// already fills the chip.  Per step and wave: 8 * MT matrix instructions, 56 vector instructions to turn codes into
+// Prompts.  A workgroup computes 16 * MT activations x 64 * NW channels with eight waves: NW side by side times 8 / NW groups
+// that take the 64-column steps of the row in turn, each with activations of its own in LDS (two buffers, in the order of
+// the matrix operands), so that two waves on each SIMD overlap matrix and vector work and a 2048 x 2048 result already
+// fills the chip.  Per step and wave: 8 * MT matrix instructions, 56 vector instructions to turn codes into
 // operands and 16 * MT to scale the finished group sums (every 64 columns at least): the two kinds nearly balance.  The
 // wave that brings activations in sums them, with one matrix instruction a fragment.  The groups' results are added
 // through LDS, in a fixed order.
-constexpr int kGroups = 4, kManyWaves = 2 * kGroups, kManyRows = 128;
+constexpr int kManyWaves = 8;
 
-template <typename T, int MT> struct ManyLayout {
+// NW waves side by side (of 64 channels each), 8 / NW groups along the row.
+template <typename T, int MT, int NW> struct ManyLayout {
     static constexpr int kParts = Int4Traits<T>::kParts;
+    static constexpr int kGroups = kManyWaves / NW;
     static constexpr int kStage = 2 * MT * kParts * kWave;            // operands (16 bytes) of a 64-column step
     static constexpr int kSums = 2 * MT * 4;                          // f32x4 of the two halves' sums
     static constexpr size_t kBytes = (size_t)kGroups * 2 * (kStage + kSums) * 16;
-    static constexpr size_t kJoin = (size_t)(kGroups / 2) * 2 * MT * 4 * kWave * 16;
+    static constexpr size_t kJoin = (size_t)(kGroups / 2) * NW * MT * 4 * kWave * 16;
     static constexpr size_t kLds = kBytes > kJoin ? kBytes : kJoin;
 };
 
-template <typename T, int FOLD, int MT, bool ASYM>
+// WHOLE: rows start on 16-byte boundaries and are whole steps long, so that no load has to be looked at.
+template <typename T, int FOLD, int MT, int NW, bool ASYM, bool WHOLE>
 __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel(Int4Args a, int mblocks, int nblocks) {
     typedef typename Int4Traits<T>::Frag Frag;
-    typedef ManyLayout<T, MT> Layout;
+    typedef ManyLayout<T, MT, NW> Layout;
+    constexpr int kGroups = Layout::kGroups;
     constexpr int P = Int4Traits<T>::kParts;
     constexpr int NT = 4;                  // row tiles of a wave
     constexpr int kFolds = 2 / FOLD;       // of a step
-    constexpr int kMine = MT / 2;          // activation tiles that a wave brings in
+    constexpr int kMine = MT / NW;         // activation tiles that a wave brings in
+    static_assert(MT % NW == 0, "each wave brings in as many");
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i = lane & 15, c = lane >> 4;
-    const int half = wave & 1, group = wave >> 1;
+    const int side = wave % NW, group = wave / NW;
     // Blocks on one XCD (every eighth workgroup) form a band of four activation blocks: they share activations and
     // weights in its L2.
     const int total = mblocks * nblocks, per_xcd = (total + 7) / 8;
@@ -313,27 +318,32 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
     const int in_band = order - band * 4 * nblocks;
     const int mblock = 4 * band + in_band % band_rows, nblock = in_band / band_rows;
     const int64_t m0 = (int64_t)mblock * (16 * MT);
-    const int64_t tile0 = (int64_t)nblock * (kManyRows / kTileRows) + half * NT;
+    const int64_t tile0 = (int64_t)nblock * (NW * NT) + side * NT;
 
     extern __shared__ u32x4_t lds[];
     Frag* stages = reinterpret_cast<Frag*>(lds) + (size_t)group * 2 * Layout::kStage;
     f32x4* sums = reinterpret_cast<f32x4*>(lds) + (size_t)kGroups * 2 * Layout::kStage + group * 2 * Layout::kSums;
 
+    // Rows behind the last one repeat it and are not stored.  WHOLE: a scalar base and 32-bit offsets of the lane.
     const T* rows[kMine];
+    uint32_t row_at[kMine];
+    const char* block = static_cast<const char*>(a.x) + m0 * a.ldx * (int64_t)sizeof(T);
 #pragma unroll
     for (int t = 0; t < kMine; ++t) {
-        const int64_t m = m0 + 16 * (half * kMine + t) + i;  // rows behind the last one repeat it and are not stored
-        rows[t] = static_cast<const T*>(a.x) + (m < a.m ? m : a.m - 1) * a.ldx;
+        const int r = 16 * (side * kMine + t) + i, in = m0 + r < a.m ? r : (int)(a.m - 1 - m0);
+        if constexpr (WHOLE) row_at[t] = (uint32_t)((in * (int)a.ldx + 8 * c) * (int)sizeof(T));
+        else rows[t] = static_cast<const T*>(a.x) + (m0 + in) * a.ldx;
     }
-    const u32x4_t* wp[NT];
+    // scalar bases; the lane's offset is added at the load
+    const uint8_t* wp[NT];
     const float* sp[NT];
     const int8_t* zp[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int64_t t = tile0 + nt < a.ntiles ? tile0 + nt : a.ntiles - 1;
-        wp[nt] = reinterpret_cast<const u32x4_t*>(a.w + t * a.tiles * kTileBytes) + lane;
-        sp[nt] = a.scale + t * a.groups * kTileRows + i;
-        zp[nt] = ASYM ? a.zero + t * a.groups * kTileRows + i : nullptr;
+        wp[nt] = a.w + t * a.tiles * kTileBytes;
+        sp[nt] = a.scale + t * a.groups * kTileRows;
+        zp[nt] = ASYM ? a.zero + t * a.groups * kTileRows : nullptr;
     }
     const int tiles = (int)a.tiles, groups = (int)a.groups;
     const int rounds = (tiles + kGroups - 1) / kGroups;  // the same for all waves: they meet at barriers
@@ -343,7 +353,12 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
 #pragma unroll
         for (int t = 0; t < kMine; ++t)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) raw[t][j] = load_raw<T>(rows[t], (int64_t)step * 64 + 32 * j + 8 * c, a.k, a.vec_x);
+            for (int j = 0; j < 2; ++j) {
+                if constexpr (WHOLE)
+                    raw[t][j] = *reinterpret_cast<const typename Int4Traits<T>::Raw*>(block + (int64_t)step * (64 * sizeof(T)) + row_at[t] + 32 * j * sizeof(T));
+                else
+                    raw[t][j] = load_raw<T>(rows[t], (int64_t)step * 64 + 32 * j + 8 * c, a.k, a.vec_x);
+            }
     };
     const Frag ones = ones_fragment<Frag>();
     const auto put = [&](int buffer) {
@@ -357,7 +372,7 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
                 if (j % FOLD == 0) part[j / FOLD] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    stages[buffer * Layout::kStage + ((j * MT + half * kMine + t) * P + p) * kWave + lane] = f[p];
+                    stages[buffer * Layout::kStage + ((j * MT + side * kMine + t) * P + p) * kWave + lane] = f[p];
                     part[j / FOLD] = mma(f[p], ones, part[j / FOLD]);
                 }
             }
@@ -367,7 +382,7 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
 #pragma unroll
                     for (int r = 0; r < 4; ++r) part[f][r] *= a.zero_const;
                 }
-                if (i == 0) sums[buffer * Layout::kSums + (f * MT + half * kMine + t) * 4 + c] = part[f];
+                if (i == 0) sums[buffer * Layout::kSums + (f * MT + side * kMine + t) * 4 + c] = part[f];
             }
         }
     };
@@ -377,80 +392,101 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    u32x4_t next_w[NT];
-    const auto fetch_w = [&](int tile) {
+    // Codes and scales are asked for one step before their use, activations two: loads are waited for in order.
+    u32x2_t next_w[NT];
+    float next_scale[kFolds][NT];
+    int next_zero[kFolds][NT];
+    const auto fetch_weight = [&](int step) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) next_w[nt] = wp[nt][tile * (kTileBytes / 16)];
+        for (int nt = 0; nt < NT; ++nt)
+            next_w[nt] = *reinterpret_cast<const u32x2_t*>(wp[nt] + (int64_t)(step >> 1) * kTileBytes + (step & 1) * 8 + (uint32_t)(lane * 16));
+#pragma unroll
+        for (int f = 0; f < kFolds; ++f) {
+            int g = (int)(((uint64_t)(unsigned)(step * kFolds + f) * a.fold_inverse) >> 32);
+            g = g < groups ? g : groups - 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                next_scale[f][nt] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(sp[nt] + (int64_t)g * kTileRows) + (uint32_t)(4 * i));
+                if constexpr (ASYM) next_zero[f][nt] = (zp[nt] + (int64_t)g * kTileRows)[(uint32_t)i];
+            }
+        }
     };
-    const auto at_most = [&](int tile) { return tile < tiles ? tile : tiles - 1; };
-    fetch(2 * at_most(group));
-    fetch_w(at_most(group));
-    for (int round = 0; round < rounds; ++round) {
-        const int tile = round * kGroups + group;
-        u32x4_t w[NT];
+    // The workgroups of a band start at four places of the row, so that they do not ask the same memory channels at once.
+    const int turn = (mblock & 3) * rounds / 4;
+    const auto step_of = [&](int n) {  // the n-th step of this group; behind the row's end (and this group's last): live = false
+        const int r = (n >> 1) + turn;
+        return ((r < rounds ? r : r - rounds) * kGroups + group) * 2 + (n & 1);
+    };
+    const int row_steps = (int)((a.k + 63) / 64);
+    const auto at_most = [&](int step) { return step < row_steps ? step : row_steps - 1; };
+    const int steps = 2 * rounds;
+    fetch(at_most(step_of(0)));
+    fetch_weight(at_most(step_of(0)));
+    put(0);
+    fetch(at_most(step_of(1)));
+    for (int n0 = 0; n0 < steps; n0 += 2) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) w[nt] = next_w[nt];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {  // the two steps of a tile use the two buffers
-            put(s);
-            // one barrier a step: this buffer was last read two steps ago, in front of the previous barrier
+        for (int s = 0; s < 2; ++s) {  // the two buffers take turns
+            const int n = n0 + s;
+            // one barrier a step: what is read behind it was stored in front of it; what is stored behind it goes where
+            // the last reads were in front of it
             __syncthreads();
-            float scale[kFolds][NT];
-            float zero[kFolds][NT];
+            float scale[kFolds][NT], zero[kFolds][NT];
+            Frag wf[kFolds][NT][FOLD];
+            const bool live = step_of(n) < row_steps;  // behind the row's end there is nothing to add
 #pragma unroll
-            for (int f = 0; f < kFolds; ++f) {
-                int g = (int)(((uint64_t)(unsigned)((2 * at_most(tile) + s) * kFolds + f) * a.fold_inverse) >> 32);
-                g = g < groups ? g : groups - 1;
+            for (int f = 0; f < kFolds; ++f)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    scale[f][nt] = sp[nt][g * kTileRows];
-                    if constexpr (ASYM) zero[f][nt] = a.zero_const + (float)zp[nt][g * kTileRows];
+                    scale[f][nt] = live ? next_scale[f][nt] : 0.0f;
+                    if constexpr (ASYM) zero[f][nt] = a.zero_const + (float)next_zero[f][nt];
+#pragma unroll
+                    for (int j = 0; j < FOLD; ++j) wf[f][nt][j] = decode_codes<Frag>(next_w[nt][f * FOLD + j]);
                 }
-            }
-            if (s == 0) {
-                fetch(2 * at_most(tile) + 1);
-            } else {
-                fetch(2 * at_most(tile + kGroups));
-                fetch_w(at_most(tile + kGroups));
-            }
-            if (tile < tiles) {
+            fetch_weight(at_most(step_of(n + 1 < steps ? n + 1 : n)));
+            // operands of the next activation tile are read while this one's products run, in an order that is kept
+            Frag xf[2][FOLD][P];
+            f32x4 sum[2];
+            const auto read = [&](int at) {
+                const int f = at / MT, mt = at % MT;
 #pragma unroll
-                for (int f = 0; f < kFolds; ++f) {
-                    Frag wf[NT][FOLD];
+                for (int j = 0; j < FOLD; ++j)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int p = 0; p < P; ++p)
+                        xf[at & 1][j][p] = stages[s * Layout::kStage + (((f * FOLD + j) * MT + mt) * P + p) * kWave + lane];
+                sum[at & 1] = sums[s * Layout::kSums + (f * MT + mt) * 4 + c];
+            };
+            read(0);
 #pragma unroll
-                        for (int j = 0; j < FOLD; ++j) wf[nt][j] = decode_codes<Frag>(w[nt][2 * s + f * FOLD + j]);
+            for (int at = 0; at < kFolds * MT; ++at) {
+                const int f = at / MT, mt = at % MT;
+                if (at == kFolds * MT / 2) {  // half way: the next step's activations have come
+                    put(s ^ 1);
+                    fetch(at_most(step_of(n + 2 < steps ? n + 2 : n)));
+                }
+                if (at + 1 < kFolds * MT) read(at + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        Frag xf[FOLD][P];
+                for (int nt = 0; nt < NT; ++nt) {
+                    f32x4 part = sum[at & 1];
+                    if constexpr (ASYM) {
 #pragma unroll
-                        for (int j = 0; j < FOLD; ++j)
-#pragma unroll
-                            for (int p = 0; p < P; ++p)
-                                xf[j][p] = stages[s * Layout::kStage + (((f * FOLD + j) * MT + mt) * P + p) * kWave + lane];
-                        const f32x4 sum = sums[s * Layout::kSums + (f * MT + mt) * 4 + c];
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            f32x4 part = sum;
-                            if constexpr (ASYM) {
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) part[r] *= zero[f][nt];
-                            }
-#pragma unroll
-                            for (int j = 0; j < FOLD; ++j)
-#pragma unroll
-                                for (int p = 0; p < P; ++p) part = mma(xf[j][p], wf[nt][j], part);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) acc[mt][nt][r] = __builtin_fmaf(scale[f][nt], part[r], acc[mt][nt][r]);
-                        }
+                        for (int r = 0; r < 4; ++r) part[r] *= zero[f][nt];
                     }
+#pragma unroll
+                    for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) part = mma(xf[at & 1][j][p], wf[f][nt][j], part);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[mt][nt][r] = __builtin_fmaf(scale[f][nt], part[r], acc[mt][nt][r]);
+                    asm volatile("" : "+v"(acc[mt][nt]));  // the sum is formed here, not with all others at the end
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
 
-    // groups 2 and 3 hand their sums to 0 and 1, then 1 to 0
+    // the upper half of the groups hands its sums to the lower one, until one group has them all
     f32x4* join = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
     for (int far = kGroups / 2; far >= 1; far /= 2) {
@@ -459,7 +495,7 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) join[(((group - far) * 2 + half) * MT * NT + mt * NT + nt) * kWave + lane] = acc[mt][nt];
+                for (int nt = 0; nt < NT; ++nt) join[(((group - far) * NW + side) * MT * NT + mt * NT + nt) * kWave + lane] = acc[mt][nt];
         }
         __syncthreads();
         if (group < far) {
@@ -467,7 +503,7 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const f32x4 u = join[((group * 2 + half) * MT * NT + mt * NT + nt) * kWave + lane];
+                    const f32x4 u = join[((group * NW + side) * MT * NT + mt * NT + nt) * kWave + lane];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[mt][nt][r] += u[r];
                 }
@@ -533,22 +569,24 @@ int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stre
     return a.zero ? launch_lds<T, FOLD, MT, true>(a, row_bytes, lds, stream) : launch_lds<T, FOLD, MT, false>(a, row_bytes, lds, stream);
 }
 
-template <typename T, int FOLD, int MT, bool ASYM>
+template <typename T, int FOLD, int MT, int NW, bool ASYM, bool WHOLE>
 int launch_many(const Int4Args& a, hipStream_t stream) {
-    constexpr size_t lds = ManyLayout<T, MT>::kLds;
-    const auto kernel = int4_linear_many_kernel<T, FOLD, MT, ASYM>;
+    constexpr size_t lds = ManyLayout<T, MT, NW>::kLds;
+    const auto kernel = int4_linear_many_kernel<T, FOLD, MT, NW, ASYM, WHOLE>;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
     }
-    const int64_t mblocks = ceil_div(a.m, 16 * MT), nblocks = ceil_div(a.n, kManyRows);
+    const int64_t mblocks = ceil_div(a.m, 16 * MT), nblocks = ceil_div(a.n, 64 * NW);
     if (mblocks * nblocks > (1 << 30)) return set_error("too many activations and channels in one call"), AHQ_ERR_UNSUPPORTED;
     kernel<<<(unsigned)(ceil_div(mblocks * nblocks, 8) * 8), kManyWaves * kWave, lds, stream>>>(a, (int)mblocks, (int)nblocks);
     return check_launch("ahq_int4_linear");
 }
-template <typename T, int FOLD, int MT>
+template <typename T, int FOLD, int MT, int NW>
 int launch_many(const Int4Args& a, hipStream_t stream) {
-    return a.zero ? launch_many<T, FOLD, MT, true>(a, stream) : launch_many<T, FOLD, MT, false>(a, stream);
+    const bool whole = a.vec_x && a.k % 64 == 0 && a.ldx * (int64_t)sizeof(T) * 16 * MT < (1ll << 31);
+    if (a.zero) return whole ? launch_many<T, FOLD, MT, NW, true, true>(a, stream) : launch_many<T, FOLD, MT, NW, true, false>(a, stream);
+    return whole ? launch_many<T, FOLD, MT, NW, false, true>(a, stream) : launch_many<T, FOLD, MT, NW, false, false>(a, stream);
 }
 
 template <typename T, int FOLD>
@@ -569,12 +607,17 @@ int launch_linear(Int4Args a, int64_t group, hipStream_t stream) {
     constexpr int kFold = FOLD == 1 ? 1 : 2;
     folds(32 * kFold);
     if constexpr (sizeof(T) == 2) {
-        // the largest block of activations that still gives most compute units a workgroup
-        const int64_t nblocks = ceil_div(a.n, kManyRows);
-        if (a.m > 64 && ceil_div(a.m, 128) * nblocks >= 192) return launch_many<T, kFold, 8>(a, stream);
-        if (a.m > 32 && ceil_div(a.m, 64) * nblocks >= 192) return launch_many<T, kFold, 4>(a, stream);
+        // the largest block that still gives most of the 256 compute units a workgroup
+#ifndef T4
+#define T4 192
+#endif
+#ifndef T2
+#define T2 100
+#endif
+        if (ceil_div(a.m, 64) * ceil_div(a.n, 256) >= T4) return launch_many<T, kFold, 4, 4>(a, stream);
+        if (ceil_div(a.m, 64) * ceil_div(a.n, 128) >= T2) return launch_many<T, kFold, 4, 2>(a, stream);
     }
-    return launch_many<T, kFold, 2>(a, stream);
+    return launch_many<T, kFold, 2, 2>(a, stream);
 }
 
 template <typename T>
