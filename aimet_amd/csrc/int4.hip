@@ -276,7 +276,7 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
 
 // ------------------------------------------------------------------------------------------------------ many activations --
 // Prompts.  A workgroup computes 16 * MT activations x 64 * NW channels with eight waves: NW side by side times 8 / NW groups
-// that take the 64-column steps of the row in turn, each with activations of its own in LDS (two buffers, in the order of
+// that take steps of 128 columns of the row (float32: 64) in turn, each with activations of its own in LDS (two buffers, in the order of
 // the matrix operands), so that two waves on each SIMD overlap matrix and vector work and a 2048 x 2048 result already
 // fills the chip.  Per step and wave: 8 * MT matrix instructions, 56 vector instructions to turn codes into
 // operands and 16 * MT to scale the finished group sums (every 64 columns at least): the two kinds nearly balance.  The
@@ -288,8 +288,9 @@ constexpr int kManyWaves = 8;
 template <typename T, int MT, int NW> struct ManyLayout {
     static constexpr int kParts = Int4Traits<T>::kParts;
     static constexpr int kGroups = kManyWaves / NW;
-    static constexpr int kStage = 2 * MT * kParts * kWave;            // operands (16 bytes) of a 64-column step
-    static constexpr int kSums = 2 * MT * 4;                          // f32x4 of the two halves' sums
+    static constexpr int kDeep = kParts == 1 ? 4 : 2;                 // matrix instructions along a step: 128 or 64 columns
+    static constexpr int kStage = kDeep * MT * kParts * kWave;        // operands (16 bytes) of a step
+    static constexpr int kSums = kDeep * MT * 4;                      // f32x4 of its folds' sums
     static constexpr size_t kBytes = (size_t)kGroups * 2 * (kStage + kSums) * 16;
     static constexpr size_t kJoin = (size_t)(kGroups / 2) * NW * MT * 4 * kWave * 16;
     static constexpr size_t kLds = kBytes > kJoin ? kBytes : kJoin;
@@ -303,7 +304,9 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
     constexpr int kGroups = Layout::kGroups;
     constexpr int P = Int4Traits<T>::kParts;
     constexpr int NT = 4;                  // row tiles of a wave
-    constexpr int kFolds = 2 / FOLD;       // of a step
+    constexpr int kDeep = Layout::kDeep, kCols = 32 * kDeep;
+    constexpr int kFolds = kDeep / FOLD;   // of a step
+    typedef uint32_t Words __attribute__((ext_vector_type(kDeep)));
     constexpr int kMine = MT / NW;         // activation tiles that a wave brings in
     static_assert(MT % NW == 0, "each wave brings in as many");
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -345,44 +348,44 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
         sp[nt] = a.scale + t * a.groups * kTileRows;
         zp[nt] = ASYM ? a.zero + t * a.groups * kTileRows : nullptr;
     }
-    const int tiles = (int)a.tiles, groups = (int)a.groups;
-    const int rounds = (tiles + kGroups - 1) / kGroups;  // the same for all waves: they meet at barriers
+    const int steps = (int)((a.k + kCols - 1) / kCols), groups = (int)a.groups;
+    const int rounds = (steps + kGroups - 1) / kGroups;  // the same for all waves: they meet at barriers
 
-    typename Int4Traits<T>::Raw raw[kMine][2];
-    const auto fetch = [&](int step) {  // 64-column steps
+    typename Int4Traits<T>::Raw raw[kMine][kDeep];
+    const auto fetch = [&](int step) {
 #pragma unroll
         for (int t = 0; t < kMine; ++t)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < kDeep; ++j) {
                 if constexpr (WHOLE)
-                    raw[t][j] = *reinterpret_cast<const typename Int4Traits<T>::Raw*>(block + (int64_t)step * (64 * sizeof(T)) + row_at[t] + 32 * j * sizeof(T));
+                    raw[t][j] = *reinterpret_cast<const typename Int4Traits<T>::Raw*>(block + (int64_t)step * (kCols * sizeof(T)) + row_at[t] + 32 * j * sizeof(T));
                 else
-                    raw[t][j] = load_raw<T>(rows[t], (int64_t)step * 64 + 32 * j + 8 * c, a.k, a.vec_x);
+                    raw[t][j] = load_raw<T>(rows[t], (int64_t)step * kCols + 32 * j + 8 * c, a.k, a.vec_x);
             }
     };
     const Frag ones = ones_fragment<Frag>();
     const auto put = [&](int buffer) {
 #pragma unroll
         for (int t = 0; t < kMine; ++t) {
-            f32x4 part[kFolds];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                Frag f[P];
-                raw_to_fragments<T>(raw[t][j], f);
-                if (j % FOLD == 0) part[j / FOLD] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    stages[buffer * Layout::kStage + ((j * MT + side * kMine + t) * P + p) * kWave + lane] = f[p];
-                    part[j / FOLD] = mma(f[p], ones, part[j / FOLD]);
-                }
-            }
+            const int mt = side * kMine + t;
 #pragma unroll
             for (int f = 0; f < kFolds; ++f) {
+                f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = f * FOLD; j < (f + 1) * FOLD; ++j) {
+                    Frag x[P];
+                    raw_to_fragments<T>(raw[t][j], x);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        stages[buffer * Layout::kStage + ((j * MT + mt) * P + p) * kWave + lane] = x[p];
+                        part = mma(x[p], ones, part);
+                    }
+                }
                 if constexpr (!ASYM) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) part[f][r] *= a.zero_const;
+                    for (int r = 0; r < 4; ++r) part[r] *= a.zero_const;
                 }
-                if (i == 0) sums[buffer * Layout::kSums + (f * MT + side * kMine + t) * 4 + c] = part[f];
+                if (i == 0) sums[buffer * Layout::kSums + (f * MT + mt) * 4 + c] = part;
             }
         }
     };
@@ -393,13 +396,13 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
         for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // Codes and scales are asked for one step before their use, activations two: loads are waited for in order.
-    u32x2_t next_w[NT];
+    Words next_w[NT];
     float next_scale[kFolds][NT];
     int next_zero[kFolds][NT];
     const auto fetch_weight = [&](int step) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            next_w[nt] = *reinterpret_cast<const u32x2_t*>(wp[nt] + (int64_t)(step >> 1) * kTileBytes + (step & 1) * 8 + (uint32_t)(lane * 16));
+            next_w[nt] = *reinterpret_cast<const Words*>(wp[nt] + (int64_t)(step * kDeep / 4) * kTileBytes + step * kDeep % 4 * 4 + (uint32_t)(lane * 16));
 #pragma unroll
         for (int f = 0; f < kFolds; ++f) {
             int g = (int)(((uint64_t)(unsigned)(step * kFolds + f) * a.fold_inverse) >> 32);
@@ -413,76 +416,77 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
     };
     // The workgroups of a band start at four places of the row, so that they do not ask the same memory channels at once.
     const int turn = (mblock & 3) * rounds / 4;
-    const auto step_of = [&](int n) {  // the n-th step of this group; behind the row's end (and this group's last): live = false
-        const int r = (n >> 1) + turn;
-        return ((r < rounds ? r : r - rounds) * kGroups + group) * 2 + (n & 1);
+    const auto step_of = [&](int n) {  // this group's n-th step; may lie behind the row's end
+        const int r = n + turn;
+        return (r < rounds ? r : r - rounds) * kGroups + group;
     };
-    const int row_steps = (int)((a.k + 63) / 64);
-    const auto at_most = [&](int step) { return step < row_steps ? step : row_steps - 1; };
-    const int steps = 2 * rounds;
+    const auto at_most = [&](int step) { return step < steps ? step : steps - 1; };
     fetch(at_most(step_of(0)));
     fetch_weight(at_most(step_of(0)));
     put(0);
-    fetch(at_most(step_of(1)));
-    for (int n0 = 0; n0 < steps; n0 += 2) {
+    fetch(at_most(step_of(rounds > 1 ? 1 : 0)));
+    for (int n = 0; n < rounds; ++n) {
+        const int s = n & 1;  // the two buffers take turns
+        // one barrier a step: what is read behind it was stored in front of it; what is stored behind it goes where the
+        // last reads were in front of it
+        __syncthreads();
+        const bool live = step_of(n) < steps;  // behind the row's end there is nothing to add
+        Words w[NT];
+        float scale[kFolds][NT], zero[kFolds][NT];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {  // the two buffers take turns
-            const int n = n0 + s;
-            // one barrier a step: what is read behind it was stored in front of it; what is stored behind it goes where
-            // the last reads were in front of it
-            __syncthreads();
-            float scale[kFolds][NT], zero[kFolds][NT];
-            Frag wf[kFolds][NT][FOLD];
-            const bool live = step_of(n) < row_steps;  // behind the row's end there is nothing to add
+        for (int nt = 0; nt < NT; ++nt) {
+            w[nt] = next_w[nt];
 #pragma unroll
-            for (int f = 0; f < kFolds; ++f)
+            for (int f = 0; f < kFolds; ++f) {
+                scale[f][nt] = live ? next_scale[f][nt] : 0.0f;
+                if constexpr (ASYM) zero[f][nt] = a.zero_const + (float)next_zero[f][nt];
+            }
+        }
+        // operands of the next activation tile are read while this one's products run, in an order that is kept
+        Frag xf[2][FOLD][P], wf[NT][FOLD];
+        f32x4 sum[2];
+        const auto read = [&](int at) {
+            const int f = at / MT, mt = at % MT;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    scale[f][nt] = live ? next_scale[f][nt] : 0.0f;
-                    if constexpr (ASYM) zero[f][nt] = a.zero_const + (float)next_zero[f][nt];
+            for (int j = 0; j < FOLD; ++j)
 #pragma unroll
-                    for (int j = 0; j < FOLD; ++j) wf[f][nt][j] = decode_codes<Frag>(next_w[nt][f * FOLD + j]);
+                for (int p = 0; p < P; ++p)
+                    xf[at & 1][j][p] = stages[s * Layout::kStage + (((f * FOLD + j) * MT + mt) * P + p) * kWave + lane];
+            sum[at & 1] = sums[s * Layout::kSums + (f * MT + mt) * 4 + c];
+        };
+        read(0);
+#pragma unroll
+        for (int at = 0; at < kFolds * MT; ++at) {
+            const int f = at / MT, mt = at % MT;
+            if (mt == 0) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < FOLD; ++j) wf[nt][j] = decode_codes<Frag>(w[nt][f * FOLD + j]);
+            }
+            if (at == kFolds * MT / 2) {  // half way: the next step's activations have come
+                put(s ^ 1);
+                fetch_weight(at_most(step_of(n + 1 < rounds ? n + 1 : n)));
+                fetch(at_most(step_of(n + 2 < rounds ? n + 2 : n)));
+            }
+            if (at + 1 < kFolds * MT) read(at + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                f32x4 part = sum[at & 1];
+                if constexpr (ASYM) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) part[r] *= zero[f][nt];
                 }
-            fetch_weight(at_most(step_of(n + 1 < steps ? n + 1 : n)));
-            // operands of the next activation tile are read while this one's products run, in an order that is kept
-            Frag xf[2][FOLD][P];
-            f32x4 sum[2];
-            const auto read = [&](int at) {
-                const int f = at / MT, mt = at % MT;
 #pragma unroll
                 for (int j = 0; j < FOLD; ++j)
 #pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        xf[at & 1][j][p] = stages[s * Layout::kStage + (((f * FOLD + j) * MT + mt) * P + p) * kWave + lane];
-                sum[at & 1] = sums[s * Layout::kSums + (f * MT + mt) * 4 + c];
-            };
-            read(0);
+                    for (int p = 0; p < P; ++p) part = mma(xf[at & 1][j][p], wf[nt][j], part);
 #pragma unroll
-            for (int at = 0; at < kFolds * MT; ++at) {
-                const int f = at / MT, mt = at % MT;
-                if (at == kFolds * MT / 2) {  // half way: the next step's activations have come
-                    put(s ^ 1);
-                    fetch(at_most(step_of(n + 2 < steps ? n + 2 : n)));
-                }
-                if (at + 1 < kFolds * MT) read(at + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    f32x4 part = sum[at & 1];
-                    if constexpr (ASYM) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) part[r] *= zero[f][nt];
-                    }
-#pragma unroll
-                    for (int j = 0; j < FOLD; ++j)
-#pragma unroll
-                        for (int p = 0; p < P; ++p) part = mma(xf[at & 1][j][p], wf[f][nt][j], part);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[mt][nt][r] = __builtin_fmaf(scale[f][nt], part[r], acc[mt][nt][r]);
-                    asm volatile("" : "+v"(acc[mt][nt]));  // the sum is formed here, not with all others at the end
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int r = 0; r < 4; ++r) acc[mt][nt][r] = __builtin_fmaf(scale[f][nt], part[r], acc[mt][nt][r]);
+                asm volatile("" : "+v"(acc[mt][nt]));  // the sum is formed here, not with all others at the end
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
@@ -584,7 +588,7 @@ int launch_many(const Int4Args& a, hipStream_t stream) {
 }
 template <typename T, int FOLD, int MT, int NW>
 int launch_many(const Int4Args& a, hipStream_t stream) {
-    const bool whole = a.vec_x && a.k % 64 == 0 && a.ldx * (int64_t)sizeof(T) * 16 * MT < (1ll << 31);
+    const bool whole = a.vec_x && a.k % (32 * ManyLayout<T, MT, NW>::kDeep) == 0 && a.ldx * (int64_t)sizeof(T) * 16 * MT < (1ll << 31);
     if (a.zero) return whole ? launch_many<T, FOLD, MT, NW, true, true>(a, stream) : launch_many<T, FOLD, MT, NW, true, false>(a, stream);
     return whole ? launch_many<T, FOLD, MT, NW, false, true>(a, stream) : launch_many<T, FOLD, MT, NW, false, false>(a, stream);
 }
