@@ -276,7 +276,7 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
 
 // ------------------------------------------------------------------------------------------------------ many activations --
 // Prompts.  A workgroup computes 16 * MT activations x 64 * NW channels with eight waves: NW side by side times 8 / NW groups
-// that take steps of 128 columns of the row (float32: 64) in turn, each with activations of its own in LDS (two buffers, in the order of
+// that take steps of 128 or 64 columns of the row in turn, each with activations of its own in LDS (two buffers, in the order of
 // the matrix operands), so that two waves on each SIMD overlap matrix and vector work and a 2048 x 2048 result already
 // fills the chip.  Per step and wave: 8 * MT matrix instructions, 56 vector instructions to turn codes into
 // operands and 16 * MT to scale the finished group sums (every 64 columns at least): the two kinds nearly balance.  The
@@ -288,13 +288,21 @@ constexpr int kManyWaves = 8;
 template <typename T, int MT, int NW> struct ManyLayout {
     static constexpr int kParts = Int4Traits<T>::kParts;
     static constexpr int kGroups = kManyWaves / NW;
-    static constexpr int kDeep = kParts == 1 ? 4 : 2;                 // matrix instructions along a step: 128 or 64 columns
+    static constexpr int kDeep = kParts == 1 && NW == 4 ? 4 : 2;      // matrix instructions along a step: 128 or 64 columns
     static constexpr int kStage = kDeep * MT * kParts * kWave;        // operands (16 bytes) of a step
     static constexpr int kSums = kDeep * MT * 4;                      // f32x4 of its folds' sums
     static constexpr size_t kBytes = (size_t)kGroups * 2 * (kStage + kSums) * 16;
     static constexpr size_t kJoin = (size_t)(kGroups / 2) * NW * MT * 4 * kWave * 16;
     static constexpr size_t kLds = kBytes > kJoin ? kBytes : kJoin;
 };
+
+// The values of the wave's four rows of 16 lanes, each for all of them.
+__device__ __forceinline__ void rows_of(uint32_t v, float* out) {
+    const auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // rows 0 0 2 2 and 1 1 3 3
+    const auto even = __builtin_amdgcn_permlane32_swap(pair[0], pair[0], false, false);
+    const auto odd = __builtin_amdgcn_permlane32_swap(pair[1], pair[1], false, false);
+    out[0] = bits_to_f32(even[0]), out[1] = bits_to_f32(odd[0]), out[2] = bits_to_f32(even[1]), out[3] = bits_to_f32(odd[1]);
+}
 
 // WHOLE: rows start on 16-byte boundaries and are whole steps long, so that no load has to be looked at.
 template <typename T, int FOLD, int MT, int NW, bool ASYM, bool WHOLE>
@@ -339,15 +347,12 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
     }
     // scalar bases; the lane's offset is added at the load
     const uint8_t* wp[NT];
-    const float* sp[NT];
-    const int8_t* zp[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int64_t t = tile0 + nt < a.ntiles ? tile0 + nt : a.ntiles - 1;
-        wp[nt] = a.w + t * a.tiles * kTileBytes;
-        sp[nt] = a.scale + t * a.groups * kTileRows;
-        zp[nt] = ASYM ? a.zero + t * a.groups * kTileRows : nullptr;
-    }
+    for (int nt = 0; nt < NT; ++nt) wp[nt] = a.w + (tile0 + nt < a.ntiles ? tile0 + nt : a.ntiles - 1) * a.tiles * kTileBytes;
+    // lane 16 c + i brings in the scale of channel i of row tile c; rows_of() hands it to all lanes of column i
+    const int64_t scale_at = (tile0 + c < a.ntiles ? tile0 + c : a.ntiles - 1) * a.groups * kTileRows + i;
+    const float* sp = a.scale + scale_at;
+    const int8_t* zp = ASYM ? a.zero + scale_at : nullptr;
     const int steps = (int)((a.k + kCols - 1) / kCols), groups = (int)a.groups;
     const int rounds = (steps + kGroups - 1) / kGroups;  // the same for all waves: they meet at barriers
 
@@ -395,23 +400,20 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // Codes and scales are asked for one step before their use, activations two: loads are waited for in order.
-    Words next_w[NT];
-    float next_scale[kFolds][NT];
-    int next_zero[kFolds][NT];
-    const auto fetch_weight = [&](int step) {
+    // Codes, scales and activations are asked for two steps before their use.
+    Words next_w[2][NT];
+    uint32_t next_scale[2][kFolds];
+    int next_zero[2][kFolds];
+    const auto fetch_weight = [&](int q, int step) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            next_w[nt] = *reinterpret_cast<const Words*>(wp[nt] + (int64_t)(step * kDeep / 4) * kTileBytes + step * kDeep % 4 * 4 + (uint32_t)(lane * 16));
+            next_w[q][nt] = *reinterpret_cast<const Words*>(wp[nt] + (int64_t)(step * kDeep / 4) * kTileBytes + step * kDeep % 4 * 4 + (uint32_t)(lane * 16));
 #pragma unroll
         for (int f = 0; f < kFolds; ++f) {
             int g = (int)(((uint64_t)(unsigned)(step * kFolds + f) * a.fold_inverse) >> 32);
             g = g < groups ? g : groups - 1;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                next_scale[f][nt] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(sp[nt] + (int64_t)g * kTileRows) + (uint32_t)(4 * i));
-                if constexpr (ASYM) next_zero[f][nt] = (zp[nt] + (int64_t)g * kTileRows)[(uint32_t)i];
-            }
+            next_scale[q][f] = f32_to_bits(sp[(int64_t)g * kTileRows]);
+            if constexpr (ASYM) next_zero[q][f] = zp[(int64_t)g * kTileRows];
         }
     };
     // The workgroups of a band start at four places of the row, so that they do not ask the same memory channels at once.
@@ -422,11 +424,11 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
     };
     const auto at_most = [&](int step) { return step < steps ? step : steps - 1; };
     fetch(at_most(step_of(0)));
-    fetch_weight(at_most(step_of(0)));
+    fetch_weight(0, at_most(step_of(0)));
     put(0);
     fetch(at_most(step_of(rounds > 1 ? 1 : 0)));
-    for (int n = 0; n < rounds; ++n) {
-        const int s = n & 1;  // the two buffers take turns
+    fetch_weight(1, at_most(step_of(rounds > 1 ? 1 : 0)));
+    const auto work = [&](int n, int s) {  // the two buffers take turns: s = n % 2
         // one barrier a step: what is read behind it was stored in front of it; what is stored behind it goes where the
         // last reads were in front of it
         __syncthreads();
@@ -434,14 +436,13 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
         Words w[NT];
         float scale[kFolds][NT], zero[kFolds][NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            w[nt] = next_w[nt];
+        for (int nt = 0; nt < NT; ++nt) w[nt] = next_w[s][nt];
 #pragma unroll
-            for (int f = 0; f < kFolds; ++f) {
-                scale[f][nt] = live ? next_scale[f][nt] : 0.0f;
-                if constexpr (ASYM) zero[f][nt] = a.zero_const + (float)next_zero[f][nt];
-            }
+        for (int f = 0; f < kFolds; ++f) {
+            rows_of(live ? next_scale[s][f] : 0u, scale[f]);
+            if constexpr (ASYM) rows_of(f32_to_bits(a.zero_const + (float)next_zero[s][f]), zero[f]);
         }
+        fetch_weight(s, at_most(step_of(n + 2 < rounds ? n + 2 : n)));
         // operands of the next activation tile are read while this one's products run, in an order that is kept
         Frag xf[2][FOLD][P], wf[NT][FOLD];
         f32x4 sum[2];
@@ -466,7 +467,6 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
             }
             if (at == kFolds * MT / 2) {  // half way: the next step's activations have come
                 put(s ^ 1);
-                fetch_weight(at_most(step_of(n + 1 < rounds ? n + 1 : n)));
                 fetch(at_most(step_of(n + 2 < rounds ? n + 2 : n)));
             }
             if (at + 1 < kFolds * MT) read(at + 1);
@@ -488,6 +488,10 @@ __global__ __launch_bounds__(kManyWaves * kWave, 2) void int4_linear_many_kernel
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    for (int n = 0; n < rounds; n += 2) {
+        work(n, 0);
+        if (n + 1 < rounds) work(n + 1, 1);
     }
 
     // the upper half of the groups hands its sums to the lower one, until one group has them all
