@@ -77,43 +77,44 @@ __device__ __forceinline__ float finite_magnitude(float v) {
     return m < __builtin_inff() ? m : 0.0f;  // neither infinities nor NaN set a block's scale
 }
 
-// rint(127 v / amax), half to even, exact.  Fast form: with amax and 127 v exact in few bits, the remainder of the
-// approximate quotient is exact in float32 and says which neighbour is nearer; otherwise float64, whose quotient of
-// these operands (31 and 24 bits) is correctly rounded and therefore falls on the right side of every border.
-struct CodeRule {
-    float amax, inverse;
-    bool fast;
-};
-__device__ __forceinline__ CodeRule code_rule(float amax, bool narrow) {
-    CodeRule r;
-    r.amax = amax;
-    r.fast = narrow && amax > 1e-30f && amax < 1e36f && (f32_to_bits(amax) & 0x1fffu) == 0;
-    r.inverse = r.fast ? 127.0f / amax : 0.0f;
-    return r;
+// rint(127 v / amax) + 128, half to even and exact, as the low byte of the result.
+//
+// Fast form, for finite values of at most 11 bits under a maximum of as many: 127 v is exact (18 bits), and the quotient's
+// first estimate, corrected once with its exact remainder, is the rounded quotient.  One that lies half-way between two
+// codes has few bits and is met exactly; any other between 2^(6-j) and 2^(7-j) is at least 2^-(12+j) away from half-way,
+// 64 times its rounding error.  Adding 1.5 * 2^23 + 128 rounds to a whole number, half to even, and leaves it in the low bits.
+__device__ __forceinline__ uint32_t to_byte_fast(float v, float amax, float inverse) {
+    const float t = 127.0f * v;
+    const float q = t * inverse;
+    const float q1 = __builtin_fmaf(__builtin_fmaf(-q, amax, t), inverse, q);
+    return f32_to_bits(q1 + 12583040.0f);
 }
-__device__ __forceinline__ int to_code(float v, const CodeRule& rule) {
-    if (!(rule.amax > 0.0f) || v != v) return 0;
-    float q;
-    if (rule.fast) {
-        v = fminf(fmaxf(v, -rule.amax), rule.amax);
-        q = __builtin_rintf(v * rule.inverse);
-        const float twice = 2.0f * __builtin_fmaf(-q, rule.amax, 127.0f * v);
-        const bool odd = ((int)q & 1) != 0;
-        if (twice > rule.amax || (odd && twice == rule.amax)) q += 1.0f;
-        if (twice < -rule.amax || (odd && twice == -rule.amax)) q -= 1.0f;
-    } else {
-        const double w = fmin(fmax((double)v, -(double)rule.amax), (double)rule.amax);
-        q = (float)__builtin_rint(127.0 * w / (double)rule.amax);
-    }
-    return (int)q;
+// Every other case: the remainder of the float64 estimate is exact (31 and 31 bits) and says which neighbour is nearer.
+__device__ __forceinline__ uint32_t to_byte_exact(float v, float amax, double inverse) {
+    if (v != v) return kCodeBias;
+    const double w = fmin(fmax((double)v, -(double)amax), (double)amax);
+    double q = __builtin_rint(w * inverse);
+    const double twice = 2.0 * __builtin_fma(-q, (double)amax, 127.0 * w);
+    const bool odd = ((int)q & 1) != 0;
+    if (twice > amax || (odd && twice == amax)) q += 1.0;
+    if (twice < -amax || (odd && twice == -amax)) q -= 1.0;
+    return (uint32_t)((int)q + kCodeBias);
+}
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return hi << 16 | lo;
 }
 
-// VEC elements per thread and step, one step per thread; THREADS = block * D / 8 capped at 512, ITEMS steps.
+// A thread has four tokens and eight channels of the block.  Bound by the memory traffic of long prompts, by the launch
+// for single tokens: the block is read once, its maximum found with integer comparisons (a pair of 16-bit values at a
+// time), and its codes go through LDS so that whole runs of the tile's order are written.
+template <int D, int BT> constexpr int kAppendItems = BT / 4 * (D / 8);
+template <int D, int BT> constexpr int kAppendThreads = kAppendItems<D, BT> < kWave ? kWave : kAppendItems<D, BT>;
+
 template <typename T, int D, int BT>
-__global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append_kernel(KvAppendArgs a) {
-    constexpr int kVecs = BT * D / 8;
-    constexpr int kThreads = kVecs < 512 ? kVecs : 512;
-    constexpr int kItems = kVecs / kThreads;
+__global__ __launch_bounds__((kAppendThreads<D, BT>)) void kv_append_kernel(KvAppendArgs a) {
+    constexpr int kThreads = kAppendThreads<D, BT>;
+    constexpr int kPairs = sizeof(T) == 2 ? 4 : 8;  // registers of eight values
     const int which = blockIdx.z;
     const int bh = blockIdx.y, b = bh / a.heads, h = bh % a.heads;
     const TokenRange range = new_tokens(a.start, a.start0, a.counts, a.count0, a.tokens, a.capacity, b);
@@ -125,83 +126,154 @@ __global__ __launch_bounds__(BT * D / 8 < 512 ? BT * D / 8 : 512) void kv_append
     const int old_end = lo > p0 ? lo - p0 : 0;                       // tokens of the block that were there before
     const int new_end = range.end - p0 < BT ? range.end - p0 : BT;   // [old_end, new_end) are written
 
+    float* amax_at = a.amax[which] + (int64_t)bh * (a.capacity / BT) + blk;
+    const float before = old_end > 0 ? *amax_at : 0.0f;
     const T* x = static_cast<const T*>(a.x[which]) + b * a.sb[which] + h * a.sh[which];
-    float v[kItems][8];
-    float top = 0.0f;
+    const bool item = kAppendItems<D, BT> >= kWave || threadIdx.x < kAppendItems<D, BT>;
+    const int quad = threadIdx.x / (D / 8), d = threadIdx.x % (D / 8) * 8;
+    uint32_t raw[4][kPairs];
+    const auto value = [&](int r, int e) {
+        if constexpr (sizeof(T) == 4) return bits_to_f32(raw[r][e]);
+        else return load_f32(T{(uint16_t)(raw[r][e / 2] >> (16 * (e & 1)))});
+    };
+    uint32_t top = 0;  // of the magnitudes' bit patterns, which are ordered as the magnitudes are
 #pragma unroll
-    for (int it = 0; it < kItems; ++it) {
-        const int id = it * kThreads + threadIdx.x, t = id / (D / 8), d = id % (D / 8) * 8;
+    for (int r = 0; r < 4; ++r) {
+        const int t = 4 * quad + r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[it][e] = 0.0f;
-        if (t >= old_end && t < new_end) {
+        for (int e = 0; e < kPairs; ++e) raw[r][e] = 0;
+        if (item && t >= old_end && t < new_end) {
             const T* row = x + (int64_t)(p0 + t - range.begin) * a.st[which] + d;
             if (a.vec) {
-                constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-                for (int u = 0; u < 8 / kPer; ++u) {
-                    const Pack<T, kPer> w = load_pack<T, kPer>(row + u * kPer);
+                for (int u = 0; u < kPairs / 4; ++u) {
+                    const u32x4_t w = reinterpret_cast<const u32x4_t*>(row)[u];
 #pragma unroll
-                    for (int e = 0; e < kPer; ++e) v[it][u * kPer + e] = load_f32(w.v[e]);
+                    for (int e = 0; e < 4; ++e) raw[r][4 * u + e] = w[e];
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[it][e] = load_f32(row[e]);
+                for (int e = 0; e < 8; ++e) {
+                    if constexpr (sizeof(T) == 4) raw[r][e] = f32_to_bits(row[e]);
+                    else raw[r][e / 2] |= (uint32_t)row[e].bits << (16 * (e & 1));
+                }
             }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, finite_magnitude(v[it][e]));
+        for (int e = 0; e < kPairs; ++e) {
+            if constexpr (sizeof(T) == 4) {
+                const uint32_t m = raw[r][e] & 0x7fffffffu;
+                top = m > top ? m : top;
+            } else {
+                typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                             __builtin_bit_cast(u16x2, raw[r][e] & 0x7fff7fffu)));
+            }
+        }
     }
     __shared__ float part[kThreads / kWave];
-    top = wave_reduce(top, OpMaxF());
-    if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = top;
-    float* amax_at = a.amax[which] + (int64_t)bh * (a.capacity / BT) + blk;
-    const float before = old_end > 0 ? *amax_at : 0.0f;
-    __syncthreads();
+    const auto over_block = [&](float v) {
+        v = wave_reduce(v, OpMaxF());
+        if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = v;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / kWave; ++w) top = fmaxf(top, part[w]);
-    const float amax = fmaxf(before, top);
+        for (int w = 0; w < kThreads / kWave; ++w) v = fmaxf(v, part[w]);
+        return v;
+    };
+    float size;
+    if constexpr (sizeof(T) == 4) size = bits_to_f32(top);
+    else size = load_f32(T{(uint16_t)((top & 0xffffu) > (top >> 16) ? top & 0xffffu : top >> 16)});
+    // NaN loses every comparison: it goes through the maximum as an infinity
+    float most = over_block(size == size ? size : __builtin_inff());
+    const bool special = !(most < __builtin_inff());  // the same for the whole workgroup
+    if (special) {
+        float finite = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) finite = fmaxf(finite, finite_magnitude(value(r, e)));
+        __syncthreads();
+        most = over_block(finite);
+    }
+    const float amax = fmaxf(before, most);
     const bool rescale = old_end > 0 && amax > before;
-    const CodeRule rule = code_rule(amax, sizeof(T) == 2);
     const int first = rescale ? 0 : old_end;  // first token whose codes are stored
 
     uint8_t* tile = a.codes[which] + ((int64_t)bh * a.capacity + p0 / kKvTile * kKvTile) * D;
     const int t0 = p0 % kKvTile;  // the block's first token in its tile
-    __shared__ alignas(16) uint8_t stage[D * kKvTile];  // an image of the tile
+    uint32_t code[4][8];
+    if (!(amax > 0.0f)) {
 #pragma unroll
-    for (int it = 0; it < kItems; ++it) {
-        const int id = it * kThreads + threadIdx.x, t = id / (D / 8), d = id % (D / 8) * 8;
-        if (t < first || t >= new_end) continue;
-        union { uint8_t b[8]; u32x2_t w; } out;
-        if (t >= old_end) {
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out.b[e] = (uint8_t)(to_code(v[it][e], rule) + kCodeBias);
-        } else {
+            for (int e = 0; e < 8; ++e) code[r][e] = kCodeBias;
+    } else if (sizeof(T) == 2 && !special && amax > 1e-30f && amax < 1e36f && (f32_to_bits(amax) & 0x1fffu) == 0) {
+        const float inverse = 1.0f / amax;
 #pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) code[r][e] = to_byte_fast(value(r, e), amax, inverse);
+    } else {
+        const double inverse = 127.0 / (double)amax;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) code[r][e] = to_byte_exact(value(r, e), amax, inverse);
+    }
+    if (rescale && item && 4 * quad < old_end) {
+        for (int r = 0; r < 4; ++r) {
+            const int t = 4 * quad + r;
+            if (t >= old_end) break;
             for (int e = 0; e < 8; ++e) {
                 const int q = tile[which ? value_offset(t0 + t, d + e) : key_offset<D>(t0 + t, d + e)] - kCodeBias;
-                out.b[e] = (uint8_t)((int)__builtin_rint((double)q * (double)before / (double)amax) + kCodeBias);
+                const uint32_t v = (uint32_t)((int)__builtin_rint((double)q * (double)before / (double)amax) + kCodeBias);
+#pragma unroll
+                for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+                    for (int ee = 0; ee < 8; ++ee) code[rr][ee] = rr == r && ee == e ? v : code[rr][ee];
             }
         }
-        if (which == 0) {
-            *reinterpret_cast<u32x2_t*>(stage + key_offset<D>(t0 + t, d)) = out.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) stage[value_offset(t0 + t, d + e)] = out.b[e];
-        }
     }
-    __syncthreads();
-    // 16 bytes at a time: 16 channels of a token, or 16 tokens of a channel
-    for (int id = threadIdx.x; id < D * BT / 16; id += kThreads) {
-        if (which == 0) {
-            const int t = id % BT, at = key_offset<D>(t0 + t, id / BT * 16);
-            if (t >= first && t < new_end) *reinterpret_cast<u32x4_t*>(tile + at) = *reinterpret_cast<const u32x4_t*>(stage + at);
-        } else {
-            const int t = id / D * 16, at = value_offset(t0 + t, id % D);
+    constexpr int kRun = BT / 4 * 16, kPitch = D + 4;  // bytes of a run of the keys' order; channels of a row of quads
+    __shared__ alignas(16) uint8_t stage[D / 4 * (kRun + 16) > BT * kPitch ? D / 4 * (kRun + 16) : BT * kPitch];
+    if (which == 0) {
+        if (item) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                u32x2_t w = {pack_bytes(code[r][0], code[r][1], code[r][2], code[r][3]), pack_bytes(code[r][4], code[r][5], code[r][6], code[r][7])};
+                *reinterpret_cast<u32x2_t*>(stage + ((quad & 3) * (D / 16) + d / 16) * (kRun + 16) + ((quad >> 2) * 4 + r) * 16 + (d & 8)) = w;
+            }
+        }
+        __syncthreads();
+        for (int id = threadIdx.x; id < BT * D / 16; id += kThreads) {
+            const int i = id % (BT / 4), run = id / (BT / 4);
+            const int t = (i >> 2) * 16 + run / (D / 16) * 4 + (i & 3);
+            if (t >= first && t < new_end)
+                *reinterpret_cast<u32x4_t*>(tile + run * 256 + (t0 / 4 + i) * 16) = *reinterpret_cast<const u32x4_t*>(stage + run * (kRun + 16) + i * 16);
+        }
+    } else {
+        uint32_t* quads = reinterpret_cast<uint32_t*>(stage);  // four tokens of a channel: [quad][channel]
+        if (item) {
+            u32x4_t w[2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = pack_bytes(code[0][e], code[1][e], code[2][e], code[3][e]);
+            *reinterpret_cast<u32x4_t*>(quads + quad * kPitch + d) = w[0];
+            *reinterpret_cast<u32x4_t*>(quads + quad * kPitch + d + 4) = w[1];
+        }
+        __syncthreads();
+        for (int id = threadIdx.x; id < BT * D / 16; id += kThreads) {
+            const int i = id & 15, c = (id >> 4) % (BT / 16), u = (id >> 4) / (BT / 16);
+            u32x4_t w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = quads[(4 * c + j) * kPitch + 16 * u + i];
+            uint8_t* to = tile + (u * 4 + t0 / 16 + c) * 256 + i * 16;
+            const int t = 16 * c;
             if (first <= t && t + 16 <= new_end) {
-                *reinterpret_cast<u32x4_t*>(tile + at) = *reinterpret_cast<const u32x4_t*>(stage + at);
+                *reinterpret_cast<u32x4_t*>(to) = w;
             } else {
+#pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (t + e >= first && t + e < new_end) tile[at + e] = stage[at + e];
+                    if (t + e >= first && t + e < new_end) to[e] = (uint8_t)(w[e / 4] >> (8 * (e & 3)));
             }
         }
     }
@@ -214,39 +286,69 @@ struct KvValuesArgs {
     const uint8_t* codes[2];
     const float* amax[2];
     void* out[2];  // [sequence, head, length, D]
-    int32_t capacity, length, block;
+    int32_t capacity, length, block_shift;
 };
 
+// A workgroup has one tile of 64 tokens.  Bound by memory: the tile is read whole and in order, and turned round in LDS
+// (keys: runs of 256 bytes 16 apart; values: [four tokens][channel + 4]), both without bank conflicts.
 template <typename T, int D>
 __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
+    constexpr int kPitch = D + 4;
     const int which = blockIdx.z, tile = blockIdx.x;
     const int64_t bh = blockIdx.y;
     const int p0 = tile * kKvTile;
-    const uint8_t* codes = a.codes[which] + (bh * a.capacity + p0) * D;
-    const float* amax = a.amax[which] + bh * (a.capacity / a.block);
+    const u32x4_t* codes = reinterpret_cast<const u32x4_t*>(a.codes[which] + (bh * a.capacity + p0) * D);
+    const float* amax = a.amax[which] + (bh * a.capacity >> a.block_shift);
     T* out = static_cast<T*>(a.out[which]) + (bh * a.length + p0) * D;
-    __shared__ alignas(16) uint8_t stage[D * kKvTile];
-    for (int id = threadIdx.x; id < D * 4; id += kBlock)
-        *reinterpret_cast<u32x4_t*>(stage + id * 16) = *reinterpret_cast<const u32x4_t*>(codes + id * 16);
-    __syncthreads();
-    for (int id = threadIdx.x; id < kKvTile * (D / 8); id += kBlock) {
-        const int t = id / (D / 8), d = id % (D / 8) * 8;
-        if (p0 + t >= a.length) break;
-        const float s = amax[(p0 + t) / a.block] / 127.0f;
-        union { uint8_t b[8]; u32x2_t w; } in;
-        if (which) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) in.b[e] = stage[value_offset(t, d + e)];
+    static_assert(68 * D >= 64 * kPitch, "the keys' image is the larger");
+    __shared__ alignas(16) uint8_t stage[68 * D];
+    uint32_t* quads = reinterpret_cast<uint32_t*>(stage);
+    for (int id = threadIdx.x; id < D * 4; id += kBlock) {
+        const u32x4_t w = codes[id];
+        if (which == 0) {
+            *reinterpret_cast<u32x4_t*>(stage + id * 16 + (id >> 4) * 16) = w;
         } else {
-            in.w = *reinterpret_cast<const u32x2_t*>(stage + key_offset<D>(t, d));
+            const int i = id & 15, c = id >> 4 & 3, u = id >> 6;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) quads[(4 * c + j) * kPitch + 16 * u + i] = w[j];
         }
+    }
+    __syncthreads();
+    const auto store = [&](int t, int d, const float* v) {  // eight channels of a token
         constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
         for (int u = 0; u < 8 / kPer; ++u) {
             Pack<T, kPer> w;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) w.v[e] = store_cast<T>((float)(in.b[u * kPer + e] - kCodeBias) * s);
+            for (int e = 0; e < kPer; ++e) w.v[e] = store_cast<T>(v[u * kPer + e]);
             store_pack<T, kPer>(out + (int64_t)t * D + d + u * kPer, w);
+        }
+    };
+    // (byte - 128) * scale with one rounding
+    const auto scaled = [](uint32_t w, int byte, float s) { return __builtin_fmaf((float)(w >> (8 * byte) & 0xffu), s, -128.0f * s); };
+    for (int id = threadIdx.x; id < 16 * (D / 8); id += kBlock) {
+        const int quad = id / (D / 8), d = id % (D / 8) * 8;
+        if (p0 + 4 * quad >= a.length) break;
+        const float s = amax[(p0 + 4 * quad) >> a.block_shift] / 127.0f;
+        u32x4_t w[2];
+        if (which) {
+            w[0] = *reinterpret_cast<const u32x4_t*>(quads + quad * kPitch + d);
+            w[1] = *reinterpret_cast<const u32x4_t*>(quads + quad * kPitch + d + 4);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int t = 4 * quad + r;
+            float v[8];
+            if (which) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = scaled(w[e / 4][e % 4], r, s);
+            } else {
+                const int at = key_offset<D>(t, d);
+                const u32x2_t k = *reinterpret_cast<const u32x2_t*>(stage + at + (at >> 8) * 16);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = scaled(k[e / 4], e % 4, s);
+            }
+            if (p0 + t < a.length) store(t, d, v);
         }
     }
 }
@@ -791,8 +893,7 @@ inline bool supported(const ahq_kv_cache* cache) {
 
 template <typename T, int D, int BT>
 int launch_append(const KvAppendArgs& a, int64_t bh, int32_t blocks, hipStream_t s) {
-    constexpr int kVecs = BT * D / 8;
-    kv_append_kernel<T, D, BT><<<dim3(blocks, (unsigned)bh, 2), kVecs < 512 ? kVecs : 512, 0, s>>>(a);
+    kv_append_kernel<T, D, BT><<<dim3(blocks, (unsigned)bh, 2), kAppendThreads<D, BT>, 0, s>>>(a);
     return check_launch("ahq_kv_append");
 }
 template <typename T, int D>
@@ -922,7 +1023,7 @@ extern "C" int ahq_kv_dequantize(const ahq_kv_cache* cache, int32_t dtype, int32
     if (((uintptr_t)k | (uintptr_t)v) % 16) return set_error("outputs must be 16-byte aligned"), AHQ_ERR_INVALID;
     KvValuesArgs a;
     a.codes[0] = cache->k_codes, a.codes[1] = cache->v_codes, a.amax[0] = cache->k_amax, a.amax[1] = cache->v_amax;
-    a.out[0] = k, a.out[1] = v, a.capacity = cache->capacity, a.length = length, a.block = cache->block;
+    a.out[0] = k, a.out[1] = v, a.capacity = cache->capacity, a.length = length, a.block_shift = cache->block == 16 ? 4 : cache->block == 32 ? 5 : 6;
     const int64_t bh = (int64_t)cache->batch * cache->heads;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == AHQ_F32) return launch_values<float>(a, bh, cache->head_dim, s);
