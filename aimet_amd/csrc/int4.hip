@@ -110,23 +110,23 @@ struct Int4Args {
     int64_t groups;
     uint64_t fold_inverse;  // ceil(2^32 / folds per group)
     float zero_const;
-    int32_t vec_x, vec_y;
+    int32_t vec_x;
 };
 
 // ------------------------------------------------------------------------------------------------------- few activations --
-// For activations that fit LDS (decoding: one to a few tokens).  One workgroup of 16 waves to a compute unit; `splits`
-// waves share a row tile and take its 128-column tiles in turn, so a workgroup owns 16 / splits row tiles.  Activations
-// are the A operand here, the weight's rows the columns of the result: a lane's results belong to one channel, whose scale
-// and zero point are one register.  Bound by the stream of codes, so a wave asks for DEPTH tiles at once, right behind
-// its share of the activations; those are read back from LDS, whose waits do not hold up the stream.
+// Decoding: one to a few tokens.  One workgroup of 16 waves to a compute unit; `splits` waves share a row tile and take its
+// 128-column tiles in turn, so a workgroup owns 16 / splits row tiles.  Activations wait in LDS (CHUNKED: `turns` turns of
+// the waves at a time) and are the A operand here, the weight's rows the columns of the result: a lane's results belong to
+// one channel, whose scale and zero point are one register.  Bound by the stream of codes, so a wave asks for kDepth tiles
+// at once, right behind its share of the activations; those are read back from LDS, whose waits do not hold up the stream.
 constexpr int kLdsWaves = 16;
 constexpr int kLdsThreads = kLdsWaves * kWave;
 
-template <typename T, int FOLD, int MT, int DEPTH, bool ASYM>
-__global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a, int splits, int row_bytes) {
+template <typename T, int FOLD, int MT, bool ASYM, bool CHUNKED>
+__global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a, int splits, int turns, int row_bytes) {
     typedef typename Int4Traits<T>::Frag Frag;
     constexpr int P = Int4Traits<T>::kParts;
-    constexpr int kFolds = 4 / FOLD;
+    constexpr int kFolds = 4 / FOLD, kDepth = 2;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int i = lane & 15, c = lane >> 4;
     const int m = (int)a.m, tiles = (int)a.tiles, groups = (int)a.groups;
@@ -136,11 +136,14 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
     extern __shared__ u32x4_t lds[];
     char* xs = reinterpret_cast<char*>(lds);
 
-    // activations: [part][row][columns], rows padded by 16 bytes so that 16 of them lie on different banks
-    const int chunks = tiles * 16, total = m * chunks;
+    // activations of `held` tiles from tile `from` on: [part][row][columns], rows padded by 16 bytes so that 16 of them lie
+    // on different banks
+    const int held = CHUNKED ? turns * splits : tiles;
+    const int chunks = held * 16, total = m * chunks;
+    int from = 0;
     const auto fetch = [&](int id) {
         const int row = id / chunks;
-        return load_raw<T>(static_cast<const T*>(a.x) + row * a.ldx, (id - row * chunks) * 8, a.k, a.vec_x);
+        return load_raw<T>(static_cast<const T*>(a.x) + row * a.ldx, (CHUNKED ? from * kTileCols : 0) + (id - row * chunks) * 8, a.k, a.vec_x);
     };
     const auto put = [&](int id, const typename Int4Traits<T>::Raw& raw) {
         const int row = id / chunks;
@@ -152,26 +155,35 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
     };
     // all but the last kBatch rounds are stored at once; those wait until the first codes have been asked for
     constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;
-    int id = threadIdx.x;
     typename Int4Traits<T>::Raw raw[kBatch];
-    for (; id + kBatch * kLdsThreads < total; id += kBatch * kLdsThreads) {
+    int id;
+    const auto begin_activations = [&] {
+        for (id = threadIdx.x; id + kBatch * kLdsThreads < total; id += kBatch * kLdsThreads) {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) raw[u] = fetch(id + u * kLdsThreads);
+            for (int u = 0; u < kBatch; ++u) raw[u] = fetch(id + u * kLdsThreads);
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) put(id + u * kLdsThreads, raw[u]);
-    }
+            for (int u = 0; u < kBatch; ++u) put(id + u * kLdsThreads, raw[u]);
+        }
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-        if (id + u * kLdsThreads < total) raw[u] = fetch(id + u * kLdsThreads);
+        for (int u = 0; u < kBatch; ++u)
+            if (id + u * kLdsThreads < total) raw[u] = fetch(id + u * kLdsThreads);
+    };
+    const auto end_activations = [&] {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (id + u * kLdsThreads < total) put(id + u * kLdsThreads, raw[u]);
+        __syncthreads();
+    };
+    begin_activations();
 
     const bool live = tile < a.ntiles;
     const int64_t tile_at = live ? tile : a.ntiles - 1;
     const u32x4_t* wp = reinterpret_cast<const u32x4_t*>(a.w + tile_at * a.tiles * kTileBytes) + lane;
     const float* sp = a.scale + tile_at * a.groups * kTileRows + i;
     const int8_t* zp = ASYM ? a.zero + tile_at * a.groups * kTileRows + i : nullptr;
-    u32x4_t w[DEPTH];
-    float scale[DEPTH][kFolds];
-    int zero[DEPTH][kFolds];
+    u32x4_t w[kDepth];
+    float scale[kDepth][kFolds];
+    int zero[kDepth][kFolds];
     const auto load = [&](int d, int kt) {
         w[d] = __builtin_nontemporal_load(wp + kt * (kTileBytes / 16));
 #pragma unroll
@@ -183,12 +195,9 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
         }
     };
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
+    for (int d = 0; d < kDepth; ++d)
         if (split + d * splits < tiles) load(d, split + d * splits);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-        if (id + u * kLdsThreads < total) put(id + u * kLdsThreads, raw[u]);
-    __syncthreads();
+    end_activations();
 
     f32x4 acc[MT];
     const char* xrow[MT];
@@ -201,28 +210,45 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
     // sums of the activations over each fold, times z where it is the same everywhere: [fold][MT][16]
     f32x4* sums = reinterpret_cast<f32x4*>(xs + P * m * row_bytes);
     const Frag ones = ones_fragment<Frag>();
-    for (int fold = wave; fold < tiles * kFolds; fold += kLdsWaves)
+    const auto sum_activations = [&] {
+        for (int fold = wave; fold < held * kFolds; fold += kLdsWaves)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            f32x4 part = {0.f, 0.f, 0.f, 0.f};
+            for (int mt = 0; mt < MT; ++mt) {
+                f32x4 part = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < FOLD; ++j)
+                for (int j = 0; j < FOLD; ++j)
 #pragma unroll
-                for (int p = 0; p < P; ++p)
-                    part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + (fold * FOLD + j) * 64), ones, part);
-            if constexpr (!ASYM) {
+                    for (int p = 0; p < P; ++p)
+                        part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + (fold * FOLD + j) * 64), ones, part);
+                if constexpr (!ASYM) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) part[r] *= a.zero_const;
+                    for (int r = 0; r < 4; ++r) part[r] *= a.zero_const;
+                }
+                if (i == 0) sums[(fold * MT + mt) * 4 + c] = part;
             }
-            if (i == 0) sums[(fold * MT + mt) * 4 + c] = part;
-        }
-    __syncthreads();
+        __syncthreads();
+    };
+    sum_activations();
 
-    for (int kt0 = split; kt0 < tiles; kt0 += DEPTH * splits) {
+    // CHUNKED: as many turns for every wave, since they meet at barriers
+    const int end = CHUNKED ? (tiles + splits - 1) / splits * splits : tiles;
+    int left = turns;  // that the activations in LDS serve
+    for (int kt0 = split; kt0 < end; kt0 += kDepth * splits) {
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
+        for (int d = 0; d < kDepth; ++d) {
             const int kt = kt0 + d * splits;
+            if constexpr (CHUNKED) {
+                if (left == 0 && kt < end) {
+                    __syncthreads();
+                    from = kt - split, left = turns;
+                    begin_activations();
+                    end_activations();
+                    sum_activations();
+                }
+                --left;
+            }
             if (kt < tiles) {
+                const int at = CHUNKED ? kt - from : kt;
 #pragma unroll
                 for (int f = 0; f < kFolds; ++f) {
                     Frag wf[FOLD];
@@ -231,7 +257,7 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
                     const float z = ASYM ? a.zero_const + (float)zero[d][f] : a.zero_const;
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        f32x4 part = sums[((kt * kFolds + f) * MT + mt) * 4 + c];
+                        f32x4 part = sums[((at * kFolds + f) * MT + mt) * 4 + c];
                         if constexpr (ASYM) {
 #pragma unroll
                             for (int r = 0; r < 4; ++r) part[r] *= z;
@@ -240,12 +266,12 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
                         for (int j = 0; j < FOLD; ++j)
 #pragma unroll
                             for (int p = 0; p < P; ++p)
-                                part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + kt * 256 + (f * FOLD + j) * 64), wf[j], part);
+                                part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + at * 256 + (f * FOLD + j) * 64), wf[j], part);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[mt][r] = __builtin_fmaf(scale[d][f], part[r], acc[mt][r]);
                     }
                 }
-                if (kt + DEPTH * splits < tiles) load(d, kt + DEPTH * splits);
+                if (kt + kDepth * splits < tiles) load(d, kt + kDepth * splits);
             }
         }
     }
@@ -558,23 +584,41 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
 // ------------------------------------------------------------------------------------------------------------- host --
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <typename T, int FOLD, int MT, bool ASYM>
-int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stream) {
-    constexpr int kDepth = 2;
-    const auto kernel = int4_linear_lds_kernel<T, FOLD, MT, kDepth, ASYM>;
-    if (lds > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+// How the kernel of few activations shares a call out: waves to a row tile, turns whose activations LDS holds at a time
+// (0: not even one), bytes of LDS.
+struct LdsPlan { int splits, turns, row_bytes; bool chunked; size_t lds; };
+inline LdsPlan plan_lds(const Int4Args& a, int parts, int folds, int mt) {
+    LdsPlan p;
+    // as many waves to a row tile as one workgroup on each of the 256 compute units gives
+    p.splits = kLdsWaves;
+    while (p.splits > 1 && (p.splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / p.splits) > 256)) p.splits /= 2;
+    const int64_t room = 160 * 1024 - a.m * parts * 16, of_tile = a.m * parts * 256 + folds * mt * 64;
+    const int64_t fit = room > 0 ? room / of_tile : 0;
+    while (p.splits > 1 && p.splits > fit) p.splits /= 2;
+    const int64_t all = ceil_div(a.tiles, p.splits), most = fit / p.splits;
+    p.chunked = a.tiles > fit;
+    p.turns = most == 0 ? 0 : (int)ceil_div(all, ceil_div(all, most));
+    const int64_t held = p.chunked ? p.turns * p.splits : a.tiles;
+    p.row_bytes = (int)(held * 256 + 16);
+    const size_t red = (size_t)kLdsWaves * 1024 * mt, bytes = (size_t)(a.m * parts * p.row_bytes + held * folds * mt * 64);
+    p.lds = bytes > red ? bytes : red;
+    return p;
+}
+
+template <typename T, int FOLD, int MT, bool ASYM, bool CHUNKED>
+int launch_lds(const Int4Args& a, const LdsPlan& p, hipStream_t stream) {
+    const auto kernel = int4_linear_lds_kernel<T, FOLD, MT, ASYM, CHUNKED>;
+    if (p.lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
         if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
     }
-    // as many waves to a row tile as one workgroup on each of the 256 compute units gives
-    int splits = kLdsWaves;
-    while (splits > 1 && (splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / splits) > 256)) splits /= 2;
-    kernel<<<(unsigned)ceil_div(a.ntiles, kLdsWaves / splits), kLdsThreads, lds, stream>>>(a, splits, (int)row_bytes);
+    kernel<<<(unsigned)ceil_div(a.ntiles, kLdsWaves / p.splits), kLdsThreads, p.lds, stream>>>(a, p.splits, p.turns, p.row_bytes);
     return check_launch("ahq_int4_linear");
 }
 template <typename T, int FOLD, int MT>
-int launch_lds(const Int4Args& a, size_t row_bytes, size_t lds, hipStream_t stream) {
-    return a.zero ? launch_lds<T, FOLD, MT, true>(a, row_bytes, lds, stream) : launch_lds<T, FOLD, MT, false>(a, row_bytes, lds, stream);
+int launch_lds(const Int4Args& a, const LdsPlan& p, hipStream_t stream) {
+    if (p.chunked) return a.zero ? launch_lds<T, FOLD, MT, true, true>(a, p, stream) : launch_lds<T, FOLD, MT, false, true>(a, p, stream);
+    return a.zero ? launch_lds<T, FOLD, MT, true, false>(a, p, stream) : launch_lds<T, FOLD, MT, false, false>(a, p, stream);
 }
 
 template <typename T, int FOLD, int MT, int NW, bool ASYM, bool WHOLE>
@@ -586,7 +630,7 @@ int launch_many(const Int4Args& a, hipStream_t stream) {
         if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
     }
     const int64_t mblocks = ceil_div(a.m, 16 * MT), nblocks = ceil_div(a.n, 64 * NW);
-    if (mblocks * nblocks > (1 << 30)) return set_error("too many activations and channels in one call"), AHQ_ERR_UNSUPPORTED;
+    if (mblocks * nblocks > (1 << 22)) return set_error("too many activations and channels in one call"), AHQ_ERR_UNSUPPORTED;
     kernel<<<(unsigned)(ceil_div(mblocks * nblocks, 8) * 8), kManyWaves * kWave, lds, stream>>>(a, (int)mblocks, (int)nblocks);
     return check_launch("ahq_int4_linear");
 }
@@ -599,33 +643,34 @@ int launch_many(const Int4Args& a, hipStream_t stream) {
 
 template <typename T, int FOLD>
 int launch_linear(Int4Args a, int64_t group, hipStream_t stream) {
-    // Folds per group, and the activations' room in LDS for the kernel of few activations.
+    // folds per group
     const auto folds = [&](int64_t columns) {
         const uint64_t n = group == a.k ? 1ull << 32 : (uint64_t)(group / columns);
         a.fold_inverse = ((1ull << 32) + n - 1) / n;
     };
-    const size_t row_bytes = (size_t)a.tiles * 256 + 16;
-    const size_t xbytes = (size_t)a.m * row_bytes * Int4Traits<T>::kParts + (size_t)a.tiles * (4 / FOLD) * (a.m > 16 ? 128 : 64);
-    const size_t red = (size_t)kLdsWaves * 1024 * (a.m > 16 ? 2 : 1), lds = xbytes > red ? xbytes : red;
-    if (a.m <= 32 && lds <= 160 * 1024) {
-        folds(32 * FOLD);
-        if (a.m <= 16) return launch_lds<T, FOLD, 1>(a, row_bytes, lds, stream);
-        return launch_lds<T, FOLD, 2>(a, row_bytes, lds, stream);
+    // at 32 activations, against blocks of 32 x 64: 4096 x 4096 13.6 and 16.5 us, 4096 x 14336 41 and 57 us against 32 x 128
+    if (a.m <= 32) {
+        const LdsPlan p = plan_lds(a, Int4Traits<T>::kParts, 4 / FOLD, a.m <= 16 ? 1 : 2);
+        if (p.turns > 0) {
+            folds(32 * FOLD);
+            return a.m <= 16 ? launch_lds<T, FOLD, 1>(a, p, stream) : launch_lds<T, FOLD, 2>(a, p, stream);
+        }
     }
     constexpr int kFold = FOLD == 1 ? 1 : 2;
     folds(32 * kFold);
     if constexpr (sizeof(T) == 2) {
-        // the largest block that still gives most of the 256 compute units a workgroup
-#ifndef T4
-#define T4 192
-#endif
-#ifndef T2
-#define T2 100
-#endif
-        if (ceil_div(a.m, 64) * ceil_div(a.n, 256) >= T4) return launch_many<T, kFold, 4, 4>(a, stream);
-        if (ceil_div(a.m, 64) * ceil_div(a.n, 128) >= T2) return launch_many<T, kFold, 4, 2>(a, stream);
+        // The smallest block whose workgroups still run on the 256 compute units all at once, else the largest: a block's time
+        // hardly depends on how many others run, and it grows more slowly than its size.  At 4096 x 4096, in the order 32 x 64,
+        // 32 x 128, 64 x 128, 64 x 256: 64 activations 17, 21, 29, 40 us; 256: 31, 23, 30, 41; 512: -, 40, 31, 41;
+        // 640: -, 56, 57, 41.
+        const auto one_round = [&](int64_t rows, int64_t channels) { return ceil_div(a.m, rows) * ceil_div(a.n, channels) <= 256; };
+        if (one_round(32, 64)) return launch_many<T, kFold, 2, 1>(a, stream);
+        if (one_round(32, 128)) return launch_many<T, kFold, 2, 2>(a, stream);
+        if (one_round(64, 128)) return launch_many<T, kFold, 4, 2>(a, stream);
+        return launch_many<T, kFold, 4, 4>(a, stream);
+    } else {
+        return launch_many<T, kFold, 2, 2>(a, stream);  // its three parts fill LDS
     }
-    return launch_many<T, kFold, 2, 2>(a, stream);
 }
 
 template <typename T>
@@ -640,7 +685,7 @@ int launch_linear(const Int4Args& a, int64_t group, hipStream_t stream) {
 }  // namespace ahq
 
 extern "C" size_t ahq_int4_packed_bytes(int64_t n, int64_t k) {
-    if (n <= 0 || k <= 0 || n > (1ll << 31) || k > (1ll << 20)) return 0;
+    if (n <= 0 || k <= 0 || n > (1ll << 28) || k > (1ll << 20)) return 0;
     return (size_t)(ahq::ceil_div(n, ahq::kTileRows) * ahq::ceil_div(k, ahq::kTileCols) * ahq::kTileBytes);
 }
 
@@ -651,7 +696,7 @@ extern "C" int ahq_int4_pack(const int8_t* codes, int64_t n, int64_t k, int32_t 
     if (qmin < -128 || qmin > 112) return set_error("qmin outside [-128, 112]"), AHQ_ERR_INVALID;
     if ((uintptr_t)packed % 16) return set_error("packed weights must be 16-byte aligned"), AHQ_ERR_INVALID;
     const int64_t tiles = ceil_div(k, kTileCols), words = (int64_t)ahq_int4_packed_bytes(n, k) / 4;
-    if (ceil_div(words, kBlock) > 0x7fffffffll) return set_error("weight too large"), AHQ_ERR_UNSUPPORTED;
+    if (words > 0xffffff00ll) return set_error("weight too large"), AHQ_ERR_UNSUPPORTED;
     int4_pack_kernel<<<(unsigned)ceil_div(words, kBlock), kBlock, 0, static_cast<hipStream_t>(stream)>>>(
         codes, n, k, qmin, tiles, words, static_cast<uint32_t*>(packed));
     return check_launch("ahq_int4_pack");
@@ -680,7 +725,6 @@ extern "C" int ahq_int4_linear(const ahq_int4_weight* w, int32_t dtype, const vo
     a.tiles = ceil_div(k, kTileCols), a.ntiles = ceil_div(n, kTileRows), a.groups = k / group;
     a.zero_const = w->zero_const;
     a.vec_x = (uintptr_t)x % 16 == 0 && (ldx * (int64_t)e) % 16 == 0;
-    a.vec_y = (uintptr_t)y % (4 * e) == 0 && ldy % 4 == 0;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == AHQ_F32) return launch_linear<float>(a, group, s);
     if (dtype == AHQ_F16) return launch_linear<f16_t>(a, group, s);

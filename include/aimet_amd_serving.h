@@ -21,8 +21,8 @@ extern "C" {
  *   y[m][j] = sum_g scale[j][g] * ( sum_{k in group g} x[m][k] * (code[j][k] - qmin + zero[j][g] + zero_const) ) + bias[j]
  *
  * ahq_int4_pack lays out the codes of an [n][k] weight (row-major bytes, each in [qmin, qmin + 15]; only the low four
- * bits of code - qmin are kept) as ahq_int4_linear reads them, ahq_int4_packed_bytes(n, k) bytes (0: bad shape; k is at
- * most 2^20).
+ * bits of code - qmin are kept) as ahq_int4_linear reads them, ahq_int4_packed_bytes(n, k) bytes (0: bad shape; n is
+ * at most 2^28, k at most 2^20).
  * ahq_int4_linear: x is [m][k] of `dtype` with rows ldx elements apart, y [m][n] with rows ldy apart, both dense along
  * the row; m is at most 2^20.  bias: n values of `dtype`, or NULL.  Products and sums are float32 with exact factors; y is
  * rounded once.
