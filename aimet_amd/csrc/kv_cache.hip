@@ -991,7 +991,7 @@ extern "C" int ahq_kv_append(const ahq_kv_cache* cache, const ahq_kv_tokens* x, 
     if (!supported(cache)) return AHQ_ERR_UNSUPPORTED;
     if (x->tokens == 0) return AHQ_OK;
     if (!x->k || !x->v) return set_error("null argument"), AHQ_ERR_INVALID;
-    if (x->tokens > (1 << 29)) return set_error("too many tokens"), AHQ_ERR_UNSUPPORTED;
+    if (x->tokens > (1 << 28)) return set_error("too many tokens"), AHQ_ERR_UNSUPPORTED;
     const int64_t e = x->dtype == AHQ_F32 ? 4 : 2;
     KvAppendArgs a;
     a.x[0] = x->k, a.x[1] = x->v;
@@ -1019,6 +1019,7 @@ extern "C" int ahq_kv_dequantize(const ahq_kv_cache* cache, int32_t dtype, int32
     if (length < 0 || length > cache->capacity) return set_error("length outside the cache"), AHQ_ERR_INVALID;
     if (!supported(cache)) return AHQ_ERR_UNSUPPORTED;
     if (length == 0) return AHQ_OK;
+    if (length > (1 << 29)) return set_error("more than 2^29 tokens in one call"), AHQ_ERR_UNSUPPORTED;
     if (!k || !v) return set_error("null argument"), AHQ_ERR_INVALID;
     if (((uintptr_t)k | (uintptr_t)v) % 16) return set_error("outputs must be 16-byte aligned"), AHQ_ERR_INVALID;
     KvValuesArgs a;

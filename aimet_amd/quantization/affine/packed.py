@@ -33,9 +33,9 @@ def _refuse_gradients(what: str, *tensors) -> None:
 class PackedWeight:
     """The codes of a weight [out_features, in_features] with at most 16 levels, packed for ``packed_linear``.
 
-    Attributes: ``codes`` (uint8, the library's layout), ``scale`` (float32 [out_features / 16, groups, 16],
-    channels in sixteens and padded to them), ``zero`` (int8 of the same shape, or None where one zero point serves all), ``zero_const``, ``shape``, ``group``
-    (columns that share a scale)."""
+    Attributes: ``codes`` (uint8, the library's layout), ``scale`` (float32 [out_features / 16, groups, 16], channels in
+    sixteens and padded to them), ``zero`` (int8 of the same shape, or None where one zero point serves all),
+    ``zero_const``, ``shape``, ``group`` (columns that share a scale)."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], zero_const: float,
                  shape, group: int):
@@ -154,7 +154,8 @@ class PackedWeight:
 
 def packed_linear(x: torch.Tensor, weight: PackedWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ dequantized(weight).T + bias`` for activations [..., in_features] in float32, bfloat16 or float16; the
-    result has their type.  An infinite or NaN activation makes its row NaN."""
+    result has their type.  An infinite or NaN activation makes its row NaN, as do sums of activations times codes that
+    leave float32 before the scale is applied."""
     n, k = weight.shape
     _lib.require_device(x, "x")
     if x.dtype not in _lib.DTYPE_CODE:
@@ -168,8 +169,9 @@ def packed_linear(x: torch.Tensor, weight: PackedWeight, bias: Optional[torch.Te
         raise RuntimeError(f"bias must have shape {(n,)} and the activations' type and device; got "
                            f"{tuple(bias.shape)}, {bias.dtype}, {bias.device}")
     _refuse_gradients("packed_linear", x, bias)
-    x = x.as_subclass(torch.Tensor)
-    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=device)
+    if type(x) is not torch.Tensor:
+        x = x.as_subclass(torch.Tensor)
+    y = x.new_empty(x.shape[:-1] + (n,))
     m = y.numel() // n
     if m == 0:
         return y

@@ -170,7 +170,8 @@ class QuantizedKVCache:
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
         if not math.isfinite(scale):
             raise RuntimeError(f"scale must be finite; got {scale}")
-        q = q.as_subclass(torch.Tensor)
+        if type(q) is not torch.Tensor:
+            q = q.as_subclass(torch.Tensor)
         out = torch.empty_like(q)
         if queries == 0:
             return out

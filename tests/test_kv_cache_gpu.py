@@ -120,6 +120,24 @@ def test_append_borders(device, dtype):
     assert bool(torch.isfinite(torch.stack(cache.dequantize())).all())
 
 
+@pytest.mark.parametrize("dtype,amax", [(torch.float16, a) for a in (1.0, 127.0, 100.0625, 65504.0, 2.0 ** -14, 2.0 ** -24)]
+                         + [(torch.bfloat16, a) for a in (1.0, 127.0, 0.7109375, 2.0 ** 127, 2.0 ** -100, 2.0 ** -126)]
+                         + [(torch.float32, a) for a in (127.0, 0.1, 3e38, 1e-39)])
+def test_append_every_code(device, dtype, amax):
+    """All 16-bit values (float32: their multiples of the maximum) under one maximum, ties included: codes are exact."""
+    amax = torch.tensor(amax, dtype=dtype)
+    patterns = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16)
+    x = (patterns.view(torch.float16).float() / 65504 * amax if dtype == torch.float32 else patterns.view(dtype)).nan_to_num(0, 0, 0)
+    x = torch.where(x.abs() > amax, amax, x).view(1, 16, 64, 64)
+    x[:, :, 0, 0] = amax
+    cache = QuantizedKVCache(1, 16, 64, 64, 64, device)
+    cache.append(x.to(device), x.flip(3).to(device), 0)
+    want = (x.double() * 127 / amax.double()).round()  # the quotient is exact to 2^-53, borders are 2^-40 apart at least
+    k, v = _codes(cache)
+    assert torch.equal(k, want) and torch.equal(v, want.flip(3))
+    assert bool((cache.k_amax == amax.float().item()).all()) and bool((cache.v_amax == amax.float().item()).all())
+
+
 def test_append_leaves_the_rest(device):
     """Tokens in front of the cache and behind it are dropped, padding is not read into scales, what lies behind the last
     token stays as it was, and a rewritten block starts a new scale at its first token."""
@@ -253,6 +271,16 @@ def test_attend_several_tokens(device, heads, groups, queries, length, dtype):
 def test_attend_prompts(device, queries, length, dim, dtype):
     cache = _filled(1, 2, length, dim, 64, dtype, device)
     _attend_check(cache, _queries(1, 8, queries, dim, dtype, device), length)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("dim,capacity", [(64, 33000), (128, 16500), (256, 8250)])
+def test_attend_large_caches(device, dim, capacity, dtype):
+    """Codes that the caches do not keep (32 MiB and more), few rows; short and long sequences in one call."""
+    cache = _filled(4, 4, capacity, dim, 32, dtype, device)
+    lengths = [capacity, 1, 700, capacity // 2]
+    q = _queries(4, 8, 2, dim, dtype, device)
+    _attend_check(cache, q, lengths, 2, given=(torch.tensor(lengths, dtype=torch.int32, device=device), 2))
 
 
 @pytest.mark.parametrize("queries", [1, 4, 80, 150])

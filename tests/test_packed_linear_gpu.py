@@ -60,6 +60,11 @@ SHAPES = [  # tokens, out, in, group
     (31, 31, 31, 31), (32, 96, 4096, 4096), (33, 128, 1152, 96), (47, 200, 256, 256), (64, 112, 768, 64),
     (65, 130, 512, 32), (100, 1000, 1001, 1001), (128, 128, 128, 128), (129, 257, 384, 64), (200, 64, 8192, 64),
     (257, 512, 2048, 128), (300, 384, 1000, 1000), (513, 272, 640, 64), (1025, 144, 256, 32),
+    # activations that LDS does not hold at once
+    (16, 100, 8192, 64), (32, 50, 5000, 5000), (7, 40, 14336, 128), (3, 33, 20000, 20000), (29, 4100, 3840, 32),
+    # blocks of 32 x 128, 64 x 128 and 64 x 256: whole steps, rows that end inside one, groups of 32
+    (257, 2000, 192, 64), (300, 3300, 320, 32), (290, 3400, 130, 130), (1000, 2200, 256, 64), (999, 2201, 320, 32),
+    (1000, 2200, 130, 130),
 ]
 
 
@@ -104,6 +109,21 @@ def test_strides_and_alignment(device, dtype, m):
     assert torch.equal(packed_linear(x, w), packed_linear(x.view(-1, k), w).view(2, 3, m, n))
     assert packed_linear(x[0, 0, 0], w).shape == (n,)
     assert packed_linear(x[:, :0], w).shape == (2, 0, m, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d).split(".")[-1])
+def test_large_strides(device, dtype):
+    """Rows 64 MB apart, so that a block's last row lies past 32-bit offsets; one row that is repeated."""
+    n, k, m = 40, 64, 70
+    codes, scale, offset = _case(n, k, 32, False, 3, device)
+    w = PackedWeight.pack(codes, scale, offset)
+    base = torch.empty(m << 24, dtype=dtype, device=device)
+    x = base.view(m, 1 << 24)[:, 8:8 + k]
+    x.copy_(torch.randn(m, k, generator=torch.Generator().manual_seed(1)).to(dtype))
+    want = packed_linear(x.contiguous(), w)
+    _check(want, x, codes, scale, offset)
+    assert torch.equal(packed_linear(x, w), want)
+    assert torch.equal(packed_linear(x[:20], w), packed_linear(x[:20].contiguous(), w))
 
 
 def test_grids(device):
