@@ -86,11 +86,16 @@ class PackedWeight:
         if groups > 1 and (k // groups) % 32:
             raise RuntimeError(f"groups of {k // groups} columns are not supported: a multiple of 32, or the whole row")
         qmin = (-8 if offset is None else 0) if qmin is None else int(qmin)
-        lo, hi = codes.min().item(), codes.max().item()
-        if lo < qmin or hi > qmin + 15:
-            raise RuntimeError(f"codes in [{lo}, {hi}] do not fit the 16 levels from {qmin} on")
         if not -128 <= qmin <= 112:
             raise RuntimeError(f"qmin must be in [-128, 112]; got {qmin}")
+        # everything that has to be known of the values is read back at once
+        known = [t.double() for t in torch.aminmax(codes)]
+        if offset is not None:
+            off = offset.detach().float()
+            known += [t.double() for t in (*torch.aminmax(off), (off == off.round()).all())]
+        lo, hi, *about_offset = torch.stack(known).tolist()
+        if not qmin <= lo <= hi <= qmin + 15:
+            raise RuntimeError(f"codes in [{lo:g}, {hi:g}] do not fit the 16 levels from {qmin} on")
         npad = -(-n // 16) * 16
 
         def in_sixteens(t, dtype):
@@ -102,9 +107,8 @@ class PackedWeight:
         scales = in_sixteens(scale.detach(), torch.float32)
         zero, zero_const = None, qmin + float(zero_point_shift)
         if offset is not None:
-            off = offset.detach().float()
-            o_lo, o_hi = off.min().item(), off.max().item()
-            if not (math.isfinite(o_lo) and math.isfinite(o_hi)) or not bool((off == off.round()).all()):
+            o_lo, o_hi, whole = about_offset
+            if not (math.isfinite(o_lo) and math.isfinite(o_hi) and whole):
                 raise RuntimeError("offsets must be whole numbers")
             if o_lo == o_hi:
                 zero_const += o_lo
