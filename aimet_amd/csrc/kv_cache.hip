@@ -874,6 +874,45 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttendArgs a) {
     for (int r = 0; r < 4; ++r) to[r] = store_cast<T>(total == 0.0f ? 0.0f : value[r] / total);
 }
 
+// The same for up to eight splits, where rows are many: D / 4 lanes to a row (1024 queries of 1 x 8 x 4 heads in two
+// splits: 37 us in all, and 69 us with a workgroup for each row).
+template <typename T, int D>
+__global__ __launch_bounds__(kJoinThreads) void kv_join_rows_kernel(KvAttendArgs a) {
+    constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes;
+    const int row = blockIdx.x * kRows + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    const int64_t bh = blockIdx.y;
+    const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
+    if (row >= a.rows) return;
+    const int used = used_splits(a, view_sequence(a, b), row);
+    if (used <= 1) return;
+    const int64_t at = (bh * a.rows + row) * a.splits;
+    const float* stat = a.part_stat + at * 2;
+    const f32x4* part = reinterpret_cast<const f32x4*>(a.part + at * D) + lane;
+    float best = -__builtin_inff();
+    for (int s = 0; s < used; ++s) best = fmaxf(best, stat[2 * s]);
+    const float base = best == -__builtin_inff() ? 0.0f : best;
+    float total = 0.0f;
+    f32x4 value = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < used; ++s) {
+        const float f = __builtin_amdgcn_exp2f(stat[2 * s] - base);
+        const f32x4 v = part[s * kLanes];
+        total = __builtin_fmaf(f, stat[2 * s + 1], total);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) value[r] = __builtin_fmaf(f, v[r], value[r]);
+    }
+    T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * lane;
+    Pack<T, 4> out;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out.v[r] = store_cast<T>(total == 0.0f ? 0.0f : value[r] / total);
+    if (a.vec_out) {
+        store_pack<T, 4>(to, out);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[r] = out.v[r];
+    }
+}
+
 // -------------------------------------------------------------------------------------------------------------- host --
 inline bool check_cache(const ahq_kv_cache* cache) {
     if (!cache || !cache->k_codes || !cache->v_codes || !cache->k_amax || !cache->v_amax) return set_error("null cache"), false;
@@ -919,22 +958,40 @@ int launch_values(const KvValuesArgs& a, int64_t bh, int32_t dim, hipStream_t s)
     return dim == 64 ? launch_values<T, 64>(a, bh, s) : dim == 128 ? launch_values<T, 128>(a, bh, s) : launch_values<T, 256>(a, bh, s);
 }
 
-// How a call is shared out.  Up to 32 rows (decoding): 16 to a workgroup, whose four waves share the tokens.  More rows: each
-// of four or eight waves its own 32 (float32 queries, 256 channels: 16), so that a tile of codes is turned into float16
-// once for all of them.  The token axis is split until every compute unit has eight waves, which is what runs there at
-// once, in one round of equal shares with one length for all sequences; where lengths differ (and are known to the device
-// alone) shares a third as long even them out.  A share is at least four tiles.
+// How a call is shared out.
+//
+// waves = 0 (kv_attend_kernel): 16 rows to a workgroup, whose four waves share the tokens.  For up to 32 rows, and for more
+// where they make little work: fewer than 128 workgroups of the other kind, of at most 2048 token tiles together.
+// Otherwise (kv_prompt_kernel) each of four or eight waves has its own 32 rows (float32 queries, 256 channels: 16), so that
+// a tile of codes is turned into float16 once for all of them.  Eight share it better; four make more workgroups, which is
+// better where they fill the chip once without a split of the token axis, or where a split would cost more than it gives
+// (it writes and joins float32 sums, about the time of eight tiles).
+//   sequences x heads x groups, queries of tokens, head size   waves 0   4 in one split   8
+//   1 x 8 x 4,  64 of 4096, 128                                   22 us             94   32
+//   1 x 4 x 4, 512 of 1024, 128                                   17                29   29
+//   1 x 8 x 4, 256 of 16384, 128                                 131               356   81
+//   1 x 8 x 4, 512 of 512, 128                                    20                19   27
+//   1 x 8 x 4, 1024 of 1024, 128                                  38                30   37
+//   1 x 8 x 4, 1024 of 4096, 128                                 117                96   83
+//   1 x 8 x 4, 2048 of 2048, 128                                  91                59   70
+//   2 x 8 x 4, 2048 of 3048, 128                                 280               148  144
+//
+// The token axis is split until every compute unit has eight waves, which is what runs there at once, in one round of equal
+// shares with one length for all sequences; where lengths differ (and are known to the device alone) shares a third as long
+// even them out.  A share is at least four tiles.
 struct AttendPlan { int32_t waves, row_tile, splits, split_tiles; };
 inline AttendPlan plan_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q) {
     const int64_t bh = (int64_t)cache->batch * cache->heads, rows = (int64_t)q->queries * (q->query_heads / cache->heads);
     const int64_t tokens = q->lengths ? cache->capacity : q->length_all;
     const int64_t tiles = (tokens + kKvTile - 1) / kKvTile;
     const int wave_rows = q->dtype == AHQ_F32 || cache->head_dim == 256 ? 16 : 32;
+    const int64_t of_four = bh * ((rows + 4 * wave_rows - 1) / (4 * wave_rows));
+    const bool whole = of_four <= 512 && tiles * (512 - of_four) <= 8 * 512;
     AttendPlan p;
-    p.waves = rows <= 32 ? 0 : rows <= 4 * wave_rows ? 4 : 8;  // 0: waves share the tokens
+    p.waves = rows <= 32 || (of_four < 128 && of_four * tiles <= 2048) ? 0 : whole ? 4 : 8;
     p.row_tile = p.waves == 0 ? 16 : p.waves * wave_rows;
     const int64_t room = (p.waves == 8 ? 256 : 512) * (q->lengths ? 3 : 1), wgs = bh * ((rows + p.row_tile - 1) / p.row_tile);
-    int64_t n = (wgs * tiles + room - 1) / room;
+    int64_t n = p.waves == 4 ? tiles : (wgs * tiles + room - 1) / room;
     n = (n + 3) / 4 * 4;
     p.split_tiles = (int32_t)(n < 4 ? 4 : n);
     n = (tiles + p.split_tiles - 1) / p.split_tiles;
@@ -967,7 +1024,12 @@ int launch_attend(const KvAttendArgs& a, const AttendPlan& p, int64_t bh, hipStr
     else
         rc = launch_with_lds(kv_prompt_kernel<T, D, NR, 8>, grid, 8 * kWave, buffers, a, s);
     if (rc != AHQ_OK || p.splits == 1) return rc;
-    kv_join_kernel<T, D><<<dim3((unsigned)a.rows, (unsigned)bh), kJoinThreads, 0, s>>>(a);
+    if (p.splits <= 8) {
+        constexpr int kRows = kJoinThreads / (D / 4);
+        kv_join_rows_kernel<T, D><<<dim3((unsigned)((a.rows + kRows - 1) / kRows), (unsigned)bh), kJoinThreads, 0, s>>>(a);
+    } else {
+        kv_join_kernel<T, D><<<dim3((unsigned)a.rows, (unsigned)bh), kJoinThreads, 0, s>>>(a);
+    }
     return check_launch("ahq_kv_attend");
 }
 template <typename T>

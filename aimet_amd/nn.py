@@ -657,17 +657,18 @@ def fold_param_quantizers(model: nn.Module):
 def pack_linears(model: nn.Module) -> int:
     """Replaces every QuantizedLinear of ``model`` whose weight has an affine encoding of at most 16 levels by its
     packed form (QuantizedLinear.pack); returns how many.  Other layers are left as they are."""
-    count = 0
+    packed = {}  # a layer that stands in several places stays one layer
     for parent in list(model.modules()):
-        for name, child in list(parent.named_children()):
+        for name, child in list(parent._modules.items()):
             if not isinstance(child, QuantizedLinear):
                 continue
             wq = child.param_quantizers["weight"]
             encoded = wq if wq is not None else getattr(child.weight, "encoding", None)
             if isinstance(encoded, (AffineQuantizerBase, AffineEncoding)) and encoded.qmax - encoded.qmin <= 15:
-                setattr(parent, name, child.pack())
-                count += 1
-    return count
+                if child not in packed:
+                    packed[child] = child.pack()
+                setattr(parent, name, packed[child])
+    return len(packed)
 
 
 def _remove_from_all(model, method: str) -> _Removed:

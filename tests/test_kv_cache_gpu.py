@@ -274,6 +274,29 @@ def test_attend_prompts(device, queries, length, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("batch,heads,groups,queries,length,dim", [
+    # four waves with rows of their own; eight in several splits; eight in one; a long cache in many splits
+    (8, 16, 1, 40, 200, 64), (8, 16, 3, 40, 300, 128), (8, 16, 1, 64, 333, 256), (8, 16, 1, 50, 750, 64),
+    (4, 32, 2, 70, 1100, 128), (8, 16, 1, 50, 770, 256), (8, 16, 1, 600, 600, 64), (1, 1, 1, 40, 140000, 64)])
+def test_attend_many_prompts(device, batch, heads, groups, queries, length, dim, dtype):
+    cache = _filled(batch, heads, length, dim, 32, dtype, device)
+    _attend_check(cache, _queries(batch, heads * groups, queries, dim, dtype, device), length)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("capacity,dim", [(300, 64), (800, 64), (800, 128), (700, 256)])
+def test_attend_many_ragged_prompts(device, capacity, dim, dtype):
+    b, t = 64, 40
+    cache = _filled(b, 2, capacity, dim, 16, dtype, device)
+    g = torch.Generator().manual_seed(0)
+    lengths, counts = (torch.randint(0, n + 1, (b,), generator=g, dtype=torch.int32) for n in (capacity, t))
+    q = _queries(b, 2, t, dim, dtype, device).contiguous()
+    clean = _attend_check(cache, q, lengths.tolist(), counts.tolist(), given=(lengths.to(device), counts.to(device)))
+    q[(torch.arange(t) >= counts[:, None]).to(device)[:, None].expand(b, 2, t)] = float("nan")
+    assert torch.equal(cache.attend(q, lengths.to(device), counts.to(device)), clean)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
 @pytest.mark.parametrize("dim,capacity", [(64, 33000), (128, 16500), (256, 8250)])
 def test_attend_large_caches(device, dim, capacity, dtype):
     """Codes that the caches do not keep (32 MiB and more), few rows; short and long sequences in one call."""

@@ -295,6 +295,13 @@ def test_packed_model_round_trip(device):
         assert torch.equal(twin(x).as_subclass(torch.Tensor), model[0](x).as_subclass(torch.Tensor))
 
 
+def test_a_shared_layer_stays_one_layer(device):
+    layer, _ = _layer(device, torch.float32, WEIGHT_QUANTIZERS["channel"]())
+    model = torch.nn.ModuleDict({"a": layer, "b": torch.nn.Sequential(layer, torch.nn.ReLU()), "c": layer})
+    assert qnn.pack_linears(model) == 1
+    assert model["a"] is model["b"][0] is model["c"] and isinstance(model["a"], qnn.PackedLinear)
+
+
 def test_folded_weight_packs(device):
     q, x = _layer(device, torch.float32, WEIGHT_QUANTIZERS["block"]())
     want = q.pack()
