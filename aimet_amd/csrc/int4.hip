@@ -119,6 +119,9 @@ struct Int4Args {
 // the waves at a time) and are the A operand here, the weight's rows the columns of the result: a lane's results belong to
 // one channel, whose scale and zero point are one register.  Bound by the stream of codes, so a wave asks for kDepth tiles
 // at once, right behind its share of the activations; those are read back from LDS, whose waits do not hold up the stream.
+//
+// One token x 14336 x 4096 (33 MB): 10.7 us, 3.1 TB/s; of that launch 2.0, activations and epilogue 2.1, their sums 0.8, the
+// loop 5.8.  One, three and four tiles at once instead of two: 12.0, 11.3, 11.7 us.
 constexpr int kLdsWaves = 16;
 constexpr int kLdsThreads = kLdsWaves * kWave;
 
@@ -308,6 +311,9 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
 // operands and 16 * MT to scale the finished group sums (every 64 columns at least): the two kinds nearly balance.  The
 // wave that brings activations in sums them, with one matrix instruction a fragment.  The groups' results are added
 // through LDS, in a fixed order.
+//
+// Bound by the issue of vector instructions next to the matrix ones.  2048 x 2048 x 8192 bfloat16: 83 us, 830 TFLOP/s;
+// 300 x 4096 x 4096 float16 with zero points: 33.5 us.  Codes asked for four steps ahead instead of two: 107 us (spills).
 constexpr int kManyWaves = 8;
 
 // NW waves side by side (of 64 channels each), 8 / NW groups along the row.
