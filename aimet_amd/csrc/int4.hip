@@ -590,20 +590,20 @@ __global__ __launch_bounds__(kBlock) void int4_pack_kernel(const int8_t* __restr
 // ------------------------------------------------------------------------------------------------------------- host --
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How the kernel of few activations shares a call out: waves to a row tile, turns whose activations LDS holds at a time
-// (0: not even one), bytes of LDS.
+// How the kernel of few activations shares a call out: waves to a row tile, turns whose activations LDS holds at a time,
+// bytes of LDS.
 struct LdsPlan { int splits, turns, row_bytes; bool chunked; size_t lds; };
 inline LdsPlan plan_lds(const Int4Args& a, int parts, int folds, int mt) {
     LdsPlan p;
     // as many waves to a row tile as one workgroup on each of the 256 compute units gives
     p.splits = kLdsWaves;
     while (p.splits > 1 && (p.splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / p.splits) > 256)) p.splits /= 2;
-    const int64_t room = 160 * 1024 - a.m * parts * 16, of_tile = a.m * parts * 256 + folds * mt * 64;
-    const int64_t fit = room > 0 ? room / of_tile : 0;
+    // 6 tiles at least: 32 activations, three parts, four folds
+    const int64_t fit = (160 * 1024 - a.m * parts * 16) / (a.m * parts * 256 + folds * mt * 64);
     while (p.splits > 1 && p.splits > fit) p.splits /= 2;
     const int64_t all = ceil_div(a.tiles, p.splits), most = fit / p.splits;
     p.chunked = a.tiles > fit;
-    p.turns = most == 0 ? 0 : (int)ceil_div(all, ceil_div(all, most));
+    p.turns = (int)ceil_div(all, ceil_div(all, most));  // even shares
     const int64_t held = p.chunked ? p.turns * p.splits : a.tiles;
     p.row_bytes = (int)(held * 256 + 16);
     const size_t red = (size_t)kLdsWaves * 1024 * mt, bytes = (size_t)(a.m * parts * p.row_bytes + held * folds * mt * 64);
@@ -657,10 +657,8 @@ int launch_linear(Int4Args a, int64_t group, hipStream_t stream) {
     // at 32 activations, against blocks of 32 x 64: 4096 x 4096 13.6 and 16.5 us, 4096 x 14336 41 and 57 us against 32 x 128
     if (a.m <= 32) {
         const LdsPlan p = plan_lds(a, Int4Traits<T>::kParts, 4 / FOLD, a.m <= 16 ? 1 : 2);
-        if (p.turns > 0) {
-            folds(32 * FOLD);
-            return a.m <= 16 ? launch_lds<T, FOLD, 1>(a, p, stream) : launch_lds<T, FOLD, 2>(a, p, stream);
-        }
+        folds(32 * FOLD);
+        return a.m <= 16 ? launch_lds<T, FOLD, 1>(a, p, stream) : launch_lds<T, FOLD, 2>(a, p, stream);
     }
     constexpr int kFold = FOLD == 1 ? 1 : 2;
     folds(32 * kFold);

@@ -673,7 +673,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
     const int i = lane & 15, c = lane >> 4;
     const int64_t bh = blockIdx.x;
     const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-    const int split = blockIdx.z, row0 = blockIdx.y * 16;
+    const int split = blockIdx.z, row0 = (int)(gridDim.y - 1 - blockIdx.y) * 16;  // the rows that see most come first
     const SequenceView seq = view_sequence(a, b);
     const int used = used_splits(a, seq, row0);
     if (split >= used && split > 0) return;
@@ -1117,6 +1117,7 @@ extern "C" int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q,
     if (!supported(cache)) return AHQ_ERR_UNSUPPORTED;
     if (q->queries == 0) return AHQ_OK;
     if (!q->q || !q->out) return set_error("null argument"), AHQ_ERR_INVALID;
+    if (!(q->scale > -0x1p126f && q->scale < 0x1p126f)) return set_error("the scale must be finite"), AHQ_ERR_INVALID;
     const size_t need = ahq_kv_attend_workspace_bytes(cache, q);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return set_error("workspace too small"), AHQ_ERR_WORKSPACE;

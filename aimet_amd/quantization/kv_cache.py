@@ -168,7 +168,7 @@ class QuantizedKVCache:
         count_ptr, count = self._per_sequence(queries if counts is None else counts, "counts", queries)
         length_ptr, length = self._per_sequence(lengths, "lengths", self.capacity)
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        if not math.isfinite(scale):
+        if not abs(scale) < 2.0 ** 126:  # as float32, with room for a factor of log2(e)
             raise RuntimeError(f"scale must be finite; got {scale}")
         if type(q) is not torch.Tensor:
             q = q.as_subclass(torch.Tensor)

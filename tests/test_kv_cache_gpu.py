@@ -471,6 +471,28 @@ def test_another_stream_and_graph(device):
     _attend_check(eager, q, other.tolist(), given=(other, None))
 
 
+def test_two_graphs_and_streams_at_once(device):
+    """Calls whose token axis is split, in two graphs replayed on two streams together: neither uses the other's scratch."""
+    made = []
+    for i, (queries, length) in enumerate(((1, 9000), (40, 140000))):
+        cache = _filled(1, 1, length, 64, 64, torch.bfloat16, device, seed=i)
+        q = _queries(1, 2, queries, 64, torch.bfloat16, device, seed=i).clone()
+        want = cache.attend(q, length)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = cache.attend(q, length)
+        made.append((graph, out, want, torch.cuda.Stream(), cache, q))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, out, _, stream, *_ in made:
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, *_ in made:
+            assert torch.equal(out, want)
+
+
 def test_copies_are_their_own(device):
     import copy
 
@@ -508,7 +530,7 @@ def test_refusals(device):
     for lengths in (-1, 129, 2.0, lens.long(), lens[:1], None):
         with pytest.raises(RuntimeError):
             cache.attend(q, lengths)
-    for bad in ({"scale": float("inf")}, {"scale": float("nan")}, {"counts": 2}):
+    for bad in ({"scale": float("inf")}, {"scale": float("nan")}, {"scale": 1e300}, {"counts": 2}):
         with pytest.raises(RuntimeError):
             cache.attend(q, 4, **bad)
     with pytest.raises(RuntimeError, match="no backward"):

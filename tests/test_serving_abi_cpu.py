@@ -2,6 +2,7 @@
 anything is launched."""
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -94,9 +95,9 @@ def _tokens(**kw):
 
 def _queries(**kw):
     p = 1 << 12
-    a = {**dict(dtype=0, heads=4, queries=1, q=p, out=p, lengths=None, length=100), **kw}
+    a = {**dict(dtype=0, heads=4, queries=1, q=p, out=p, lengths=None, length=100, scale=0.125), **kw}
     return _lib.KvQueries(a["dtype"], a["heads"], a["queries"], a["q"], a["out"], 256, 64, 64, 256, 64, 64, a["lengths"], None,
-                          a["length"], a["queries"], 0.125)
+                          a["length"], a["queries"], a["scale"])
 
 
 BAD_CACHES = [dict(batch=0), dict(heads=-1), dict(capacity=0), dict(capacity=100), dict(batch=40000), dict(k=None),
@@ -120,13 +121,15 @@ def test_kv_refusals(lib):
     for bad in (dict(dtype=5), dict(tokens=-1), dict(k=None), dict(v=None), dict(k=(1 << 12) + 2)):
         assert lib.ahq_kv_append(c, _tokens(**bad), None) == 1, bad
     assert lib.ahq_kv_append(c, _tokens(tokens=0, k=None, v=None), None) == 0
-    assert lib.ahq_kv_append(c, _tokens(tokens=(1 << 29) + 1), None) == _lib.AHQ_ERR_UNSUPPORTED
+    assert lib.ahq_kv_append(c, _tokens(tokens=(1 << 28) + 1), None) == _lib.AHQ_ERR_UNSUPPORTED
     for length in (-1, 129):
         assert lib.ahq_kv_dequantize(c, 0, length, 4096, 4096, None) == 1
     assert lib.ahq_kv_dequantize(c, 0, 4, None, 4096, None) == 1 and lib.ahq_kv_dequantize(c, 9, 4, 4096, 4096, None) == 1
     assert lib.ahq_kv_dequantize(c, 0, 4, 4096, 4100, None) == 1 and lib.ahq_kv_dequantize(c, 0, 0, None, None, None) == 0
+    large = _cache(batch=1, heads=1, capacity=1 << 30)
+    assert lib.ahq_kv_dequantize(large, 0, (1 << 29) + 1, 4096, 4096, None) == _lib.AHQ_ERR_UNSUPPORTED
     for bad in (dict(dtype=3), dict(heads=3), dict(heads=0), dict(queries=-1), dict(q=None), dict(out=None), dict(q=(1 << 12) + 1),
-                dict(queries=1 << 20)):
+                dict(queries=1 << 20), dict(scale=math.inf), dict(scale=-math.inf), dict(scale=math.nan), dict(scale=3e38)):
         assert lib.ahq_kv_attend(c, _queries(**bad), None, 0, None) == 1, bad
     assert lib.ahq_kv_attend(c, _queries(queries=0, q=None, out=None), None, 0, None) == 0
 
