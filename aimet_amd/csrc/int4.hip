@@ -5,8 +5,8 @@
 // u are the codes counted from the lower end of their grid (0..15), z = offset + qmin + zero-point shift, s the float32
 // scale of the group.  The inner sums run on the matrix cores with both factors exact: u is a whole number that
 // bfloat16 and float16 hold, x is used as it is (float32 as a sum of three bfloat16 parts), the accumulators are
-// float32.  z is taken out of the inner sum as z * sum(x), where sum(x) is one more matrix instruction against ones; it
-// enters as the starting value of the group's accumulator.  The scale multiplies the finished group sum in float32, so
+// float32.  z is taken out of the inner sum as z * sum(x), where sum(x) is one more matrix instruction against ones, and
+// added to the group's sum in float32.  The scale multiplies the finished group sum in float32, so
 // the only rounding to fewer bits is the one of y.  An infinite x makes its row NaN (0 * inf and inf - inf both occur).
 //
 // Weight layout: tiles of 16 rows x 128 columns, 1 KB each, along a row of tiles first.  Lane 16 c + i of the wave that
@@ -120,8 +120,11 @@ struct Int4Args {
 // one channel, whose scale and zero point are one register.  Bound by the stream of codes, so a wave asks for kDepth tiles
 // at once, right behind its share of the activations; those are read back from LDS, whose waits do not hold up the stream.
 //
-// One token x 14336 x 4096 (33 MB): 10.7 us, 3.1 TB/s; of that launch 2.0, activations and epilogue 2.1, their sums 0.8, the
-// loop 5.8.  One, three and four tiles at once instead of two: 12.0, 11.3, 11.7 us.
+// The activations' sums are formed along with the products, by every wave for itself: matrix instructions wait for nobody
+// here, and a pass of their own with its barrier took 0.4 to 0.8 us (32 x 4096 x 4096 14.0 -> 12.4 us).
+//
+// One token x 14336 x 4096 (33 MB): 10.6 us, 3.1 TB/s, of which the start takes 4.1 (launch 2.0, activations).  One, three and
+// four tiles at once instead of two: 12.0, 11.3, 11.7 us; two workgroups on a compute unit (64 registers): 17 us, spills.
 constexpr int kLdsWaves = 16;
 constexpr int kLdsThreads = kLdsWaves * kWave;
 
@@ -210,29 +213,7 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
         const int row = 16 * mt + i;  // rows behind the last one repeat it and are not stored
         xrow[mt] = xs + (row < m ? row : m - 1) * row_bytes + 16 * c;
     }
-    // sums of the activations over each fold, times z where it is the same everywhere: [fold][MT][16]
-    f32x4* sums = reinterpret_cast<f32x4*>(xs + P * m * row_bytes);
     const Frag ones = ones_fragment<Frag>();
-    const auto sum_activations = [&] {
-        for (int fold = wave; fold < held * kFolds; fold += kLdsWaves)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                f32x4 part = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < FOLD; ++j)
-#pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + (fold * FOLD + j) * 64), ones, part);
-                if constexpr (!ASYM) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) part[r] *= a.zero_const;
-                }
-                if (i == 0) sums[(fold * MT + mt) * 4 + c] = part;
-            }
-        __syncthreads();
-    };
-    sum_activations();
-
     // CHUNKED: as many turns for every wave, since they meet at barriers
     const int end = CHUNKED ? (tiles + splits - 1) / splits * splits : tiles;
     int left = turns;  // that the activations in LDS serve
@@ -246,7 +227,6 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
                     from = kt - split, left = turns;
                     begin_activations();
                     end_activations();
-                    sum_activations();
                 }
                 --left;
             }
@@ -260,18 +240,18 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
                     const float z = ASYM ? a.zero_const + (float)zero[d][f] : a.zero_const;
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        f32x4 part = sums[((at * kFolds + f) * MT + mt) * 4 + c];
-                        if constexpr (ASYM) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) part[r] *= z;
-                        }
+                        f32x4 sum = {0.f, 0.f, 0.f, 0.f}, part = sum;  // of the activations, and of the products
 #pragma unroll
                         for (int j = 0; j < FOLD; ++j)
 #pragma unroll
-                            for (int p = 0; p < P; ++p)
-                                part = mma(*reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + at * 256 + (f * FOLD + j) * 64), wf[j], part);
+                            for (int p = 0; p < P; ++p) {
+                                const Frag x = *reinterpret_cast<const Frag*>(xrow[mt] + p * m * row_bytes + at * 256 + (f * FOLD + j) * 64);
+                                part = mma(x, wf[j], part);
+                                sum = mma(x, ones, sum);
+                            }
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[mt][r] = __builtin_fmaf(scale[d][f], part[r], acc[mt][r]);
+                        for (int r = 0; r < 4; ++r)
+                            acc[mt][r] = __builtin_fmaf(scale[d][f], __builtin_fmaf(z, sum[r], part[r]), acc[mt][r]);
                     }
                 }
                 if (kt + kDepth * splits < tiles) load(d, kt + kDepth * splits);
@@ -593,20 +573,19 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // How the kernel of few activations shares a call out: waves to a row tile, turns whose activations LDS holds at a time,
 // bytes of LDS.
 struct LdsPlan { int splits, turns, row_bytes; bool chunked; size_t lds; };
-inline LdsPlan plan_lds(const Int4Args& a, int parts, int folds, int mt) {
+inline LdsPlan plan_lds(const Int4Args& a, int parts, int mt) {
     LdsPlan p;
     // as many waves to a row tile as one workgroup on each of the 256 compute units gives
     p.splits = kLdsWaves;
     while (p.splits > 1 && (p.splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / p.splits) > 256)) p.splits /= 2;
-    // 6 tiles at least: 32 activations, three parts, four folds
-    const int64_t fit = (160 * 1024 - a.m * parts * 16) / (a.m * parts * 256 + folds * mt * 64);
+    const int64_t fit = (160 * 1024 - a.m * parts * 16) / (a.m * parts * 256);  // 6 tiles at least: 32 activations, three parts
     while (p.splits > 1 && p.splits > fit) p.splits /= 2;
     const int64_t all = ceil_div(a.tiles, p.splits), most = fit / p.splits;
     p.chunked = a.tiles > fit;
     p.turns = (int)ceil_div(all, ceil_div(all, most));  // even shares
     const int64_t held = p.chunked ? p.turns * p.splits : a.tiles;
     p.row_bytes = (int)(held * 256 + 16);
-    const size_t red = (size_t)kLdsWaves * 1024 * mt, bytes = (size_t)(a.m * parts * p.row_bytes + held * folds * mt * 64);
+    const size_t red = (size_t)kLdsWaves * 1024 * mt, bytes = (size_t)(a.m * parts * p.row_bytes);
     p.lds = bytes > red ? bytes : red;
     return p;
 }
@@ -654,9 +633,9 @@ int launch_linear(Int4Args a, int64_t group, hipStream_t stream) {
         const uint64_t n = group == a.k ? 1ull << 32 : (uint64_t)(group / columns);
         a.fold_inverse = ((1ull << 32) + n - 1) / n;
     };
-    // at 32 activations, against blocks of 32 x 64: 4096 x 4096 13.6 and 16.5 us, 4096 x 14336 41 and 57 us against 32 x 128
+    // at 32 activations, against the smallest blocks below: 4096 x 4096 12.4 and 16.5 us, 4096 x 14336 35 and 38 us
     if (a.m <= 32) {
-        const LdsPlan p = plan_lds(a, Int4Traits<T>::kParts, 4 / FOLD, a.m <= 16 ? 1 : 2);
+        const LdsPlan p = plan_lds(a, Int4Traits<T>::kParts, a.m <= 16 ? 1 : 2);
         folds(32 * FOLD);
         return a.m <= 16 ? launch_lds<T, FOLD, 1>(a, p, stream) : launch_lds<T, FOLD, 2>(a, p, stream);
     }
