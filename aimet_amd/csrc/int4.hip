@@ -127,6 +127,7 @@ struct Int4Args {
 // four tiles at once instead of two: 12.0, 11.3, 11.7 us; two workgroups on a compute unit (64 registers): 17 us, spills.
 constexpr int kLdsWaves = 16;
 constexpr int kLdsThreads = kLdsWaves * kWave;
+constexpr int kFewRows = 32;
 
 template <typename T, int FOLD, int MT, bool ASYM, bool CHUNKED>
 __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a, int splits, int turns, int row_bytes) {
@@ -135,7 +136,10 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
     constexpr int kFolds = 4 / FOLD, kDepth = 2;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int i = lane & 15, c = lane >> 4;
-    const int m = (int)a.m, tiles = (int)a.tiles, groups = (int)a.groups;
+    // 32 activations to a workgroup; more are further workgroups' (blockIdx.y)
+    const int64_t m0 = (int64_t)blockIdx.y * kFewRows;
+    const int m = a.m - m0 < kFewRows ? (int)(a.m - m0) : kFewRows;
+    const int tiles = (int)a.tiles, groups = (int)a.groups;
     const int per_group = kLdsWaves / splits;
     const int split = wave % splits;
     const int64_t tile = (int64_t)blockIdx.x * per_group + wave / splits;
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
     int from = 0;
     const auto fetch = [&](int id) {
         const int row = id / chunks;
-        return load_raw<T>(static_cast<const T*>(a.x) + row * a.ldx, (CHUNKED ? from * kTileCols : 0) + (id - row * chunks) * 8, a.k, a.vec_x);
+        return load_raw<T>(static_cast<const T*>(a.x) + (m0 + row) * a.ldx, (CHUNKED ? from * kTileCols : 0) + (id - row * chunks) * 8, a.k, a.vec_x);
     };
     const auto put = [&](int id, const typename Int4Traits<T>::Raw& raw) {
         const int row = id / chunks;
@@ -276,7 +280,7 @@ __global__ __launch_bounds__(kLdsThreads) void int4_linear_lds_kernel(Int4Args a
             for (int r = 0; r < 4; ++r) v[r] += u[r];
         }
         const float b = a.bias ? load_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
-        T* y = static_cast<T*>(a.y) + row * a.ldy + n;
+        T* y = static_cast<T*>(a.y) + (m0 + row) * a.ldy + n;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (row + r < m) y[r * a.ldy] = store_cast<T>(v[r] + b);
@@ -572,21 +576,24 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How the kernel of few activations shares a call out: waves to a row tile, turns whose activations LDS holds at a time,
 // bytes of LDS.
-struct LdsPlan { int splits, turns, row_bytes; bool chunked; size_t lds; };
+struct LdsPlan { int splits, turns, row_bytes; bool chunked; size_t lds; int64_t blocks, slices; };
 inline LdsPlan plan_lds(const Int4Args& a, int parts, int mt) {
     LdsPlan p;
+    const int64_t m = a.m < kFewRows ? a.m : kFewRows;
+    p.slices = ceil_div(a.m, kFewRows);
     // as many waves to a row tile as one workgroup on each of the 256 compute units gives
     p.splits = kLdsWaves;
     while (p.splits > 1 && (p.splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / p.splits) > 256)) p.splits /= 2;
-    const int64_t fit = (160 * 1024 - a.m * parts * 16) / (a.m * parts * 256);  // 6 tiles at least: 32 activations, three parts
+    const int64_t fit = (160 * 1024 - m * parts * 16) / (m * parts * 256);  // 6 tiles at least: 32 activations, three parts
     while (p.splits > 1 && p.splits > fit) p.splits /= 2;
     const int64_t all = ceil_div(a.tiles, p.splits), most = fit / p.splits;
     p.chunked = a.tiles > fit;
     p.turns = (int)ceil_div(all, ceil_div(all, most));  // even shares
     const int64_t held = p.chunked ? p.turns * p.splits : a.tiles;
     p.row_bytes = (int)(held * 256 + 16);
-    const size_t red = (size_t)kLdsWaves * 1024 * mt, bytes = (size_t)(a.m * parts * p.row_bytes);
+    const size_t red = (size_t)kLdsWaves * 1024 * mt, bytes = (size_t)(m * parts * p.row_bytes);
     p.lds = bytes > red ? bytes : red;
+    p.blocks = ceil_div(a.ntiles, kLdsWaves / p.splits);
     return p;
 }
 
@@ -597,7 +604,7 @@ int launch_lds(const Int4Args& a, const LdsPlan& p, hipStream_t stream) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
         if (e != hipSuccess) return set_error(hipGetErrorString(e)), AHQ_ERR_LAUNCH;
     }
-    kernel<<<(unsigned)ceil_div(a.ntiles, kLdsWaves / p.splits), kLdsThreads, p.lds, stream>>>(a, p.splits, p.turns, p.row_bytes);
+    kernel<<<dim3((unsigned)p.blocks, (unsigned)p.slices), kLdsThreads, p.lds, stream>>>(a, p.splits, p.turns, p.row_bytes);
     return check_launch("ahq_int4_linear");
 }
 template <typename T, int FOLD, int MT>
@@ -633,26 +640,37 @@ int launch_linear(Int4Args a, int64_t group, hipStream_t stream) {
         const uint64_t n = group == a.k ? 1ull << 32 : (uint64_t)(group / columns);
         a.fold_inverse = ((1ull << 32) + n - 1) / n;
     };
-    // at 32 activations, against the smallest blocks below: 4096 x 4096 12.4 and 16.5 us, 4096 x 14336 35 and 38 us
-    if (a.m <= 32) {
-        const LdsPlan p = plan_lds(a, Int4Traits<T>::kParts, a.m <= 16 ? 1 : 2);
+    // Few activations: against the smallest blocks below, 32 x 4096 x 4096 12.4 and 16.5 us, 32 x 4096 x 14336 35 and 38 us.
+    // More, 32 to a workgroup, while all of these run at once: 64 x 2048 x 2048 8.1 us against 11.2, 128 x 1000 x 8192 22 and 25,
+    // 300 x 400 x 14336 37 and 38.  float32, whose three parts take as much more room, up to 16: 16 x 4096 x 4096 15 us against
+    // 17, 12 x 4096 x 14336 31 and 44, but 20 x 4096 x 4096 19 and 18, 32 x 4096 x 4096 33 and 18.
+    const LdsPlan p = plan_lds(a, Int4Traits<T>::kParts, a.m <= 16 ? 1 : 2);
+    if (a.m <= 16) {
         folds(32 * FOLD);
-        return a.m <= 16 ? launch_lds<T, FOLD, 1>(a, p, stream) : launch_lds<T, FOLD, 2>(a, p, stream);
+        return launch_lds<T, FOLD, 1>(a, p, stream);
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (a.m <= kFewRows || p.blocks * p.slices <= 256) {
+            folds(32 * FOLD);
+            return launch_lds<T, FOLD, 2>(a, p, stream);
+        }
     }
     constexpr int kFold = FOLD == 1 ? 1 : 2;
     folds(32 * kFold);
+    const auto one_round = [&](int64_t rows, int64_t channels) { return ceil_div(a.m, rows) * ceil_div(a.n, channels) <= 256; };
     if constexpr (sizeof(T) == 2) {
         // The smallest block whose workgroups still run on the 256 compute units all at once, else the largest: a block's time
         // hardly depends on how many others run, and it grows more slowly than its size.  At 4096 x 4096, in the order 32 x 64,
         // 32 x 128, 64 x 128, 64 x 256: 64 activations 17, 21, 29, 40 us; 256: 31, 23, 30, 41; 512: -, 40, 31, 41;
         // 640: -, 56, 57, 41.
-        const auto one_round = [&](int64_t rows, int64_t channels) { return ceil_div(a.m, rows) * ceil_div(a.n, channels) <= 256; };
         if (one_round(32, 64)) return launch_many<T, kFold, 2, 1>(a, stream);
         if (one_round(32, 128)) return launch_many<T, kFold, 2, 2>(a, stream);
         if (one_round(64, 128)) return launch_many<T, kFold, 4, 2>(a, stream);
         return launch_many<T, kFold, 4, 4>(a, stream);
     } else {
-        return launch_many<T, kFold, 2, 2>(a, stream);  // its three parts fill LDS
+        // in the order 16 x 64, 32 x 128 (three parts fill LDS): 64 x 1000 x 8192 28 and 60 us, 64 x 4096 x 4096 34 in the second
+        if (one_round(16, 64)) return launch_many<T, kFold, 1, 1>(a, stream);
+        return launch_many<T, kFold, 2, 2>(a, stream);
     }
 }
 
