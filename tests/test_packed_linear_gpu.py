@@ -65,6 +65,8 @@ SHAPES = [  # tokens, out, in, group
     # blocks of 32 x 128, 64 x 128 and 64 x 256: whole steps, rows that end inside one, groups of 32
     (257, 2000, 192, 64), (300, 3300, 320, 32), (290, 3400, 130, 130), (1000, 2200, 256, 64), (999, 2201, 320, 32),
     (1000, 2200, 130, 130),
+    # of 32 x 64 and 32 x 128, of 32 to a workgroup
+    (64, 2100, 2048, 64), (63, 2100, 2050, 2050), (128, 4200, 2048, 32), (100, 4200, 2100, 2100), (130, 500, 4096, 128),
 ]
 
 
