@@ -20,9 +20,11 @@
 // that brings its largest value to 2^13 .. 2^14, which keeps 16-bit queries exact (bfloat16 down to 2^-30 of the row's
 // largest value); float32 queries become two parts, 22 bits.  Probabilities carry the scale of their values' block:
 // with x = score + log2(scale), weights are 2^(x - reference), the reference being such that the largest weight so far lies
-// between 2^10 and 2^15 (it is moved, and the sums with it, only when a weight passes 2^15), so float16 holds them to
-// 2^-12 (two parts for float32 queries: 2^-23) and down to 2^-34 of the largest; the softmax's denominator sums
-// weight / scale in float32.  Scales below 2^-80 count as 2^-80 there.
+// between 2^10 and 2^15 (it is moved, and the sums with it, only when a weight passes 2^15).  Weights are two float16 parts
+// for queries of every type: off by at most 2^-22 of themselves, and by 2^-25 where they are small, 2^-35 of the largest.
+// One part (2^-11) would show in 16-bit answers: those of decoding then differ from a float32 softmax's by 4e-4 relative,
+// with two by 3e-5 or not at all, at the same time; prompts pay for it (2048 of 3048 tokens: 147 -> 192 us).  The softmax's
+// denominator sums weight / scale in float32.  Scales below 2^-80 count as 2^-80 there.
 
 #include "../../include/aimet_amd_serving.h"
 #include "ahq_host.h"
@@ -418,7 +420,7 @@ __device__ __forceinline__ void split_f16(const float* v, f16x8* out) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             out[p][e] = (_Float16)rest[e];
-            if (p + 1 < N) rest[e] -= (float)out[p][e];
+            if (p + 1 < N) rest[e] = __builtin_fmaf((float)out[p][e], -1.0f, rest[e]);
         }
 }
 
@@ -439,6 +441,7 @@ template <typename T, int D, int NR>
 struct AttendRows {
     static constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
     static constexpr int kSteps = D / 32, kOut = D / 16;
+    static constexpr int kWeightParts = 2;  // of the probabilities, for every type
     f16x8 q[kSteps][NR][kParts];
     f32x4 o[kOut][NR];
     float rescale[NR];  // what the row's power of two is undone with, times the scale of the scores
@@ -543,7 +546,7 @@ struct AttendRows {
 #pragma unroll
             for (int u = 0; u < 2; ++u) vf[u][0] = value(u, 0), vf[u][1] = value(u, 1);
         }
-        f16x8 pf[2][NR][kParts];
+        f16x8 pf[2][NR][kWeightParts];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const float factor = k_scale * rescale[n], shift = v_log - reference[n];
@@ -591,7 +594,7 @@ struct AttendRows {
                     p[e] = __builtin_amdgcn_exp2f(x[2 * w + e / 4][n][e % 4]);
                     total += p[e];
                 }
-                split_f16<kParts>(p, pf[w][n]);
+                split_f16<kWeightParts>(p, pf[w][n]);
             }
             sum[n] = __builtin_fmaf(total, inverse, sum[n]);
         }
@@ -606,7 +609,7 @@ struct AttendRows {
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) {
+                for (int p = 0; p < kWeightParts; ++p) {
                     o[u][n] = mma(vf[u % 3][0], pf[0][n][p], o[u][n]);
                     o[u][n] = mma(vf[u % 3][1], pf[1][n][p], o[u][n]);
                 }
@@ -758,7 +761,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
 // Many rows (prompts): each wave has 16 * NR rows of its own, and the workgroup takes the token tiles one after the other
 // through two LDS buffers, turned into float16 once for all its waves; the next tile is on its way to registers while this
 // one is worked on.  Bound by the matrix cores and the vector work between the two products together.  2048 queries of
-// 3048 tokens, 2 x 8 x 4 heads of 128: 144 us, 940 TFLOP/s.
+// 3048 tokens, 2 x 8 x 4 heads of 128: 192 us, 708 TFLOP/s (of products in two parts: 1060).
 template <typename T, int D, int NR, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArgs a) {
     constexpr int kThreads = WAVES * kWave;

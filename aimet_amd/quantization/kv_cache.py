@@ -159,7 +159,11 @@ class QuantizedKVCache:
         tokens and its queries are the last ``queries`` of them (of a padded batch: its first ``counts`` queries are the
         last ``counts`` tokens): query t sees the tokens up to its own position, ``lengths - counts + t``.  Queries that
         see nothing, and those behind ``counts``, are answered with 0.  ``scale`` multiplies the scores (default
-        1 / sqrt(head_dim)).  The result has the queries' type, shape and, where they are dense, memory layout."""
+        1 / sqrt(head_dim)).  The result has the queries' type, shape and, where they are dense, memory layout.
+
+        16-bit queries are used as they are and float32 queries to 22 bits of a row's largest value; probabilities have
+        22 bits and are off by at most 2^-35 of the row's largest one where they are small (both weighted by the scale of
+        their values' block); all sums are float32, and the result is rounded once."""
         self._check(q, "q")
         heads, queries = q.shape[1], q.shape[2]
         if heads == 0 or heads % self.kv_heads:

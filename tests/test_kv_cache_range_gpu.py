@@ -1,0 +1,60 @@
+"""The 8-bit cache and its attention where ranges and roundings end: probabilities that cancel, queries and maxima at the
+ends of their types' ranges."""
+
+import math
+
+import pytest
+import torch
+
+from aimet_amd.quantization.kv_cache import QuantizedKVCache
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+names = lambda d: str(d).split(".")[-1]  # noqa: E731
+
+# (batch, heads, queries, length): few rows; many rows, four waves to a workgroup; eight
+FORMS = [(4, 2, 1, 64), (4, 2, 3, 704), (8, 16, 40, 192), (8, 16, 50, 768)]
+
+
+def _stored(cache):
+    """Keys and values [B, H, C, D] in 64 bits, from what the cache holds."""
+    return tuple(c.cpu().double() * (a.cpu().double() / 127).repeat_interleave(cache.block_tokens, 2)[..., None]
+                 for c, a in zip(cache.codes(), (cache.k_amax, cache.v_amax)))
+
+
+def _attention(cache, q, length, scale):
+    """(answer, sum of probability times magnitude, largest sum of |q k| of a row) in 64 bits; one query head a head."""
+    k, v = (x[:, :, :length] for x in _stored(cache))
+    qd = q.cpu().double()
+    t = q.shape[2]
+    hidden = torch.arange(length)[None] > (length - t + torch.arange(t))[:, None]
+    p = torch.softmax((qd @ k.transpose(2, 3) * scale).masked_fill(hidden, -math.inf), 3)
+    return p @ v, p @ v.abs(), (qd.abs() @ k.abs().transpose(2, 3)).amax(3, keepdim=True) * abs(scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("batch,heads,queries,length", FORMS)
+def test_probabilities_that_cancel(device, batch, heads, queries, length, dtype):
+    """Tokens in pairs, their keys one code apart and their values opposite: the answer is what is left of probabilities
+    that cancel, a few hundredths of what they add up to, so that it is the probabilities' roundings that show and not
+    the answer's own.
+
+    In relation to the sum of magnitudes: a probability's error is 2^-19 for the exponential and the logarithm of the
+    block's scale, 2^-22 for its two float16 parts, and the error of its score, of which five roundings of 2^-24 count as
+    a random walk.  (One float16 part is 2^-11 a token at most and 2^-12 / sqrt(3) of the mean square, over some ten
+    tokens a row: 2^-14 or 2^-15.)"""
+    g = torch.Generator().manual_seed(length)
+    d = 64
+    k = torch.randn(batch, heads, length // 2, 1, d, generator=g).expand(-1, -1, -1, 2, -1).clone() * 3
+    k[..., 1, 0] += k.abs().amax() / 100
+    v = torch.randn(batch, heads, length // 2, 1, d, generator=g) * torch.tensor([1.0, -1.0])[:, None]
+    cache = QuantizedKVCache(batch, heads, length, d, 64, device)
+    cache.append(*(x.reshape(batch, heads, length, d).to(device) for x in (k, v)), 0)
+    q = torch.randn(batch, heads, queries, d, generator=g).to(dtype)
+    out = cache.attend(q.to(device), length).cpu().double()
+    want, size, most = _attention(cache, q, length, 1 / math.sqrt(d))
+    even = (length - queries + torch.arange(queries)) % 2 == 1  # rows that see whole pairs
+    out, want, size = (x[:, :, even] for x in (out, want, size))
+    assert want.norm() <= 0.05 * size.norm()
+    eps = torch.finfo(dtype).eps / 2
+    assert (out - want).norm() <= eps * want.norm() + (2.0 ** -19 + 2.0 ** -22 + 5 * 2.0 ** -24 * most.amax()) * size.norm()
