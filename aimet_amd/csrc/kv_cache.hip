@@ -328,12 +328,22 @@ __global__ __launch_bounds__(kBlock) void kv_values_kernel(KvValuesArgs a) {
             store_pack<T, kPer>(out + (int64_t)t * D + d + u * kPer, w);
         }
     };
-    // (byte - 128) * scale with one rounding
-    const auto scaled = [](uint32_t w, int byte, float s) { return __builtin_fmaf((float)(w >> (8 * byte) & 0xffu), s, -128.0f * s); };
+    // The code is exact, so its product with the scale is rounded once.  float16: as (byte - 128) * scale in one instruction
+    // with the rounding to float16; larger scales than 2^100 make infinities of all codes but 0 either way.  float32: the
+    // scale of the largest number is rounded up, and 127 times that would be infinite.
+    const auto scaled = [](uint32_t w, int byte, float s) {
+        if constexpr (sizeof(T) == 4)
+            return __builtin_amdgcn_fmed3f((float)(int8_t)((w ^ 0x80808080u) >> (8 * byte)) * s, -3.402823466e38f, 3.402823466e38f);
+        else if constexpr (std::is_same_v<T, f16_t>)
+            return __builtin_fmaf((float)(w >> (8 * byte) & 0xffu), s, -128.0f * s);
+        else
+            return (float)(int8_t)((w ^ 0x80808080u) >> (8 * byte)) * s;
+    };
     for (int id = threadIdx.x; id < 16 * (D / 8); id += kBlock) {
         const int quad = id / (D / 8), d = id % (D / 8) * 8;
         if (p0 + 4 * quad >= a.length) break;
-        const float s = amax[(p0 + 4 * quad) >> a.block_shift] / 127.0f;
+        float s = amax[(p0 + 4 * quad) >> a.block_shift] / 127.0f;
+        if constexpr (std::is_same_v<T, f16_t>) s = fminf(s, 0x1p100f);
         u32x4_t w[2];
         if (which) {
             w[0] = *reinterpret_cast<const u32x4_t*>(quads + quad * kPitch + d);

@@ -58,3 +58,32 @@ def test_probabilities_that_cancel(device, batch, heads, queries, length, dtype)
     assert want.norm() <= 0.05 * size.norm()
     eps = torch.finfo(dtype).eps / 2
     assert (out - want).norm() <= eps * want.norm() + (2.0 ** -19 + 2.0 ** -22 + 5 * 2.0 ** -24 * most.amax()) * size.norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+def test_read_back_at_the_top_of_the_range(device, dtype):
+    """Blocks whose maximum is the largest number of their type, zeros and negative values beside it: a quotient and a
+    product in float32, and one rounding to the type asked for."""
+    top = torch.finfo(dtype).max
+    g = torch.Generator().manual_seed(0)
+    x = (torch.rand(1, 2, 64, 64, generator=g, dtype=torch.float64) * 2 - 1) * top
+    x[:, :, ::16, :3] = torch.tensor([top, -top, 0.0], dtype=torch.float64)
+    x = x.to(dtype)
+    cache = QuantizedKVCache(1, 2, 64, 64, 16, device)
+    cache.append(x.to(device), x.neg().flip(3).to(device), 0)
+    assert bool((cache.k_amax == top).all()) and bool((cache.v_amax == top).all())
+    for out_dtype in {torch.float32, dtype}:
+        eps = torch.finfo(out_dtype).eps / 2
+        for got, want in zip(cache.dequantize(dtype=out_dtype), _stored(cache)):
+            got = got.cpu().double()
+            assert bool(got.isfinite().all()) and bool((got[:, :, ::16].abs().amax(3) == top).all())
+            assert bool(((got - want).abs() <= (eps + 2.0 ** -23) * want.abs()).all())
+
+
+def test_read_back_into_float16_from_beyond_its_range(device):
+    x = torch.zeros(1, 1, 64, 64)
+    x[0, 0, ::16, :3] = torch.tensor([3e38, -3e38, 0.0])
+    cache = QuantizedKVCache(1, 1, 64, 64, 16, device)
+    cache.append(x.to(device), x.to(device), 0)
+    for got in cache.dequantize(dtype=torch.float16):
+        assert torch.equal(got.cpu(), x.half())
