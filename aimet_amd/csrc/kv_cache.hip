@@ -24,7 +24,9 @@
 // for queries of every type: off by at most 2^-22 of themselves, and by 2^-25 where they are small, 2^-35 of the largest.
 // One part (2^-11) would show in 16-bit answers: those of decoding then differ from a float32 softmax's by 4e-4 relative,
 // with two by 3e-5 or not at all, at the same time; prompts pay for it (2048 of 3048 tokens: 147 -> 192 us).  The softmax's
-// denominator sums weight / scale in float32.  Scales below 2^-80 count as 2^-80 there.
+// denominator sums weight / scale in float32.  Scales are counted in a unit of the workgroup's share, a power of two: 1 where
+// the largest maximum in it is between 2^-5 and 2^16, and otherwise that maximum's, so that values of any size have the same
+// precision.  Scales below 2^-84 of the unit count as that, which is what blocks of zeros weigh their tokens with.
 
 #include "../../include/aimet_amd_serving.h"
 #include "ahq_host.h"
@@ -402,6 +404,18 @@ __device__ __forceinline__ int seen_tiles(const KvAttendArgs& a, const SequenceV
     const int seen = seq.length - seq.count + t + 1;
     return t < 0 || seen <= 0 ? 0 : (seen + kKvTile - 1) / kKvTile;
 }
+// Largest of the lane's part of the blocks' maxima that a share's rows up to `row` see: those of its tiles [first, stop).
+// Blocks behind the last token hold the scales of other ones.
+__device__ __forceinline__ float seen_amax(const KvAttendArgs& a, const SequenceView& seq, const float* amax, int row, int first, int stop) {
+    int t = row / a.groups;
+    if (t >= seq.count) t = seq.count - 1;
+    const int tokens = seq.length - seq.count + t + 1, until = stop * kKvTile < tokens ? stop * kKvTile : tokens;
+    const int last = until > 0 ? (until - 1) >> a.block_shift : 0;
+    int at = (first * kKvTile >> a.block_shift) + (int)(threadIdx.x & (kWave - 1));
+    float most = amax[at < last ? at : last];  // not a masked load: short shares have no more than this one
+    for (at += kWave; at <= last; at += kWave) most = fmaxf(most, amax[at]);
+    return most;
+}
 // Splits of the token axis that hold such tiles, for the workgroup's rows that `row` is one of.
 __device__ __forceinline__ int used_splits(const KvAttendArgs& a, const SequenceView& seq, int row) {
     return (seen_tiles(a, seq, row / a.row_tile * a.row_tile + a.row_tile - 1) + a.split_tiles - 1) / a.split_tiles;
@@ -442,8 +456,15 @@ __device__ __forceinline__ float row_max(float v) {
     return fmaxf(bits_to_f32(b[0]), bits_to_f32(b[1]));
 }
 
+// An answer is an average of finite values: it is no larger than they are, whatever its roundings.  NaN stays.
+__device__ __forceinline__ float finite(float v) {
+    return v > 3.402823466e38f ? 3.402823466e38f : v < -3.402823466e38f ? -3.402823466e38f : v;
+}
+
 constexpr float kTop = 15.0f, kStart = 10.0f;  // log2 of the largest weight: at most, and where the reference is set to
-constexpr float kLeastScale = 0x1p-80f;
+constexpr float kLeastScale = 0x1p-84f;  // in units
+constexpr float kOrdinary = 0x1p-5f, kLarge = 0x1p16f;  // maxima that are counted in the unit 1
+constexpr int kLeastUnit = -126, kLargestUnit = 118;    // 2^-unit / 127 is a normal number
 constexpr int kAttendWaves = 4;
 
 // What a wave knows of its 16 * NR rows; a lane holds row 16 n + i of them and the channels 16 u + 4 c + r of its answer.
@@ -458,6 +479,8 @@ struct AttendRows {
     float reference[NR], top[NR], sum[NR];
     int last[NR];       // the last token the row sees; below 0: none
     int least;          // of the wave's rows that see anything, the least `last`
+    int unit;           // scales of values are counted in 2^unit
+    float to_unit;      // 2^-unit / 127
 
     __device__ __forceinline__ void begin(const KvAttendArgs& a, const SequenceView& seq, int b, int h, int row0, int i, int c) {
         least = 0x7fffffff;
@@ -519,6 +542,16 @@ struct AttendRows {
         }
         least = __builtin_amdgcn_readfirstlane(least);
     }
+    // The unit, from the largest of the lanes' maxima; a share of zeros has any.
+    __device__ __forceinline__ void set_unit(float most) {
+        unit = 0;
+        if (__builtin_expect(__any(most >= kLarge) || !__any(most >= kOrdinary), 0)) {
+            most = wave_reduce(most, OpMaxF());
+            const int e = __builtin_amdgcn_readfirstlane((int)(f32_to_bits(most) >> 23) - 127);
+            unit = e < kLeastUnit ? kLeastUnit : e > kLargestUnit ? kLargestUnit : e;
+        }
+        to_unit = bits_to_f32((uint32_t)(127 - unit) << 23) * (1.0f / 127.0f);
+    }
 
     // One tile of 64 tokens from p0 on: `key(s, u)` and `value(u, w)` give operands, `between` is called once the keys and
     // scales are no longer needed.  AHEAD: operands come from LDS and are asked for one group of products early, in an
@@ -526,7 +559,7 @@ struct AttendRows {
     template <bool AHEAD, typename Key, typename Value, typename Between>
     __device__ __forceinline__ void work(Key key, Value value, float k_amax, float v_amax, int p0, int c, Between between) {
         const float k_scale = k_amax * (1.0f / 127.0f);
-        const float v_scale = fmaxf(v_amax * (1.0f / 127.0f), kLeastScale);
+        const float v_scale = fmaxf(v_amax * to_unit, kLeastScale);
         const float v_log = __builtin_amdgcn_logf(v_scale);
         const float v_inverse = __builtin_amdgcn_rcpf(v_scale);
         f32x4 x[4][NR];
@@ -643,7 +676,7 @@ __device__ __forceinline__ void store_rows(const KvAttendArgs& a, const AttendRo
             for (int u = 0; u < D / 16; ++u) {
                 Pack<T, 4> out;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) out.v[r] = store_cast<T>(sum[n] == 0.0f ? 0.0f : rows.o[u][n][r] * inverse);
+                for (int r = 0; r < 4; ++r) out.v[r] = store_cast<T>(sum[n] == 0.0f ? 0.0f : finite(rows.o[u][n][r] * inverse));
                 if (a.vec_out) {
                     store_pack<T, 4>(to + 16 * u, out);
                 } else {
@@ -660,7 +693,9 @@ __device__ __forceinline__ void store_rows(const KvAttendArgs& a, const AttendRo
     }
 }
 
-// Sums over the lanes of a row; rows that saw nothing have the reference -infinity and the sum 0.
+// Sums over the lanes of a row, in the unit 1; rows that saw nothing have the reference -infinity and the sum 0.  Far units
+// are shared out between a row's answer and its sum, so that neither leaves float32; where blocks of zeros have the row's
+// weight, the sum is large, and its answer takes the rest.
 template <typename T, int D, int NR>
 __device__ __forceinline__ void finish_rows(AttendRows<T, D, NR>& rows, float* sum) {
 #pragma unroll
@@ -668,6 +703,19 @@ __device__ __forceinline__ void finish_rows(AttendRows<T, D, NR>& rows, float* s
         sum[n] = rows.sum[n];
         sum[n] += __shfl_xor(sum[n], 16, kWave);
         sum[n] += __shfl_xor(sum[n], 32, kWave);
+        if (__builtin_expect(rows.unit != 0, 0)) {
+            int share = rows.unit >= -24 && rows.unit <= 24 ? 0 : rows.unit / 2;
+            const int most = 227 + rows.unit - (int)(f32_to_bits(sum[n]) >> 23);  // leaves the sum at 2^101
+            if (most < share) share = most;
+            if (__any(share != 0)) {
+#pragma unroll
+                for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) rows.o[u][n][r] = __builtin_amdgcn_ldexpf(rows.o[u][n][r], share);
+            }
+            rows.reference[n] += (float)(rows.unit - share);
+            sum[n] = __builtin_amdgcn_ldexpf(sum[n], share - rows.unit);
+        }
         if (rows.last[n] < 0) sum[n] = 0.0f;
         if (rows.top[n] != kTop) rows.reference[n] = -__builtin_inff();
     }
@@ -717,9 +765,11 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
 #pragma unroll
             for (int u = 0; u < D / 64; ++u) kw[s][u] = piece(from, s * (D / 64) + u);
     };
+    const float most = seen_amax(a, seq, v_amax, row0 + 15, split * a.split_tiles, stop);
     if (first < stop) load(first);
     AttendRows<T, D, 1> rows;
     rows.begin(a, seq, b, h, row0, i, c);
+    rows.set_unit(most);
     for (int tile = first; tile < stop; tile += kAttendWaves) {
         u32x4_t vw[kOut];
         const uint8_t* from = values + (int64_t)tile * (kKvTile * D);
@@ -759,7 +809,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
         }
         if (used <= 1) {
             T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot;
-            to[d] = store_cast<T>(total == 0.0f ? 0.0f : value / total);
+            to[d] = store_cast<T>(total == 0.0f ? 0.0f : finite(value / total));
         } else {
             const int64_t at = (bh * a.rows + row) * a.splits + split;
             a.part[at * D + d] = value;
@@ -815,9 +865,11 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArg
             coming[n] = at < kPieces ? keys[(int64_t)tile * kPieces + at] : values[(int64_t)tile * kPieces + at - kPieces];
         }
     };
+    const float most = seen_amax(a, seq, v_amax, wg_row + a.row_tile - 1, first, stop);
     if (first < stop) load(first);
     AttendRows<T, D, NR> rows;
     rows.begin(a, seq, b, h, row0, i, c);
+    rows.set_unit(most);
     for (int tile = first; tile < stop; ++tile) {
         f16x8* buffer = buffers + (tile & 1) * 4 * kPieces;
         const float k_now = k_next, v_now = v_next;
@@ -890,7 +942,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttendArgs a) {
         for (int r = 0; r < 4; ++r) value[r] += sums[j][lane][r];
     T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * lane;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) to[r] = store_cast<T>(total == 0.0f ? 0.0f : value[r] / total);
+    for (int r = 0; r < 4; ++r) to[r] = store_cast<T>(total == 0.0f ? 0.0f : finite(value[r] / total));
 }
 
 // The same for up to eight splits, where rows are many: D / 4 lanes to a row (1024 queries of 1 x 8 x 4 heads in two
@@ -923,7 +975,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_rows_kernel(KvAttendArgs
     T* to = static_cast<T*>(a.out) + b * a.ob + (int64_t)(h * a.groups + row % a.groups) * a.oh + (int64_t)(row / a.groups) * a.ot + 4 * lane;
     Pack<T, 4> out;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) out.v[r] = store_cast<T>(total == 0.0f ? 0.0f : value[r] / total);
+    for (int r = 0; r < 4; ++r) out.v[r] = store_cast<T>(total == 0.0f ? 0.0f : finite(value[r] / total));
     if (a.vec_out) {
         store_pack<T, 4>(to, out);
     } else {

@@ -87,3 +87,92 @@ def test_read_back_into_float16_from_beyond_its_range(device):
     cache.append(x.to(device), x.to(device), 0)
     for got in cache.dequantize(dtype=torch.float16):
         assert torch.equal(got.cpu(), x.half())
+
+
+def _fill_blocks(shape, sizes, seed):
+    """Values [B, H, T, D] whose blocks of 16 tokens are of the given sizes, in turn."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g, dtype=torch.float64).clamp(-4, 4) / 4
+    size = torch.tensor(sizes, dtype=torch.float64).repeat(shape[2] // 16 // len(sizes) + 1)[:shape[2] // 16]
+    return x * size.repeat_interleave(16)[:, None]
+
+
+def _check_sizes(cache, q, length):
+    """Every answer against the formula, as accurate for values of any size: the roundings of scores (d products a float32
+    sum in instructions of 32, five more) and of probabilities as in the other tests, 2^-25 of a weight that is at least 2^10 at
+    the largest for every token, and 2^-72 of the largest value for blocks that are smaller than that."""
+    d = q.shape[3]
+    out = cache.attend(q, length).cpu().double()
+    want, size, most = _attention(cache, q, length, 1 / math.sqrt(d))
+    eps, parts = torch.finfo(q.dtype).eps / 2, 2 if q.dtype == torch.float32 else 1
+    scale = (cache.v_amax.cpu().double() / 127).repeat_interleave(cache.block_tokens, 2)[:, :, None, :length]
+    t = q.shape[2]
+    hidden = torch.arange(length)[None] > (length - t + torch.arange(t))[:, None]
+    s = (q.cpu().double() @ _stored(cache)[0][:, :, :length].transpose(2, 3) / math.sqrt(d)).masked_fill(hidden, -math.inf)
+    heavy = (torch.softmax(s, 3) * scale).amax(3, keepdim=True)
+    bound = eps * want.abs() + length * 2.0 ** -35 * 127 * heavy + 2.0 ** -72 * 127 * scale.amax()
+    bound += (2 * (33 * parts * d / 32 + 5) * 2.0 ** -23 * most + 2.0 ** -19 + 2.0 ** -21 + (66 + cache.capacity / 32) * 2.0 ** -22) * size
+    bound += torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+    err = (out - want).abs()
+    assert bool(out.isfinite().all())
+    assert bool((err <= bound).all()), (err / bound).max().item()
+    return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=names)
+@pytest.mark.parametrize("batch,heads,queries,length", FORMS + [(1, 1, 1, 2560)])
+@pytest.mark.parametrize("sizes", [
+    (1e-24,), (1e-30, 4e-31, 0.0), (1e-37, 3e-38), (0.0, 0.0, 0.0, 0.0, 1e-33), (1e-33, 0.0, 0.0, 0.0, 0.0), (2e-38, 1e-24, 1e-10, 3e4),
+    (3e38, 1e-20, 1.0), (3e4, 1e-10, 1e-24, 2e-38), (3.3e38,), (0.0,)], ids=lambda s: "-".join(map(str, s)))
+def test_values_of_any_size(device, batch, heads, queries, length, dtype, sizes):
+    cache = QuantizedKVCache(batch, heads, length, 64, 16, device)
+    k = torch.randn(batch, heads, length, 64, generator=torch.Generator().manual_seed(1))
+    v = _fill_blocks((batch, heads, length, 64), sizes, 2)
+    cache.append(k.to(device), v.float().to(device), 0)
+    q = torch.randn(batch, heads, queries, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    out = _check_sizes(cache, q.to(device), length)
+    assert bool(out.any()) == any(sizes[:length // 16])
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=names)
+@pytest.mark.parametrize("batch,heads,queries,length", FORMS)
+@pytest.mark.parametrize("dim", [128, 256])
+def test_values_of_any_size_in_wider_heads(device, dim, batch, heads, queries, length, dtype):
+    cache = QuantizedKVCache(batch, heads, length, dim, 16, device)
+    k = torch.randn(batch, heads, length, dim, generator=torch.Generator().manual_seed(1))
+    v = _fill_blocks((batch, heads, length, dim), (1e-30, 1e-33, 0.0, 2e-38), 2)
+    cache.append(k.to(device), v.float().to(device), 0)
+    q = torch.randn(batch, heads, queries, dim, generator=torch.Generator().manual_seed(3)).to(dtype)
+    _check_sizes(cache, q.to(device), length)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=names)
+@pytest.mark.parametrize("batch,heads,queries,length", FORMS)
+def test_weight_on_blocks_of_zeros(device, batch, heads, queries, length, dtype):
+    """Blocks of zeros that have nearly all of the weight, in front of and behind tiny and huge ones: answers go to zero, and
+    neither infinities nor NaN come of it."""
+    for sizes in ((1e-30, 0.0, 1e30, 0.0), (0.0, 1e-36), (1e30, 0.0, 1e-30, 1e-4)):
+        cache = QuantizedKVCache(batch, heads, length, 64, 16, device)
+        k = torch.randn(batch, heads, length, 64, generator=torch.Generator().manual_seed(1))
+        v = _fill_blocks((batch, heads, length, 64), sizes, 2)
+        k[..., 0] += 30 * (v.abs().amax(3) == 0)
+        cache.append(k.to(device), v.float().to(device), 0)
+        q = torch.randn(batch, heads, queries, 64, generator=torch.Generator().manual_seed(3))
+        q[..., 0] = 8
+        _check_sizes(cache, q.to(dtype).to(device), length)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=names)
+@pytest.mark.parametrize("queries", [1, 60])
+def test_scales_of_discarded_tokens(device, queries, dtype):
+    """Small values over a longer sequence of huge ones that were discarded: their blocks' scales play no part."""
+    batch, heads, length = (2, 2, 70) if queries == 1 else (8, 16, 70)
+    q = torch.randn(batch, heads, queries, 64, generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    k, v = (torch.randn(batch, heads, 192, 64, generator=torch.Generator().manual_seed(s)).to(device) for s in (1, 2))
+    outs = []
+    for discarded in (1.0, 1e30):
+        cache = QuantizedKVCache(batch, heads, 192, 64, 16, device)
+        cache.append(k, v * discarded, 0)
+        cache.append(k[:, :, :length], v[:, :, :length] * 1e-20, 0)
+        outs.append(_check_sizes(cache, q, length))
+    assert torch.equal(*outs)
