@@ -131,14 +131,15 @@ class PackedWeight:
     @classmethod
     def from_encoding(cls, weight: torch.Tensor, encoding) -> "PackedWeight":
         """The packed form of a weight under an affine encoding (per tensor, per channel or blockwise, grouped block
-        scales included) of at most 16 levels: the codes are those of ``encoding.quantize``."""
+        scales included) of at most 16 levels: the codes are those of ``encoding.quantize``, and on a shifted grid those
+        of the values of ``encoding.quantize_dequantize``."""
         if weight.dim() != 2:
             raise RuntimeError(f"a weight of two dimensions is expected; got shape {tuple(weight.shape)}")
         if encoding.qmax - encoding.qmin > 15:
             raise RuntimeError(f"the grid [{encoding.qmin}, {encoding.qmax}] has more than 16 levels")
         n, k = weight.shape
         with torch.no_grad():
-            codes = encoding.quantize(weight.detach().as_subclass(torch.Tensor)).as_subclass(torch.Tensor)
+            weight = weight.detach().as_subclass(torch.Tensor)
 
             def spread(t):
                 t = t.detach().as_subclass(torch.Tensor).float()
@@ -153,7 +154,17 @@ class PackedWeight:
                 concretize_block_size((n, k), tuple(encoding.scale.shape), encoding.block_size)  # its own errors
             if scale.shape[1] not in (1, k) and encoding.block_size is None:
                 raise RuntimeError(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
-            return cls.pack(codes, scale, offset, encoding.qmin, encoding.zero_point_shift or 0.0)
+            shift = encoding.zero_point_shift or 0.0
+            if shift == 0.0:
+                codes = encoding.quantize(weight).as_subclass(torch.Tensor)
+            else:
+                # quantize() knows no shift: what lies on the shifted grid lies half-way between its codes
+                if scale.shape[0] != n or k % scale.shape[1]:
+                    raise RuntimeError(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
+                on_grid = encoding.quantize_dequantize(weight).as_subclass(torch.Tensor).float()
+                levels = on_grid.view(n, scale.shape[1], -1) / scale[..., None] - offset[..., None] - shift
+                codes = levels.round().clamp(encoding.qmin, encoding.qmax).view(n, k)
+            return cls.pack(codes, scale, offset, encoding.qmin, shift)
 
 
 def packed_linear(x: torch.Tensor, weight: PackedWeight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

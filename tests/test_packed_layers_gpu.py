@@ -1,0 +1,51 @@
+"""Packed layers made from quantizers of every kind, and what stands around them in a model: shifted grids, layers that have
+no packed form, quantizers and hooks, autocast, captured calls."""
+
+import pytest
+import torch
+
+from aimet_amd import nn as qnn
+from aimet_amd.quantization.affine import PackedWeight, QuantizeDequantize, packed_linear
+
+pytestmark = pytest.mark.gpu
+names = lambda d: str(d).split(".")[-1]  # noqa: E731
+plain = lambda t: t.as_subclass(torch.Tensor)  # noqa: E731
+
+SHIFTED = {
+    "tensor": ((), None), "channel": ((96, 1), None), "block": ((96, 4), (1, 64)), "rows": ((12, 2), (8, 128)),
+}
+
+
+def _layer(wq, device, dtype=torch.float32, in_f=256, out_f=96, bias=True):
+    torch.manual_seed(0)
+    q = qnn.QuantizedLinear(in_f, out_f, bias=bias).to(device=device, dtype=dtype)
+    q.param_quantizers["weight"] = None if wq is None else wq.to(device)
+    q.input_quantizers[0] = QuantizeDequantize((), 16, symmetric=False).to(device)
+    q.output_quantizers[0] = QuantizeDequantize((), 16, symmetric=False).to(device)
+    x = torch.randn(9, in_f, device=device, dtype=dtype)
+    with torch.no_grad(), qnn.compute_encodings(q):
+        q(x)
+    return q, x
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=names)
+@pytest.mark.parametrize("kind", list(SHIFTED))
+def test_shifted_grids(device, kind, dtype):
+    """Grids of half steps: the packed values are the quantizer's, up to a rounding of the scale and of the product to the
+    weight's type; a code next to the right one would be off by a fifteenth of the largest value at least."""
+    shape, block = SHIFTED[kind]
+    q, x = _layer(QuantizeDequantize(shape, 4, symmetric=True, block_size=block, zero_point_shift=0.5), device, dtype)
+    wq = q.param_quantizers["weight"]
+    eye = torch.eye(256, device=device)
+    with torch.no_grad():
+        dense = plain(wq(q.weight)).float()
+        for weight in (q.pack().weight, PackedWeight.from_encoding(q.weight, wq.get_encodings()),
+                       PackedWeight.from_encoding(wq(q.weight).dequantize(), wq.get_encodings())):
+            read = packed_linear(eye, weight).T
+            assert bool(((read - dense).abs() <= 1.01 * torch.finfo(dtype).eps * read.abs()).all())
+        # all the roundings of the layer: the weight's, products of 256 terms in float32, the output's and one of its steps
+        eps, xin = torch.finfo(dtype).eps, plain(q.input_quantizers[0](x)).double()
+        total = xin.abs() @ dense.double().abs().T + q.bias.double().abs()
+        step = q.output_quantizers[0].get_encodings().scale.double()
+        got, want = (plain(layer(x)).double() for layer in (q.pack(), q))
+        assert bool(((got - want).abs() <= (1.01 * eps + 512 * 2.0 ** -23) * total + eps * want.abs() + step).all())
