@@ -90,10 +90,14 @@ class PackedWeight:
             raise RuntimeError(f"qmin must be in [-128, 112]; got {qmin}")
         # everything that has to be known of the values is read back at once
         known = [t.double() for t in torch.aminmax(codes)]
+        if codes.is_floating_point():
+            known.append((codes == codes.round()).all().double())
         if offset is not None:
             off = offset.detach().float()
             known += [t.double() for t in (*torch.aminmax(off), (off == off.round()).all())]
         lo, hi, *about_offset = torch.stack(known).tolist()
+        if codes.is_floating_point() and not about_offset.pop(0):
+            raise RuntimeError("codes must be whole numbers")
         if not qmin <= lo <= hi <= qmin + 15:
             raise RuntimeError(f"codes in [{lo:g}, {hi:g}] do not fit the 16 levels from {qmin} on")
         npad = -(-n // 16) * 16

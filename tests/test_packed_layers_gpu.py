@@ -49,3 +49,17 @@ def test_shifted_grids(device, kind, dtype):
         step = q.output_quantizers[0].get_encodings().scale.double()
         got, want = (plain(layer(x)).double() for layer in (q.pack(), q))
         assert bool(((got - want).abs() <= (1.01 * eps + 512 * 2.0 ** -23) * total + eps * want.abs() + step).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=names)
+def test_codes_that_are_not_whole_are_refused(device, dtype):
+    codes = torch.randint(-8, 8, (32, 64), generator=torch.Generator().manual_seed(0)).to(dtype).to(device)
+    scale, offset = torch.full((32, 2), 0.25, device=device), torch.arange(64.0, device=device).view(32, 2)
+    for args in ((scale,), (scale, offset, -8)):
+        whole = PackedWeight.pack(codes, *args)
+        assert torch.equal(whole.codes, PackedWeight.pack(codes.to(torch.int8), *args).codes)
+        for place, value in (((5, 3), 0.5), ((0, 0), -7.75), ((31, 63), float("nan"))):
+            bad = codes.clone()
+            bad[place] = value
+            with pytest.raises(RuntimeError):
+                PackedWeight.pack(bad, *args)
