@@ -8,7 +8,8 @@ output channel and group of columns.  ``packed_linear`` is ``torch.nn.functional
 
 Products are exact and sums are float32; the result is rounded once, to the activations' type.  (Quantize-dequantizing a
 bfloat16 weight rounds code * scale to bfloat16; here the scale stays float32, so the two agree to that rounding.)
-There is no backward pass: the weight is frozen and the calls are those of inference.
+There is no backward pass and no forward-mode derivative: the weight is frozen and the calls are those of inference;
+tensors that require gradients or carry tangents are refused.
 """
 
 from __future__ import annotations
@@ -17,6 +18,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from aimet_amd import _lib
 from aimet_amd.quantization._utils import concretize_block_size
@@ -28,6 +30,10 @@ def _refuse_gradients(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on tensors that do not "
                            "require gradients")
+    # tangents are carried whether gradients are enabled or not
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None  # pylint: disable=protected-access
+                                              for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
 
 
 class PackedWeight:

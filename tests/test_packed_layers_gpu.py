@@ -63,3 +63,21 @@ def test_codes_that_are_not_whole_are_refused(device, dtype):
             bad[place] = value
             with pytest.raises(RuntimeError):
                 PackedWeight.pack(bad, *args)
+
+
+def test_tangents_are_refused_at_every_entry(device):
+    from torch.autograd import forward_ad
+
+    from aimet_amd.quantization.kv_cache import QuantizedKVCache
+
+    w = PackedWeight.pack(torch.ones(32, 64, device=device), torch.ones(32, 1, device=device))
+    x, bias = torch.randn(3, 64, device=device), torch.randn(32, device=device)
+    cache = QuantizedKVCache(1, 1, 64, 64, 64, device)
+    k = torch.randn(1, 1, 2, 64, device=device)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: packed_linear(dual(x), w), lambda: packed_linear(x, w, dual(bias)), lambda: cache.append(dual(k), k, 0),
+                     lambda: cache.append(k, dual(k), 0), lambda: cache.attend(dual(k), 2)):
+            with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                call()
+        packed_linear(x, w, bias), cache.append(k, k, 0), cache.attend(k, 2)
