@@ -27,7 +27,7 @@ from torch.nn import functional as F
 
 from aimet_amd.quantization._decompose import _DecompositionError, _decompose_prequantized_tensor
 from aimet_amd.quantization._utils import concretize_block_size, patch_attr
-from aimet_amd.quantization.affine.packed import PackedWeight, packed_linear
+from aimet_amd.quantization.affine.packed import NotPackable, PackedWeight, packed_linear
 from aimet_amd.quantization.affine.encoding import AffineEncoding
 from aimet_amd.quantization.affine.quantizer import AffineQuantizerBase, GroupedBlockQuantizeDequantize
 from aimet_amd.quantization.base.quantizer import QuantizerBase
@@ -339,7 +339,8 @@ class QuantizedLinear(nn.Linear):
     def pack(self) -> "PackedLinear":
         """The inference form of this layer: its weight as 4-bit codes under the weight quantizer's encoding (or the one
         a folded weight carries), its activation quantizers shared, its bias quantize-dequantized once.  Raises
-        where the weight has no affine encoding of at most 16 levels."""
+        NotPackable where the weight has no affine encoding of at most 16 levels, or one whose blocks or offsets the packed
+        form does not hold (blocks along a row that are neither multiples of 32 columns nor the whole row)."""
         from aimet_amd.quantization.tensor import QuantizedTensorBase
 
         self._compute_param_encodings(overwrite=False)
@@ -351,7 +352,7 @@ class QuantizedLinear(nn.Linear):
             if isinstance(wq, AffineQuantizerBase) and wq.is_initialized():
                 weight = wq(weight)
             if not isinstance(weight, QuantizedTensorBase) or not isinstance(weight.encoding, AffineEncoding):
-                raise RuntimeError("packing needs a weight with an affine encoding")
+                raise NotPackable("packing needs a weight with an affine encoding")
             weight = PackedWeight.from_encoding(weight.dequantize(), weight.encoding)
             bias = self.bias
             if bias is not None:
@@ -655,20 +656,28 @@ def fold_param_quantizers(model: nn.Module):
 
 
 def pack_linears(model: nn.Module) -> int:
-    """Replaces every QuantizedLinear of ``model`` whose weight has an affine encoding of at most 16 levels by its
-    packed form (QuantizedLinear.pack); returns how many.  Other layers are left as they are."""
+    """Replaces every QuantizedLinear of ``model`` that has a packed form (QuantizedLinear.pack) by it; returns how many.
+    Other layers are left as they are.  Nothing is replaced before all are packed, so an error leaves the model whole."""
     packed = {}  # a layer that stands in several places stays one layer
-    for parent in list(model.modules()):
-        for name, child in list(parent._modules.items()):
+    places = []
+    for parent in model.modules():
+        for name, child in parent._modules.items():
             if not isinstance(child, QuantizedLinear):
                 continue
             wq = child.param_quantizers["weight"]
             encoded = wq if wq is not None else getattr(child.weight, "encoding", None)
-            if isinstance(encoded, (AffineQuantizerBase, AffineEncoding)) and encoded.qmax - encoded.qmin <= 15:
-                if child not in packed:
+            if not isinstance(encoded, (AffineQuantizerBase, AffineEncoding)) or encoded.qmax - encoded.qmin > 15:
+                continue
+            if child not in packed:
+                try:
                     packed[child] = child.pack()
-                setattr(parent, name, packed[child])
-    return len(packed)
+                except NotPackable:
+                    packed[child] = None
+            if packed[child] is not None:
+                places.append((parent, name, packed[child]))
+    for parent, name, layer in places:
+        setattr(parent, name, layer)
+    return sum(layer is not None for layer in packed.values())
 
 
 def _remove_from_all(model, method: str) -> _Removed:

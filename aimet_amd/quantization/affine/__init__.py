@@ -18,4 +18,4 @@ from aimet_amd.quantization.affine.quantizer import (  # noqa: F401,E402
     Dequantize,
     GroupedBlockQuantizeDequantize,
 )
-from aimet_amd.quantization.affine.packed import PackedWeight, packed_linear  # noqa: F401,E402
+from aimet_amd.quantization.affine.packed import NotPackable, PackedWeight, packed_linear  # noqa: F401,E402

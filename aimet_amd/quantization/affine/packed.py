@@ -23,7 +23,11 @@ from torch.autograd import forward_ad
 from aimet_amd import _lib
 from aimet_amd.quantization._utils import concretize_block_size
 
-__all__ = ["PackedWeight", "packed_linear"]
+__all__ = ["PackedWeight", "NotPackable", "packed_linear"]
+
+
+class NotPackable(RuntimeError):
+    """A weight or an encoding that has no packed form."""
 
 
 def _refuse_gradients(what: str, *tensors) -> None:
@@ -90,10 +94,10 @@ class PackedWeight:
             raise RuntimeError("codes, scale and offset must be on one device")
         groups = scale.shape[1]
         if groups > 1 and (k // groups) % 32:
-            raise RuntimeError(f"groups of {k // groups} columns are not supported: a multiple of 32, or the whole row")
+            raise NotPackable(f"groups of {k // groups} columns are not supported: a multiple of 32, or the whole row")
         qmin = (-8 if offset is None else 0) if qmin is None else int(qmin)
         if not -128 <= qmin <= 112:
-            raise RuntimeError(f"qmin must be in [-128, 112]; got {qmin}")
+            raise NotPackable(f"qmin must be in [-128, 112]; got {qmin}")
         # everything that has to be known of the values is read back at once
         known = [t.double() for t in torch.aminmax(codes)]
         if codes.is_floating_point():
@@ -119,18 +123,18 @@ class PackedWeight:
         if offset is not None:
             o_lo, o_hi, whole = about_offset
             if not (math.isfinite(o_lo) and math.isfinite(o_hi) and whole):
-                raise RuntimeError("offsets must be whole numbers")
+                raise NotPackable("offsets must be whole numbers")
             if o_lo == o_hi:
                 zero_const += o_lo
             else:
                 if o_lo + qmin < -128 or o_hi + qmin > 127:
-                    raise RuntimeError(f"offset + qmin in [{o_lo + qmin}, {o_hi + qmin}] does not fit 8 bits")
+                    raise NotPackable(f"offset + qmin in [{o_lo + qmin}, {o_hi + qmin}] does not fit 8 bits")
                 zero = in_sixteens(off + qmin, torch.int8)
                 zero_const = float(zero_point_shift)
         lib = _lib.load()
         nbytes = lib.ahq_int4_packed_bytes(n, k)
         if nbytes == 0:
-            raise RuntimeError(f"a weight of shape {(n, k)} is too large to pack")
+            raise NotPackable(f"a weight of shape {(n, k)} is too large to pack")
         packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
         raw = codes.detach().to(torch.int8).contiguous()
         with torch.cuda.device(codes.device):
@@ -146,7 +150,7 @@ class PackedWeight:
         if weight.dim() != 2:
             raise RuntimeError(f"a weight of two dimensions is expected; got shape {tuple(weight.shape)}")
         if encoding.qmax - encoding.qmin > 15:
-            raise RuntimeError(f"the grid [{encoding.qmin}, {encoding.qmax}] has more than 16 levels")
+            raise NotPackable(f"the grid [{encoding.qmin}, {encoding.qmax}] has more than 16 levels")
         n, k = weight.shape
         with torch.no_grad():
             weight = weight.detach().as_subclass(torch.Tensor)
@@ -163,14 +167,14 @@ class PackedWeight:
             if encoding.block_size is not None:
                 concretize_block_size((n, k), tuple(encoding.scale.shape), encoding.block_size)  # its own errors
             if scale.shape[1] not in (1, k) and encoding.block_size is None:
-                raise RuntimeError(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
+                raise NotPackable(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
             shift = encoding.zero_point_shift or 0.0
             if shift == 0.0:
                 codes = encoding.quantize(weight).as_subclass(torch.Tensor)
             else:
                 # quantize() knows no shift: what lies on the shifted grid lies half-way between its codes
                 if scale.shape[0] != n or k % scale.shape[1]:
-                    raise RuntimeError(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
+                    raise NotPackable(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
                 on_grid = encoding.quantize_dequantize(weight).as_subclass(torch.Tensor).float()
                 levels = on_grid.view(n, scale.shape[1], -1) / scale[..., None] - offset[..., None] - shift
                 codes = levels.round().clamp(encoding.qmin, encoding.qmax).view(n, k)

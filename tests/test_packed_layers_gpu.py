@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from aimet_amd import nn as qnn
-from aimet_amd.quantization.affine import PackedWeight, QuantizeDequantize, packed_linear
+from aimet_amd.quantization.affine import NotPackable, PackedWeight, QuantizeDequantize, packed_linear
 
 pytestmark = pytest.mark.gpu
 names = lambda d: str(d).split(".")[-1]  # noqa: E731
@@ -81,3 +81,40 @@ def test_tangents_are_refused_at_every_entry(device):
             with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
                 call()
         packed_linear(x, w, bias), cache.append(k, k, 0), cache.attend(k, 2)
+
+
+def _mixed(device):
+    """Layers with a packed form and without one: blocks of 16 columns, 8 bits, no weight quantizer."""
+    return torch.nn.ModuleDict({
+        "block64": _layer(QuantizeDequantize((96, 4), 4, symmetric=True, block_size=(1, 64)), device)[0],
+        "block16": _layer(QuantizeDequantize((96, 16), 4, symmetric=True, block_size=(1, 16)), device)[0],
+        "bits8": _layer(QuantizeDequantize((96, 1), 8, symmetric=True), device)[0],
+        "none": _layer(None, device)[0],
+        "channel": _layer(QuantizeDequantize((96, 1), 4, symmetric=False), device)[0]})
+
+
+def test_layers_without_a_packed_form_stay(device):
+    model = _mixed(device)
+    before = dict(model.items())
+    with pytest.raises(NotPackable, match="16 columns"):
+        before["block16"].pack()
+    x = torch.randn(5, 256, device=device)
+    with torch.no_grad():
+        want = {k: plain(m(x)) for k, m in model.items()}
+        assert qnn.pack_linears(model) == 2
+        for k, m in model.items():
+            if k in ("block64", "channel"):
+                assert isinstance(m, qnn.PackedLinear)
+            else:
+                assert m is before[k] and torch.equal(plain(m(x)), want[k])
+        assert qnn.pack_linears(model) == 0
+
+
+def test_an_error_leaves_the_model_whole(device):
+    """A layer that cannot be packed for another reason than its encoding: its weight is not on the device."""
+    model = _mixed(device)
+    before = dict(model.items())
+    before["channel"].weight.data = before["channel"].weight.data.cpu()
+    with pytest.raises(RuntimeError):
+        qnn.pack_linears(model)
+    assert all(model[k] is m for k, m in before.items())
