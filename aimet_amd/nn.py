@@ -116,7 +116,53 @@ class _Removed:
         return False
 
 
-class QuantizedLinear(nn.Linear):
+class _ActivationQuantizers:
+    """What layers with ``input_quantizers`` and ``output_quantizers`` have in common."""
+
+    def _remove_input_quantizers(self, indices=None):
+        """nn/base.py:983-993: the input quantizers (all, one index or several) are taken out at once; used as a
+        context manager, the call puts them back on leaving."""
+        if isinstance(indices, int):
+            indices = [indices]
+        elif indices is None:
+            indices = list(range(len(self.input_quantizers)))
+        return _Removed(self.input_quantizers, [str(i) for i in indices])
+
+    def _remove_output_quantizers(self, indices=None):
+        """nn/base.py:1007-1017."""
+        if isinstance(indices, int):
+            indices = [indices]
+        elif indices is None:
+            indices = list(range(len(self.output_quantizers)))
+        return _Removed(self.output_quantizers, [str(i) for i in indices])
+
+    def _remove_activation_quantizers(self):
+        """nn/base.py:1019-1026."""
+        return _Removed.both(self._remove_output_quantizers(), self._remove_input_quantizers())
+
+    def _remove_all_quantizers(self):
+        """nn/base.py:1028-1035."""
+        return _Removed.both(self._remove_activation_quantizers(), self._remove_param_quantizers())
+
+    def export_input_encodings(self, encoding_version: str):
+        """One exported dictionary (or None) per input quantizer (nn/base.py:527-539)."""
+        return [q.get_encodings().to_qnn_encoding_dict(encoding_version)
+                if isinstance(q, QuantizerBase) and q.is_initialized() else None for q in self.input_quantizers]
+
+    def export_output_encodings(self, encoding_version: str):
+        """nn/base.py:586-598."""
+        return [q.get_encodings().to_qnn_encoding_dict(encoding_version)
+                if isinstance(q, QuantizerBase) and q.is_initialized() else None for q in self.output_quantizers]
+
+    def _observe_activations(self, stack: contextlib.ExitStack):
+        """Until ``stack`` is left, activation quantizers observe their inputs and pass them through; then they set their
+        ranges (nn/base.py:392-427)."""
+        for qtzr in list(self.input_quantizers) + list(self.output_quantizers):
+            if isinstance(qtzr, QuantizerBase) and qtzr.is_overwrite_allowed():
+                stack.enter_context(qtzr._compute_encodings(passthrough=True))  # pylint: disable=protected-access
+
+
+class QuantizedLinear(_ActivationQuantizers, nn.Linear):
     """``nn.Linear`` with quantizers at its input, weight and output (any of them may be None)."""
 
     def __init__(self, *args, **kwargs):
@@ -249,49 +295,14 @@ class QuantizedLinear(nn.Linear):
             names.append(name)
         return names
 
-    def _remove_input_quantizers(self, indices=None):
-        """nn/base.py:983-993: the input quantizers (all, one index or several) are taken out at once; used as a
-        context manager, the call puts them back on leaving."""
-        if isinstance(indices, int):
-            indices = [indices]
-        elif indices is None:
-            indices = list(range(len(self.input_quantizers)))
-        return _Removed(self.input_quantizers, [str(i) for i in indices])
-
     def _remove_param_quantizers(self, keys=None):
         """nn/base.py:995-1005."""
         keys = list(self.param_quantizers.keys()) if keys is None else ([keys] if isinstance(keys, str) else list(keys))
         return _Removed(self.param_quantizers, keys)
 
-    def _remove_output_quantizers(self, indices=None):
-        """nn/base.py:1007-1017."""
-        if isinstance(indices, int):
-            indices = [indices]
-        elif indices is None:
-            indices = list(range(len(self.output_quantizers)))
-        return _Removed(self.output_quantizers, [str(i) for i in indices])
-
-    def _remove_activation_quantizers(self):
-        """nn/base.py:1019-1026."""
-        return _Removed.both(self._remove_output_quantizers(), self._remove_input_quantizers())
-
-    def _remove_all_quantizers(self):
-        """nn/base.py:1028-1035."""
-        return _Removed.both(self._remove_activation_quantizers(), self._remove_param_quantizers())
-
     def compute_param_encodings(self):
         """Compute the encodings of the parameter quantizers (nn/base.py:388-390)."""
         self._compute_param_encodings(overwrite=True)
-
-    def export_input_encodings(self, encoding_version: str):
-        """One exported dictionary (or None) per input quantizer (nn/base.py:527-539)."""
-        return [q.get_encodings().to_qnn_encoding_dict(encoding_version)
-                if isinstance(q, QuantizerBase) and q.is_initialized() else None for q in self.input_quantizers]
-
-    def export_output_encodings(self, encoding_version: str):
-        """nn/base.py:586-598."""
-        return [q.get_encodings().to_qnn_encoding_dict(encoding_version)
-                if isinstance(q, QuantizerBase) and q.is_initialized() else None for q in self.output_quantizers]
 
     def export_param_encodings(self, encoding_version: str):
         """{parameter name: exported dictionary or None} (nn/base.py:645-678); a parameter that is an already
@@ -377,14 +388,11 @@ class QuantizedLinear(nn.Linear):
             if once:
                 stack.enter_context(self._patch_quantized_parameters(once, _quantized=quantized))
                 stack.enter_context(self._remove_param_quantizers(once))
-            for qtzr in list(self.input_quantizers) + list(self.output_quantizers):
-                if not isinstance(qtzr, QuantizerBase) or not qtzr.is_overwrite_allowed():
-                    continue
-                stack.enter_context(qtzr._compute_encodings(passthrough=True))  # pylint: disable=protected-access
+            self._observe_activations(stack)
             yield
 
 
-class PackedLinear(nn.Module):
+class PackedLinear(_ActivationQuantizers, nn.Module):
     """A linear layer that runs on 4-bit codes (``QuantizedLinear.pack``): quantize-dequantizes its input and output as
     the layer it was made from, but reads a packed weight instead of quantize-dequantizing a floating-point one.
     Inference only: nothing in it learns and ``forward`` refuses tensors that require gradients."""
@@ -416,6 +424,17 @@ class PackedLinear(nn.Module):
         out = packed_linear(input, self.weight, self.bias)
         return out if oq is None else oq(out)
 
+    def _remove_param_quantizers(self, keys=None):
+        """The weight's grid is part of it, as where a quantizer was folded: there is none to take out."""
+        return _Removed(nn.ModuleDict(), [])
+
+    @contextlib.contextmanager
+    def compute_encodings(self):
+        """The ranges of the activation quantizers from what passes inside the context; the weight keeps its codes."""
+        with contextlib.ExitStack() as stack:
+            self._observe_activations(stack)
+            yield
+
     def _apply(self, fn, recurse=True):
         """Conversions to another floating-point type leave the scales in float32."""
         scale = self.weight_scale
@@ -442,6 +461,11 @@ class PackedLinear(nn.Module):
 
 def quantized_linears(model: nn.Module) -> Iterable[QuantizedLinear]:
     return (m for m in model.modules() if isinstance(m, QuantizedLinear))
+
+
+def _layers_with_quantizers(model: nn.Module):
+    """The quantized layers and the packed ones, whose activation quantizers work as before."""
+    return (m for m in model.modules() if isinstance(m, (QuantizedLinear, PackedLinear)))
 
 
 def _probe_parameters_together(candidates):
@@ -631,7 +655,7 @@ def compute_encodings(model: nn.Module):
                 stack.enter_context(m._remove_param_quantizers(once))  # pylint: disable=protected-access
         # 2. activations: observed and passed through unquantized; ranges set on leaving (nn/base.py:392-427)
         observing = []
-        for m in modules:
+        for m in _layers_with_quantizers(model):
             for qtzr in list(m.input_quantizers) + list(m.output_quantizers):
                 if not isinstance(qtzr, QuantizerBase) or not qtzr.is_overwrite_allowed():
                     continue
@@ -682,7 +706,7 @@ def pack_linears(model: nn.Module) -> int:
 
 def _remove_from_all(model, method: str) -> _Removed:
     removed = None
-    for m in quantized_linears(model):
+    for m in _layers_with_quantizers(model):
         one = getattr(m, method)()
         removed = one if removed is None else _Removed.both(removed, one)
     return removed if removed is not None else _Removed(nn.ModuleList(), [])

@@ -118,3 +118,38 @@ def test_an_error_leaves_the_model_whole(device):
     with pytest.raises(RuntimeError):
         qnn.pack_linears(model)
     assert all(model[k] is m for k, m in before.items())
+
+
+def test_activation_quantizers_of_packed_layers(device):
+    """The model-level helpers treat a packed layer's activation quantizers as those of the layer it was made from."""
+    q, x = _layer(QuantizeDequantize((96, 4), 4, symmetric=True, block_size=(1, 64)), device)
+    p = q.pack()
+    model = torch.nn.Sequential(p)
+    with torch.no_grad():
+        bare = packed_linear(x, p.weight, p.bias)
+        quantized = plain(model(x))
+        assert not torch.equal(quantized, bare)
+        for remove in (qnn.remove_activation_quantizers, qnn.remove_all_quantizers):
+            with remove(model):
+                assert torch.equal(plain(model(x)), bare)
+            assert torch.equal(plain(model(x)), quantized)
+        with qnn.remove_input_quantizers(model):
+            assert p.input_quantizers[0] is None and p.output_quantizers[0] is not None
+        with qnn.remove_output_quantizers(model):
+            assert p.input_quantizers[0] is not None and p.output_quantizers[0] is None
+        with qnn.remove_param_quantizers(model):
+            assert torch.equal(plain(model(x)), quantized)
+        # calibrated anew on ten times the data, together with the model, alone, and before it was packed
+        ranges = []
+        for target, context in ((model, lambda: qnn.compute_encodings(model)), (p, p.compute_encodings), (q, q.compute_encodings)):
+            p.input_quantizers[0].set_range(-1, 1)
+            with context():
+                target(10 * x)
+            ranges.append([t.clone() for o in (p.input_quantizers[0], p.output_quantizers[0]) for t in (o.min, o.max)])
+        assert ranges[0][1] > 20
+        for a, b, c in zip(*ranges):
+            # the layers' products differ by the roundings of 256 terms in float32, the asymmetric grid by a step of 16 bits
+            assert torch.equal(a, b) and bool((a - c).abs() <= 2.0 ** -12 * c.abs().max() + 2.0 ** -12)
+        assert p.export_input_encodings("1.0.0")[0] is not None and p.export_output_encodings("1.0.0")[0] is not None
+        qnn.remove_activation_quantizers(model)
+        assert p.input_quantizers[0] is None and p.output_quantizers[0] is None
