@@ -369,7 +369,9 @@ class QuantizedLinear(_ActivationQuantizers, nn.Linear):
             if bias is not None:
                 bias = bias if bq is None else bq(bias)
                 bias = bias.detach().as_subclass(torch.Tensor).clone()
-        return PackedLinear(weight, bias, self.input_quantizers[0], self.output_quantizers[0])
+        packed = PackedLinear(weight, bias, self.input_quantizers[0], self.output_quantizers[0])
+        packed.training = self.training  # the shared quantizers' own modes stay
+        return packed
 
     @contextlib.contextmanager
     def compute_encodings(self, _verdicts=None):
@@ -681,7 +683,8 @@ def fold_param_quantizers(model: nn.Module):
 
 def pack_linears(model: nn.Module) -> int:
     """Replaces every QuantizedLinear of ``model`` that has a packed form (QuantizedLinear.pack) by it; returns how many.
-    Other layers are left as they are.  Nothing is replaced before all are packed, so an error leaves the model whole."""
+    Other layers are left as they are.  Nothing is replaced before all are packed, so an error leaves the model whole.
+    Forward hooks go over to the packed layers, and their handles still remove them."""
     packed = {}  # a layer that stands in several places stays one layer
     places = []
     for parent in model.modules():
@@ -697,6 +700,10 @@ def pack_linears(model: nn.Module) -> int:
                     packed[child] = child.pack()
                 except NotPackable:
                     packed[child] = None
+                else:
+                    for hooks in ("_forward_pre_hooks", "_forward_pre_hooks_with_kwargs", "_forward_hooks",
+                                  "_forward_hooks_with_kwargs", "_forward_hooks_always_called"):
+                        setattr(packed[child], hooks, getattr(child, hooks))
             if packed[child] is not None:
                 places.append((parent, name, packed[child]))
     for parent, name, layer in places:

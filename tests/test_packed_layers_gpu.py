@@ -153,3 +153,24 @@ def test_activation_quantizers_of_packed_layers(device):
         assert p.export_input_encodings("1.0.0")[0] is not None and p.export_output_encodings("1.0.0")[0] is not None
         qnn.remove_activation_quantizers(model)
         assert p.input_quantizers[0] is None and p.output_quantizers[0] is None
+
+
+def test_what_a_replaced_layer_had(device):
+    """Training mode and forward hooks stay with the place of the layer; the handles still remove them."""
+    q, x = _layer(QuantizeDequantize((96, 4), 4, symmetric=True, block_size=(1, 64)), device)
+    other, _ = _layer(QuantizeDequantize((96, 1), 4, symmetric=True), device)
+    model = torch.nn.ModuleDict({"a": q, "b": other.eval()})
+    calls = []
+    handles = [q.register_forward_pre_hook(lambda m, a: calls.append(type(m).__name__)),
+               q.register_forward_hook(lambda m, a, k, out: out * 0 if k.get("input") is None else out, with_kwargs=True),
+               q.register_forward_hook(lambda m, a, out: calls.append("always"), always_call=True)]
+    with torch.no_grad():
+        assert qnn.pack_linears(model) == 2
+        assert model["a"].training and not model["b"].training
+        assert not bool(plain(model["a"](x)).any()) and calls == ["PackedLinear", "always"]
+        assert bool(plain(model["a"](input=x)).any())
+        for h in handles:
+            h.remove()
+        calls.clear()
+        assert bool(plain(model["a"](x)).any()) and not calls
+        assert not other.eval().pack().training
