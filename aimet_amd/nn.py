@@ -684,7 +684,11 @@ def fold_param_quantizers(model: nn.Module):
 def pack_linears(model: nn.Module) -> int:
     """Replaces every QuantizedLinear of ``model`` that has a packed form (QuantizedLinear.pack) by it; returns how many.
     Other layers are left as they are.  Nothing is replaced before all are packed, so an error leaves the model whole.
-    Forward hooks go over to the packed layers, and their handles still remove them."""
+    Forward hooks go over to the packed layers, and their handles still remove them.  A model that is itself a
+    QuantizedLinear cannot be replaced in place and is refused."""
+    if isinstance(model, QuantizedLinear):
+        raise RuntimeError("the model is itself a QuantizedLinear, which nothing holds that could be given its packed form: "
+                           "use its pack()")
     packed = {}  # a layer that stands in several places stays one layer
     places = []
     for parent in model.modules():

@@ -174,3 +174,9 @@ def test_what_a_replaced_layer_had(device):
         calls.clear()
         assert bool(plain(model["a"](x)).any()) and not calls
         assert not other.eval().pack().training
+
+
+def test_a_model_that_is_a_layer_is_refused(device):
+    q, _ = _layer(QuantizeDequantize((96, 1), 4, symmetric=True), device)
+    with pytest.raises(RuntimeError, match="pack()"):
+        qnn.pack_linears(q)
