@@ -397,7 +397,8 @@ class QuantizedLinear(_ActivationQuantizers, nn.Linear):
 class PackedLinear(_ActivationQuantizers, nn.Module):
     """A linear layer that runs on 4-bit codes (``QuantizedLinear.pack``): quantize-dequantizes its input and output as
     the layer it was made from, but reads a packed weight instead of quantize-dequantizing a floating-point one.
-    Inference only: nothing in it learns and ``forward`` refuses tensors that require gradients."""
+    Under autocast the product has its type.  Inference only: nothing in it learns and ``forward`` refuses tensors that
+    require gradients.  Unlike the product it stands for, one infinite activation makes its whole row NaN."""
 
     def __init__(self, weight: PackedWeight, bias: Optional[torch.Tensor] = None, input_quantizer=None,
                  output_quantizer=None):
@@ -423,7 +424,11 @@ class PackedLinear(_ActivationQuantizers, nn.Module):
         iq, oq = self.input_quantizers[0], self.output_quantizers[0]
         if iq is not None:
             input = iq(input)
-        out = packed_linear(input, self.weight, self.bias)
+        bias = self.bias
+        if torch.is_autocast_enabled("cuda"):  # as the product of the layer it was made from
+            dtype = torch.get_autocast_dtype("cuda")
+            input, bias = input.as_subclass(torch.Tensor).to(dtype), None if bias is None else bias.to(dtype)
+        out = packed_linear(input, self.weight, bias)
         return out if oq is None else oq(out)
 
     def _remove_param_quantizers(self, keys=None):

@@ -180,3 +180,25 @@ def test_a_model_that_is_a_layer_is_refused(device):
     q, _ = _layer(QuantizeDequantize((96, 1), 4, symmetric=True), device)
     with pytest.raises(RuntimeError, match="pack()"):
         qnn.pack_linears(q)
+
+
+@pytest.mark.parametrize("layer_dtype", [torch.float32, torch.bfloat16], ids=names)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=names)
+def test_autocast(device, layer_dtype, dtype):
+    """Under autocast the packed layer computes in autocast's type, as the layer it was made from."""
+    q, x = _layer(QuantizeDequantize((96, 4), 4, symmetric=True, block_size=(1, 64)), device, layer_dtype)
+    p = q.pack()
+    for layer in (q, p):
+        layer.output_quantizers[0] = None
+    with torch.no_grad():
+        with torch.autocast("cuda", dtype=dtype):
+            got, want = plain(p(x)), plain(q(x))
+            xin = plain(p.input_quantizers[0](x)).to(dtype)
+        assert got.dtype == want.dtype == dtype
+        assert torch.equal(got, packed_linear(xin, p.weight, p.bias.to(dtype)))
+        # the layer's weight is rounded to autocast's type (and to its own before), the result once on either side
+        total = xin.double().abs() @ plain(q.param_quantizers["weight"](q.weight)).double().abs().T + p.bias.double().abs()
+        eps = torch.finfo(dtype).eps / 2
+        own = torch.finfo(layer_dtype).eps
+        assert bool(((got - want).double().abs() <= (eps + 1.01 * own + 512 * 2.0 ** -23) * total + 2 * eps * want.double().abs() * 1.01).all())
+        assert plain(p(x)).dtype == layer_dtype
