@@ -17,11 +17,12 @@
 //
 // Both products run in float16 with float32 sums.  Codes are exact in it: a byte b next to the byte 0x64 is the number
 // 1024 + b, and one packed addition of -1152 makes two codes of two bytes.  A query row is multiplied by the power of two
-// that brings its largest value to 2^13 .. 2^14, which keeps 16-bit queries exact (bfloat16 down to 2^-30 of the row's
-// largest value); float32 queries become two parts, 22 bits.  Probabilities carry the scale of their values' block:
-// with x = score + log2(scale), weights are 2^(x - reference), the reference being such that the largest weight so far lies
-// between 2^10 and 2^15 (it is moved, and the sums with it, only when a weight passes 2^15).  Weights are two float16 parts
-// for queries of every type: off by at most 2^-22 of themselves, and by 2^-25 where they are small, 2^-35 of the largest.
+// that brings its largest value to 2^13 .. 2^14 (float16 rows that are larger stay as they are), which keeps 16-bit
+// queries exact (bfloat16 down to 2^-30 of the row's largest value); float32 queries become two parts, 22 bits.
+// Probabilities carry the scale of their values' block: with x = score + log2(scale), weights are 2^(x - reference), the
+// reference being such that the largest weight so far lies between 2^10 and 2^15 (it is moved, and the sums with it, only
+// when a weight passes 2^15).  Weights are two float16 parts for queries of every type: off by at most 2^-22 of themselves,
+// and by 2^-25 where they are small, 2^-35 of the largest.
 // One part (2^-11) would show in 16-bit answers: those of decoding then differ from a float32 softmax's by 4e-4 relative,
 // with two by 3e-5 or not at all, at the same time; prompts pay for it (2048 of 3048 tokens: 147 -> 192 us).  The softmax's
 // denominator sums weight / scale in float32.  Scales are counted in a unit of the workgroup's share, a power of two: 1 where
@@ -523,6 +524,8 @@ struct AttendRows {
             int ex = (int)(f32_to_bits(size) >> 23);
             if (size == 0.0f || ex >= 255) ex = 140;
             if (ex < 16) ex = 16;
+            // float16 is never scaled down: its smallest numbers would lose bits, and its largest fit as they are
+            if (std::is_same_v<T, f16_t> && ex > 140) ex = 140;
             const float up = bits_to_f32((uint32_t)(267 - ex) << 23);
             rescale[n] = bits_to_f32((uint32_t)(ex - 13) << 23) * a.scale;
 #pragma unroll

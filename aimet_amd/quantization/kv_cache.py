@@ -161,7 +161,8 @@ class QuantizedKVCache:
         see nothing, and those behind ``counts``, are answered with 0.  ``scale`` multiplies the scores (default
         1 / sqrt(head_dim)).  The result has the queries' type, shape and, where they are dense, memory layout.
 
-        16-bit queries are used as they are and float32 queries to 22 bits of a row's largest value; probabilities have
+        16-bit queries are used as they are (bfloat16 down to 2^-30 of a row's largest value), float32 queries to 22 bits, those
+        far below a row's largest value to fewer; probabilities have
         22 bits and are off by at most 2^-35 of the row's largest one where they are small (both weighted by the scale of
         their values' block); all sums are float32, and the result is rounded once.  Values may be of any size; blocks whose
         values are all below 2^-72 of the largest that a query sees count as up to that."""

@@ -95,8 +95,8 @@ int ahq_kv_append(const ahq_kv_cache* cache, const ahq_kv_tokens* x, void* strea
 /* The first `length` tokens' values as [batch][heads][length][head_dim] of `dtype`, keys and values (16-byte aligned). */
 int ahq_kv_dequantize(const ahq_kv_cache* cache, int32_t dtype, int32_t length, void* k, void* v, void* stream);
 
-/* softmax(scale * q k^T) v over the cache.  Codes are exact in both products, 16-bit queries as well; float32 queries
- * have 22 bits of a row's largest value, probabilities 22 bits for queries of every type, sums are float32.  Blocks whose
+/* softmax(scale * q k^T) v over the cache.  Codes are exact in both products, 16-bit queries as well (bfloat16
+ * down to 2^-30 of a row's largest value); float32 queries have 22 bits, those far below a row's largest value fewer; probabilities 22 bits for queries of every type, sums are float32.  Blocks whose
  * values are all below 2^-72 of the largest that a query sees count as up to that.  The workspace (0 bytes where the token axis is not split) depends on the
  * shapes and on whether the lengths are a device array, not on their values. */
 size_t ahq_kv_attend_workspace_bytes(const ahq_kv_cache* cache, const ahq_kv_queries* q);

@@ -176,3 +176,21 @@ def test_scales_of_discarded_tokens(device, queries, dtype):
         cache.append(k[:, :, :length], v[:, :, :length] * 1e-20, 0)
         outs.append(_check_sizes(cache, q, length))
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("batch,heads,queries,length", FORMS)
+@pytest.mark.parametrize("top", [1.0, 16384.0, 65504.0])
+def test_float16_queries_are_exact(device, top, batch, heads, queries, length):
+    """Queries of one large channel, whose keys are zero, and of the smallest numbers of float16 in the others: those make
+    the scores, and a bit lost of them would be an error of 1 / 15 at least."""
+    g = torch.Generator().manual_seed(0)
+    d = 64
+    q = torch.randint(-15, 16, (batch, heads, queries, d), generator=g).float() * 2.0 ** -24
+    q[..., 0] = top
+    k = torch.randn(batch, heads, length, d, generator=g) * 2.0 ** 20
+    k[..., 0] = 0
+    cache = QuantizedKVCache(batch, heads, length, d, 64, device)
+    cache.append(k.to(device), torch.randn(batch, heads, length, d, generator=g).to(device), 0)
+    q = q.half()
+    assert bool((q[..., 1:] != 0).any()) and bool((q[..., 0] == top).all())
+    _check_sizes(cache, q.to(device), length)
