@@ -116,7 +116,12 @@ class QuantizedKVCache:
                counts: Optional[PerSequence] = None) -> None:
         """Stores keys and values [batch, kv_heads, tokens, head_dim] (any strides): token t of a sequence goes to
         position ``start + t``; of a padded batch only the first ``counts`` tokens of each sequence are stored.  Infinite
-        values saturate and NaN is stored as 0; neither sets a block's scale."""
+        values saturate and NaN is stored as 0; neither sets a block's scale.
+
+        A block that ``start`` lies inside keeps the scale it has, and this is also that of tokens which stood at ``start`` or
+        behind it: where those were discarded (rejected drafts), what the block holds and what is appended to it stay on their
+        grid, until a call begins at the block's first token.  What stands behind the last new token of a block counts as
+        discarded: its codes stay, but the scale may be another."""
         self._check(k, "k", self.kv_heads)
         self._check(v, "v", self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:

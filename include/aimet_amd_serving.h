@@ -86,10 +86,12 @@ typedef struct {
     float scale;
 } ahq_kv_queries;
 
-/* Stores tokens: a block's amax is the larger of what it held before `start` and of the new finite magnitudes, codes
- * are rint(127 x / amax) half to even (exact; infinities saturate, NaN and everything in a block of zeros is 0), and the
- * codes a block already had become rint(code * old amax / new amax) where it grew.  Nothing behind the last new token is
- * written.  Two calls for the same block have to be ordered. */
+/* Stores tokens: a block's amax is that of the new finite magnitudes, and no less than what it was where the first new token
+ * is not the block's first (tokens at and behind `start`, of an earlier call, have their part in it although they are
+ * overwritten or discarded), codes are rint(127 x / amax) half to even (exact; infinities saturate, NaN and everything in a
+ * block of zeros is 0), and the codes of a block's tokens in front of `start` become rint(code * old amax / new amax) where
+ * it grew.  No code behind the last new token is written; such tokens count as discarded, and the block's amax need not be
+ * theirs.  Two calls for the same block have to be ordered. */
 int ahq_kv_append(const ahq_kv_cache* cache, const ahq_kv_tokens* x, void* stream);
 
 /* The first `length` tokens' values as [batch][heads][length][head_dim] of `dtype`, keys and values (16-byte aligned). */

@@ -194,3 +194,25 @@ def test_float16_queries_are_exact(device, top, batch, heads, queries, length):
     q = q.half()
     assert bool((q[..., 1:] != 0).any()) and bool((q[..., 0] == top).all())
     _check_sizes(cache, q.to(device), length)
+
+
+def test_rewound_block_keeps_its_scale(device):
+    """A draft with one large token is discarded inside a block: what was there and what follows stay on its grid, the next
+    block and a block that is begun anew do not."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.rand(1, 1, 40, 64, generator=g) * 2 - 1
+    x[0, 0, 0, 0], x[0, 0, 9, 3], x[0, 0, 20, 5] = 1.0, -1.0, 1.0
+    draft = torch.randn(1, 1, 4, 64, generator=g)
+    draft[0, 0, 2, 7] = 50.0
+    cache = QuantizedKVCache(1, 1, 64, 64, 16, device)
+    cache.append(x[:, :, :10].to(device), x[:, :, :10].to(device), 0)
+    cache.append(draft.to(device), draft.to(device), 10)
+    cache.append(x[:, :, 10:].to(device), x[:, :, 10:].to(device), 10)
+    fine, coarse = (x.double() * 127).round(), (x.double() * 127 / 50).round()
+    coarse[:, :, :10] = (fine[:, :, :10] / 50).round()
+    for codes, amax in zip(cache.codes(), (cache.k_amax, cache.v_amax)):
+        codes = codes.cpu().double()
+        assert amax[0, 0, 0] == 50 and amax[0, 0, 1] == 1
+        assert torch.equal(codes[:, :, :16], coarse[:, :, :16]) and torch.equal(codes[:, :, 16:32], fine[:, :, 16:32])
+    cache.append(x[:, :, :16].to(device), x[:, :, :16].to(device), 0)
+    assert cache.k_amax[0, 0, 0] == 1 and torch.equal(cache.codes()[0].cpu().double()[:, :, :16], fine[:, :, :16])
