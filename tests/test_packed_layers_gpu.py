@@ -202,3 +202,46 @@ def test_autocast(device, layer_dtype, dtype):
         own = torch.finfo(layer_dtype).eps
         assert bool(((got - want).double().abs() <= (eps + 1.01 * own + 512 * 2.0 ** -23) * total + 2 * eps * want.double().abs() * 1.01).all())
         assert plain(p(x)).dtype == layer_dtype
+
+
+@pytest.mark.parametrize("m,n,k", [(20, 320, 4096), (300, 4096, 1024), (1100, 4200, 512)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=names)
+def test_captured_calls_with_large_shared_memory(device, m, n, k, dtype):
+    """Kernels that ask for more than 64 KB of shared memory at their launch, captured as their process's first call of these
+    shapes and replayed with other inputs."""
+    g = torch.Generator().manual_seed(0)
+    w = PackedWeight.pack(torch.randint(-8, 8, (n, k), generator=g).to(torch.int8).to(device), torch.rand(n, k // 64, generator=g).to(device))
+    x = torch.randn(m, k, generator=g).to(dtype).to(device)
+    packed_linear(x[:1], w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = packed_linear(x, w)
+    for _ in range(3):
+        x.copy_(torch.randn(m, k, generator=g))
+        graph.replay()
+        eager = packed_linear(x, w)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager) and bool(y.any())
+
+
+@pytest.mark.parametrize("batch,queries", [(1, 2), (8, 50)])
+def test_captured_attention_with_large_shared_memory(device, batch, queries):
+    """Head size 256: 70 KB for few rows, 128 KB for many."""
+    from aimet_amd.quantization.kv_cache import QuantizedKVCache
+
+    g = torch.Generator().manual_seed(0)
+    cache = QuantizedKVCache(batch, 16, 192, 256, 64, device)
+    kv = torch.randn(batch, 16, 190, 256, generator=g).bfloat16().to(device)
+    cache.append(kv, kv.flip(3).contiguous(), 0)
+    q = torch.randn(batch, 16, queries, 256, generator=g).bfloat16().to(device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, 190)
+    for _ in range(3):
+        q.copy_(torch.randn(q.shape, generator=g))
+        graph.replay()
+        eager = cache.attend(q, 190)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and bool(out.any())
