@@ -176,8 +176,8 @@ class PackedWeight:
                 if scale.shape[0] != n or k % scale.shape[1]:
                     raise NotPackable(f"scale of shape {tuple(encoding.scale.shape)} does not describe a weight of {(n, k)}")
                 on_grid = encoding.quantize_dequantize(weight).as_subclass(torch.Tensor).float()
-                levels = on_grid.view(n, scale.shape[1], -1) / scale[..., None] - offset[..., None] - shift
-                codes = levels.round().clamp(encoding.qmin, encoding.qmax).view(n, k)
+                levels = on_grid.reshape(n, scale.shape[1], -1) / scale[..., None] - offset[..., None] - shift
+                codes = levels.round().clamp(encoding.qmin, encoding.qmax).reshape(n, k)
             return cls.pack(codes, scale, offset, encoding.qmin, shift)
 
 

@@ -40,6 +40,7 @@ def test_shifted_grids(device, kind, dtype):
     with torch.no_grad():
         dense = plain(wq(q.weight)).float()
         for weight in (q.pack().weight, PackedWeight.from_encoding(q.weight, wq.get_encodings()),
+                       PackedWeight.from_encoding(q.weight.T.contiguous().T, wq.get_encodings()),
                        PackedWeight.from_encoding(wq(q.weight).dequantize(), wq.get_encodings())):
             read = packed_linear(eye, weight).T
             assert bool(((read - dense).abs() <= 1.01 * torch.finfo(dtype).eps * read.abs()).all())
