@@ -425,7 +425,8 @@ class PackedLinear(_ActivationQuantizers, nn.Module):
         if iq is not None:
             input = iq(input)
         bias = self.bias
-        if torch.is_autocast_enabled("cuda"):  # as the product of the layer it was made from
+        # as the product of the layer it was made from
+        if torch.is_autocast_enabled("cuda") and input.dtype in (torch.float32, torch.bfloat16, torch.float16):
             dtype = torch.get_autocast_dtype("cuda")
             input, bias = input.as_subclass(torch.Tensor).to(dtype), None if bias is None else bias.to(dtype)
         out = packed_linear(input, self.weight, bias)

@@ -203,6 +203,10 @@ def test_autocast(device, layer_dtype, dtype):
         own = torch.finfo(layer_dtype).eps
         assert bool(((got - want).double().abs() <= (eps + 1.01 * own + 512 * 2.0 ** -23) * total + 2 * eps * want.double().abs() * 1.01).all())
         assert plain(p(x)).dtype == layer_dtype
+        p.input_quantizers[0] = None
+        for other in (x.double(), x.long()):  # autocast leaves these as they are
+            with torch.autocast("cuda", dtype=dtype), pytest.raises(RuntimeError):
+                p(other)
 
 
 @pytest.mark.parametrize("m,n,k", [(20, 320, 4096), (300, 4096, 1024), (1100, 4200, 512)])
