@@ -123,7 +123,7 @@ struct Int4Args {
 // The activations' sums are formed along with the products, by every wave for itself: matrix instructions wait for nobody
 // here, and a pass of their own with its barrier took 0.4 to 0.8 us (32 x 4096 x 4096 14.0 -> 12.4 us).
 //
-// One token x 14336 x 4096 (33 MB): 10.6 us, 3.1 TB/s, of which the start takes 4.1 (launch 2.0, activations).  One, three and
+// One token x 14336 x 4096 (33 MB): 10.9 us, 3.0 TB/s, of which the start takes 4.1 (launch 2.0, activations).  One, three and
 // four tiles at once instead of two: 12.0, 11.3, 11.7 us; two workgroups on a compute unit (64 registers): 17 us, spills.
 constexpr int kLdsWaves = 16;
 constexpr int kLdsThreads = kLdsWaves * kWave;
@@ -584,7 +584,7 @@ inline LdsPlan plan_lds(const Int4Args& a, int parts, int mt) {
     // as many waves to a row tile as one workgroup on each of the 256 compute units gives
     p.splits = kLdsWaves;
     while (p.splits > 1 && (p.splits > a.tiles || ceil_div(a.ntiles, kLdsWaves / p.splits) > 256)) p.splits /= 2;
-    const int64_t fit = (160 * 1024 - m * parts * 16) / (m * parts * 256);  // 6 tiles at least: 32 activations, three parts
+    const int64_t fit = (160 * 1024 - m * parts * 16) / (m * parts * 256);  // 13 tiles at least: 16 activations in three parts
     while (p.splits > 1 && p.splits > fit) p.splits /= 2;
     const int64_t all = ceil_div(a.tiles, p.splits), most = fit / p.splits;
     p.chunked = a.tiles > fit;

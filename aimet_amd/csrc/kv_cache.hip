@@ -728,8 +728,8 @@ __device__ __forceinline__ void finish_rows(AttendRows<T, D, NR>& rows, float* s
 // Bound by the stream of codes: keys of the next tile and values of this one are asked for before the work on this one
 // begins.  STREAM: the codes are more than the caches keep, so they are read past them.
 //
-// 131071 tokens of 8 x 128 (268 MB): 48 us, 5.6 TB/s, and 4.6 us for the join; 32 sequences of up to 4096 tokens, 8 x 128
-// (134 MB): 34 us in all; 100 tokens of 32 x 64: 4.0 us.
+// 131071 tokens of 8 x 128 (268 MB): 50 us, 5.4 TB/s, and 4.6 us for the join; 32 sequences of up to 4096 tokens, 8 x 128
+// (134 MB): 35 us in all; 100 tokens of 32 x 64: 4.3 us.
 template <typename T, int D, bool STREAM>
 __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_attend_kernel(KvAttendArgs a) {
     constexpr int kOut = D / 16;
@@ -824,7 +824,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, D <= 128 ? 2 : 1) void kv_att
 // Many rows (prompts): each wave has 16 * NR rows of its own, and the workgroup takes the token tiles one after the other
 // through two LDS buffers, turned into float16 once for all its waves; the next tile is on its way to registers while this
 // one is worked on.  Bound by the matrix cores and the vector work between the two products together.  2048 queries of
-// 3048 tokens, 2 x 8 x 4 heads of 128: 192 us, 708 TFLOP/s (of products in two parts: 1060).
+// 3048 tokens, 2 x 8 x 4 heads of 128: 192 us, 707 TFLOP/s (1060 with the second parts of the weights).
 template <typename T, int D, int NR, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void kv_prompt_kernel(KvAttendArgs a) {
     constexpr int kThreads = WAVES * kWave;
@@ -949,7 +949,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KvAttendArgs a) {
 }
 
 // The same for up to eight splits, where rows are many: D / 4 lanes to a row (1024 queries of 1 x 8 x 4 heads in two
-// splits: 37 us in all, and 69 us with a workgroup for each row).
+// splits: 32 us less than with a workgroup for each row).
 template <typename T, int D>
 __global__ __launch_bounds__(kJoinThreads) void kv_join_rows_kernel(KvAttendArgs a) {
     constexpr int kLanes = D / 4, kRows = kJoinThreads / kLanes;
@@ -1041,17 +1041,27 @@ int launch_values(const KvValuesArgs& a, int64_t bh, int32_t dim, hipStream_t s)
 // better where they fill the chip once without a split of the token axis, or where a split would cost more than it gives
 // (it writes and joins float32 sums, about the time of eight tiles).
 //   sequences x heads x groups, queries of tokens, head size   waves 0   4 in one split   8
-//   1 x 8 x 4,  64 of 4096, 128                                   22 us             94   32
-//   1 x 4 x 4, 512 of 1024, 128                                   17                29   29
-//   1 x 8 x 4, 256 of 16384, 128                                 131               356   81
-//   1 x 8 x 4, 512 of 512, 128                                    20                19   27
-//   1 x 8 x 4, 1024 of 1024, 128                                  38                30   37
-//   1 x 8 x 4, 1024 of 4096, 128                                 117                96   83
-//   1 x 8 x 4, 2048 of 2048, 128                                  91                59   70
-//   2 x 8 x 4, 2048 of 3048, 128                                 280               148  144
+//   1 x 8 x 4,  64 of 4096, 128                                   24 us            123   35
+//   1 x 4 x 4, 512 of 1024, 128                                   19                37   32
+//   1 x 8 x 4, 256 of 16384, 128                                 151               467  111
+//   1 x 8 x 4, 512 of 512, 128                                    20                22   30
+//   1 x 8 x 4, 1024 of 1024, 128                                  41                39   44
+//   1 x 8 x 4, 1024 of 4096, 128                                 135               125  107
+//   1 x 8 x 4, 2048 of 2048, 128                                 103                73   95
+//   2 x 8 x 4, 2048 of 3048, 128                                 321               196  194
+//   1 x 8 x 4,  64 of 4096, 128, float32                          22                87   27
+//   1 x 8 x 4, 1024 of 4096, 128, float32                        151               132  124
+//   1 x 8 x 4,  64 of 4096, 64                                    15                88   26
+//   1 x 8 x 4, 512 of 512, 64                                     13                16   21
+//   2 x 8 x 4, 512 of 512, 64                                     22                17   24
+//   1 x 8 x 4,  64 of 4096, 256                                   46               129   34
+//   1 x 8 x 4, 512 of 512, 256                                    58                24   32
+//   1 x 8 x 4, 1024 of 4096, 256                                 351               231  169
+// The rule is made for 128 channels.  At 256 a workgroup of kv_prompt_kernel takes 128 KB of LDS, so that one runs on a compute
+// unit and not two, and the rule is not the best: the first and the last of these rows take 46 and 231 us.
 //
-// The token axis is split until every compute unit has eight waves, which is what runs there at once, in one round of equal
-// shares with one length for all sequences; where lengths differ (and are known to the device alone) shares a third as long
+// The token axis is split until every compute unit has eight waves, which is what runs there at once with up to 128
+// channels, in one round of equal shares with one length for all sequences; where lengths differ (and are known to the device alone) shares a third as long
 // even them out.  A share is at least four tiles.
 struct AttendPlan { int32_t waves, row_tile, splits, split_tiles; };
 inline AttendPlan plan_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q) {

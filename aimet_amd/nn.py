@@ -690,6 +690,8 @@ def fold_param_quantizers(model: nn.Module):
 def pack_linears(model: nn.Module) -> int:
     """Replaces every QuantizedLinear of ``model`` that has a packed form (QuantizedLinear.pack) by it; returns how many.
     Other layers are left as they are.  Nothing is replaced before all are packed, so an error leaves the model whole.
+    Packed layers save memory and are faster for few activations; whole prompts of 16-bit activations (some hundred rows and
+    more) take about a tenth longer than the library product on folded weights (fold_param_quantizers).
     Forward hooks go over to the packed layers, and their handles still remove them.  A model that is itself a
     QuantizedLinear cannot be replaced in place and is refused."""
     if isinstance(model, QuantizedLinear):

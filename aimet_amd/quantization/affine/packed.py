@@ -2,7 +2,8 @@
 
 ``PackedWeight`` holds what a calibrated weight quantizer of at most 16 levels describes: the codes, two to a byte in the
 order the kernel reads them, and one float32 scale (and, for grids that are not symmetric, one whole zero point) per
-output channel and group of columns.  ``packed_linear`` is ``torch.nn.functional.linear`` on it, for up to 2^20 rows:
+output channel and group of columns.  ``packed_linear`` is ``torch.nn.functional.linear`` on it, for up to 2^20 rows and
+results of up to 2^22 blocks of 64 x 256 values (float32: 32 x 128):
 
     y[m, n] = sum_g scale[n, g] * sum_{k in g} x[m, k] * (code[n, k] + offset[n, g] + zero_point_shift)  +  bias[n]
 

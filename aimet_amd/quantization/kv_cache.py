@@ -160,7 +160,7 @@ class QuantizedKVCache:
     def attend(self, q: torch.Tensor, lengths: PerSequence, counts: Optional[PerSequence] = None,
                scale: Optional[float] = None) -> torch.Tensor:
         """Causal attention of the queries [batch, query_heads, queries, head_dim] (any strides; query_heads a multiple
-        of kv_heads, neighbouring query heads share a key head) over the stored tokens.  A sequence holds ``lengths``
+        of kv_heads, neighbouring query heads share a key head; fewer than 2^20 queries a key head) over the stored tokens.  A sequence holds ``lengths``
         tokens and its queries are the last ``queries`` of them (of a padded batch: its first ``counts`` queries are the
         last ``counts`` tokens): query t sees the tokens up to its own position, ``lengths - counts + t``.  Queries that
         see nothing, and those behind ``counts``, are answered with 0.  ``scale`` multiplies the scores (default

@@ -24,7 +24,7 @@ extern "C" {
  * bits of code - qmin are kept) as ahq_int4_linear reads them, ahq_int4_packed_bytes(n, k) bytes (0: bad shape; n is
  * at most 2^28, k at most 2^20).
  * ahq_int4_linear: x is [m][k] of `dtype` with rows ldx elements apart, y [m][n] with rows ldy apart, both dense along
- * the row; m is at most 2^20.  bias: n values of `dtype`, or NULL.  Products and sums are float32 with exact factors; y is
+ * the row; m is at most 2^20, and the result at most 2^22 blocks of 64 x 256 (float32 32 x 128) values.  bias: n values of `dtype`, or NULL.  Products and sums are float32 with exact factors; y is
  * rounded once.
  */
 typedef struct {
@@ -74,7 +74,7 @@ typedef struct {
 /* Queries [batch][query_heads][queries][head_dim] and their answers, strides in elements, dense along head_dim.  Query
  * head j reads cache head j / (query_heads / heads).  Sequence b holds lengths[b] tokens (limited to [0, capacity]) and
  * its first counts[b] queries are the last ones of them: query t stands at position lengths[b] - counts[b] + t and sees
- * the tokens up to its own.  Queries behind counts[b], and those that see nothing, are answered with zeros.  scale
+ * the tokens up to its own.  queries * query_heads / heads is below 2^20.  Queries behind counts[b], and those that see nothing, are answered with zeros.  scale
  * multiplies the scores. */
 typedef struct {
     int32_t dtype, query_heads, queries;
