@@ -1061,8 +1061,8 @@ int launch_values(const KvValuesArgs& a, int64_t bh, int32_t dim, hipStream_t s)
 // unit and not two, and the rule is not the best: the first and the last of these rows take 46 and 231 us.
 //
 // The token axis is split until every compute unit has eight waves, which is what runs there at once with up to 128
-// channels, in one round of equal shares with one length for all sequences; where lengths differ (and are known to the device alone) shares a third as long
-// even them out.  A share is at least four tiles.
+// channels, in one round of equal shares with one length for all sequences; where lengths differ (and are known to the
+// device alone) shares a third as long even them out.  A share is at least four tiles.
 struct AttendPlan { int32_t waves, row_tile, splits, split_tiles; };
 inline AttendPlan plan_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q) {
     const int64_t bh = (int64_t)cache->batch * cache->heads, rows = (int64_t)q->queries * (q->query_heads / cache->heads);

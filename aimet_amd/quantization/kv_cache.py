@@ -170,7 +170,8 @@ class QuantizedKVCache:
         far below a row's largest value to fewer; probabilities have
         22 bits and are off by at most 2^-35 of the row's largest one where they are small (both weighted by the scale of
         their values' block); all sums are float32, and the result is rounded once.  Values may be of any size; blocks whose
-        values are all below 2^-72 of the largest that a query sees count as up to that."""
+        values are all below 2^-72 of the largest one that the call's queries see of their sequence and head count as up to
+        that."""
         self._check(q, "q")
         heads, queries = q.shape[1], q.shape[2]
         if heads == 0 or heads % self.kv_heads:

@@ -99,7 +99,7 @@ int ahq_kv_dequantize(const ahq_kv_cache* cache, int32_t dtype, int32_t length, 
 
 /* softmax(scale * q k^T) v over the cache.  Codes are exact in both products, 16-bit queries as well (bfloat16
  * down to 2^-30 of a row's largest value); float32 queries have 22 bits, those far below a row's largest value fewer; probabilities 22 bits for queries of every type, sums are float32.  Blocks whose
- * values are all below 2^-72 of the largest that a query sees count as up to that.  The workspace (0 bytes where the token axis is not split) depends on the
+ * values are all below 2^-72 of the largest one that the call's queries see of their sequence and head count as up to that.  The workspace (0 bytes where the token axis is not split) depends on the
  * shapes and on whether the lengths are a device array, not on their values. */
 size_t ahq_kv_attend_workspace_bytes(const ahq_kv_cache* cache, const ahq_kv_queries* q);
 int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q, void* workspace, size_t workspace_bytes,
