@@ -160,18 +160,18 @@ class QuantizedKVCache:
     def attend(self, q: torch.Tensor, lengths: PerSequence, counts: Optional[PerSequence] = None,
                scale: Optional[float] = None) -> torch.Tensor:
         """Causal attention of the queries [batch, query_heads, queries, head_dim] (any strides; query_heads a multiple
-        of kv_heads, neighbouring query heads share a key head; fewer than 2^20 queries a key head) over the stored tokens.  A sequence holds ``lengths``
-        tokens and its queries are the last ``queries`` of them (of a padded batch: its first ``counts`` queries are the
-        last ``counts`` tokens): query t sees the tokens up to its own position, ``lengths - counts + t``.  Queries that
-        see nothing, and those behind ``counts``, are answered with 0.  ``scale`` multiplies the scores (default
-        1 / sqrt(head_dim)).  The result has the queries' type, shape and, where they are dense, memory layout.
+        of kv_heads, neighbouring query heads share a key head; fewer than 2^20 queries a key head) over the stored
+        tokens.  A sequence holds ``lengths`` tokens and its queries are the last ``queries`` of them (of a padded
+        batch: its first ``counts`` queries are the last ``counts`` tokens): query t sees the tokens up to its own
+        position, ``lengths - counts + t``.  Queries that see nothing, and those behind ``counts``, are answered with 0.
+        ``scale`` multiplies the scores (default 1 / sqrt(head_dim)).  The result has the queries' type, shape and,
+        where they are dense, memory layout.
 
-        16-bit queries are used as they are (bfloat16 down to 2^-30 of a row's largest value), float32 queries to 22 bits, those
-        far below a row's largest value to fewer; probabilities have
-        22 bits and are off by at most 2^-35 of the row's largest one where they are small (both weighted by the scale of
-        their values' block); all sums are float32, and the result is rounded once.  Values may be of any size; blocks whose
-        values are all below 2^-72 of the largest one that the call's queries see of their sequence and head count as up to
-        that."""
+        16-bit queries are used as they are (bfloat16 down to 2^-30 of a row's largest value), float32 queries to 22
+        bits, those far below a row's largest value to fewer; probabilities have 22 bits and are off by at most 2^-35 of
+        the row's largest one where they are small (both weighted by the scale of their values' block); all sums are
+        float32, and the result is rounded once.  Values may be of any size; blocks whose values are all below 2^-72 of
+        the largest one that the call's queries see of their sequence and head count as up to that."""
         self._check(q, "q")
         heads, queries = q.shape[1], q.shape[2]
         if heads == 0 or heads % self.kv_heads:

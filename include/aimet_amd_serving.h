@@ -24,8 +24,8 @@ extern "C" {
  * bits of code - qmin are kept) as ahq_int4_linear reads them, ahq_int4_packed_bytes(n, k) bytes (0: bad shape; n is
  * at most 2^28, k at most 2^20).
  * ahq_int4_linear: x is [m][k] of `dtype` with rows ldx elements apart, y [m][n] with rows ldy apart, both dense along
- * the row; m is at most 2^20, and the result at most 2^22 blocks of 64 x 256 (float32 32 x 128) values.  bias: n values of `dtype`, or NULL.  Products and sums are float32 with exact factors; y is
- * rounded once.
+ * the row; m is at most 2^20, and the result at most 2^22 blocks of 64 x 256 (float32 32 x 128) values.  bias: n values of
+ * `dtype`, or NULL.  Products and sums are float32 with exact factors; y is rounded once.
  */
 typedef struct {
     int64_t n, k;        /* output and input channels */
@@ -74,8 +74,8 @@ typedef struct {
 /* Queries [batch][query_heads][queries][head_dim] and their answers, strides in elements, dense along head_dim.  Query
  * head j reads cache head j / (query_heads / heads).  Sequence b holds lengths[b] tokens (limited to [0, capacity]) and
  * its first counts[b] queries are the last ones of them: query t stands at position lengths[b] - counts[b] + t and sees
- * the tokens up to its own.  queries * query_heads / heads is below 2^20.  Queries behind counts[b], and those that see nothing, are answered with zeros.  scale
- * multiplies the scores. */
+ * the tokens up to its own.  queries * query_heads / heads is below 2^20.  Queries behind counts[b], and those that see
+ * nothing, are answered with zeros.  scale multiplies the scores. */
 typedef struct {
     int32_t dtype, query_heads, queries;
     const void* q;
@@ -98,9 +98,10 @@ int ahq_kv_append(const ahq_kv_cache* cache, const ahq_kv_tokens* x, void* strea
 int ahq_kv_dequantize(const ahq_kv_cache* cache, int32_t dtype, int32_t length, void* k, void* v, void* stream);
 
 /* softmax(scale * q k^T) v over the cache.  Codes are exact in both products, 16-bit queries as well (bfloat16
- * down to 2^-30 of a row's largest value); float32 queries have 22 bits, those far below a row's largest value fewer; probabilities 22 bits for queries of every type, sums are float32.  Blocks whose
- * values are all below 2^-72 of the largest one that the call's queries see of their sequence and head count as up to that.  The workspace (0 bytes where the token axis is not split) depends on the
- * shapes and on whether the lengths are a device array, not on their values. */
+ * down to 2^-30 of a row's largest value); float32 queries have 22 bits, those far below a row's largest value fewer;
+ * probabilities 22 bits for queries of every type, sums are float32.  Blocks whose values are all below 2^-72 of the largest
+ * one that the call's queries see of their sequence and head count as up to that.  The workspace (0 bytes where the token
+ * axis is not split) depends on the shapes and on whether the lengths are a device array, not on their values. */
 size_t ahq_kv_attend_workspace_bytes(const ahq_kv_cache* cache, const ahq_kv_queries* q);
 int ahq_kv_attend(const ahq_kv_cache* cache, const ahq_kv_queries* q, void* workspace, size_t workspace_bytes,
                   void* stream);
